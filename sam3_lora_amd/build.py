@@ -5,6 +5,8 @@ import glob
 import os
 import shutil
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -14,6 +16,11 @@ SRCS = [SRC, os.path.join(PKG_DIR, "csrc", "vit_kernels.hip"), os.path.join(PKG_
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libsam3_lora_amd.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
+
+
+# packed-fp32-ops off: some forms of the packed fp32 instructions that hipcc makes of ordinary float code have given wrong
+# results on this hardware now and then; the scalar forms round the same way
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
@@ -32,17 +39,25 @@ def needs_build() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/*.hip -> sam3_lora_amd/libsam3_lora_amd.so for gfx950."""
-    if not force and not needs_build():
-        return LIB_PATH
-    cmd = [_hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
-           "-I", INCLUDE] + SRCS + ["-o", LIB_PATH + ".tmp"]
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed:\n{res.stdout}\n{res.stderr}")
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
+    """Compile csrc/*.hip -> sam3_lora_amd/libsam3_lora_amd.so for gfx950."""
+    if not force and not needs_build():
+        return LIB_PATH
+    hipcc = _hipcc()
+    with tempfile.TemporaryDirectory(prefix="sam3_lora_amd_build_") as tmp:
+        objs = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SRCS]
+        cmds = [[hipcc] + FLAGS + ["-I", INCLUDE, "-c", src, "-o", obj] for src, obj in zip(SRCS, objs)]
+        with ThreadPoolExecutor(max_workers=min(len(cmds), os.cpu_count() or 1, 8)) as pool:      # one compiler process per unit
+            list(pool.map(lambda cmd: _run(cmd, verbose), cmds))
+        _run([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared"] + objs + ["-o", LIB_PATH + ".tmp"], verbose)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
     return LIB_PATH
 
