@@ -41,6 +41,9 @@ LOSS_EXPORTS = ("sam3_loss_last_error", "sam3_mask_loss_workspace_bytes", "sam3_
 FP8_EXPORTS = ("sam3_fp8_last_error", "sam3_fp8_quantize")                 # include/sam3_fp8_amd.h
 SEG_EXPORTS = ("sam3_seg_last_error", "sam3_gn_nhwc_supported", "sam3_gn_nhwc_workspace_bytes", "sam3_gn_nhwc_fwd",
                "sam3_gn_nhwc_bwd", "sam3_rpb_bias_fwd")                                             # include/sam3_seg_amd.h
+SEQ_EXPORTS = ("sam3_seq_last_error", "sam3_seq_rms_norm_fwd", "sam3_seq_rms_norm_bwd_workspace_bytes", "sam3_seq_rms_norm_bwd",
+               "sam3_seq_rotary", "sam3_seq_attn_fwd_workspace_bytes", "sam3_seq_attn_fwd", "sam3_seq_attn_bwd_workspace_bytes",
+               "sam3_seq_attn_bwd")                                                                 # include/sam3_seq_amd.h
 FP8_E4M3, FP8_E5M2 = 0, 1
 FP8_AMAX_SLOTS = 64            # SAM3_FP8_AMAX_SLOTS
 FP8_AMAX_STRIDE = 32           # SAM3_FP8_AMAX_STRIDE: floats between two slots (one 128-byte line per slot)
@@ -191,6 +194,28 @@ def _declare(lib):
                                      c_void_p]
     lib.sam3_rpb_bias_fwd.restype = c_int
     lib.sam3_rpb_bias_fwd.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 9 + [c_void_p]
+    lib.sam3_seq_last_error.restype = c_char_p
+    lib.sam3_seq_last_error.argtypes = []
+    lib.sam3_seq_rms_norm_fwd.restype = c_int
+    lib.sam3_seq_rms_norm_fwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 6 + [c_int, c_int, c_int64, c_int, c_float,
+                                                                                           c_int, c_void_p]
+    lib.sam3_seq_rms_norm_bwd_workspace_bytes.restype = c_size_t
+    lib.sam3_seq_rms_norm_bwd_workspace_bytes.argtypes = [c_int64, c_int]
+    lib.sam3_seq_rms_norm_bwd.restype = c_int
+    lib.sam3_seq_rms_norm_bwd.argtypes = [c_void_p] * 3 + [c_int64] + [c_void_p] * 4 + [c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p]
+    strided = [c_void_p, c_int64, c_int64]                     # tensor, token stride, head stride
+    lib.sam3_seq_rotary.restype = c_int
+    lib.sam3_seq_rotary.argtypes = strided * 2 + [c_void_p] * 3 + [c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                                                                   c_int64, c_int, c_int, c_int, c_int, c_void_p]
+    lib.sam3_seq_attn_fwd_workspace_bytes.restype = c_size_t
+    lib.sam3_seq_attn_fwd_workspace_bytes.argtypes = [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]
+    shape = [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int, c_float, c_int]      # Tq, Tk, B, Hq, Hk, D, max_q, max_k, ...
+    lib.sam3_seq_attn_fwd.restype = c_int
+    lib.sam3_seq_attn_fwd.argtypes = strided * 3 + [c_void_p] * 5 + shape + [c_void_p, c_size_t, c_void_p]
+    lib.sam3_seq_attn_bwd_workspace_bytes.restype = c_size_t
+    lib.sam3_seq_attn_bwd_workspace_bytes.argtypes = [c_int64, c_int]
+    lib.sam3_seq_attn_bwd.restype = c_int
+    lib.sam3_seq_attn_bwd.argtypes = strided * 4 + [c_void_p] * 7 + shape + [c_void_p, c_size_t, c_void_p]
     lib.sam3_lora_merge.restype = c_int
     lib.sam3_lora_merge.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                     c_float, c_void_p]
@@ -224,7 +249,7 @@ def load(path: str | None = None):
             lib = ctypes.CDLL(p)
         except OSError as e:  # missing libamdhip64 etc.
             raise LoRAKernelError(f"sam3_lora_amd: cannot load {p}: {e}") from e
-        missing = [s for s in EXPORTS + VIT_EXPORTS + LOSS_EXPORTS + FP8_EXPORTS + SEG_EXPORTS if not hasattr(lib, s)]
+        missing = [s for s in EXPORTS + VIT_EXPORTS + LOSS_EXPORTS + FP8_EXPORTS + SEG_EXPORTS + SEQ_EXPORTS if not hasattr(lib, s)]
         if missing:
             raise LoRAKernelError(f"sam3_lora_amd: {p} lacks symbols {missing}")
         _declare(lib)

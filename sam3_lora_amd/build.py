@@ -12,7 +12,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 SRC = os.path.join(PKG_DIR, "csrc", "lora_kernels.hip")
 SRCS = [SRC, os.path.join(PKG_DIR, "csrc", "vit_kernels.hip"), os.path.join(PKG_DIR, "csrc", "loss_kernels.hip"),
-        os.path.join(PKG_DIR, "csrc", "fp8_kernels.hip"), os.path.join(PKG_DIR, "csrc", "seg_kernels.hip")]
+        os.path.join(PKG_DIR, "csrc", "fp8_kernels.hip"), os.path.join(PKG_DIR, "csrc", "seg_kernels.hip"),
+        os.path.join(PKG_DIR, "csrc", "seq_rows.hip"), os.path.join(PKG_DIR, "csrc", "seq_attention.hip")]
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libsam3_lora_amd.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)

@@ -1,0 +1,666 @@
+// sam3_lora_amd -- attention over packed sequences with grouped heads (gfx950): C-ABI of include/sam3_seq_amd.h.
+//
+//   o_i = sum_j p_ij v_j,   p_ij = exp(c q_i k_j - lse_i)    over the keys j that query i sees
+//   D_i = go_i o_i,  dS_ij = p_ij (go_i v_j - D_i),  gq_i = c sum_j dS_ij k_j,  gk_j = c sum_i dS_ij q_i,  gv_j = sum_i p_ij go_i
+//
+// The heads that share a key head are rows of one matrix: row r of (sequence, key head) is token r / G, head r % G of the group, so
+// one tile of keys serves the whole group, and the sums over the group in gk and gv are the sums over the rows.
+//
+// Every product is a 32 x 32 x 16 matrix instruction whose result has one row (forward, gq) or one key (gk, gv) per lane, and 16 of
+// the other index in registers: statistics of a row are a lane's own scalars, and the result turns into the second operand of the
+// next product without leaving the lane -- the sum over k runs in the order the registers hold it, and the other operand, read
+// from LDS by transposing reads, follows that order.
+#include "seq_common.inc"
+
+#include "sam3_seq_amd.h"
+
+using namespace seq;
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Attn {
+    const void *q, *k, *v, *go, *o;
+    void *out, *gq, *gk, *gv;
+    float *lse, *delta;         // [Tq, Hq]
+    const int *cu_q, *cu_k, *len_k;
+    long long q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
+    long long Tq, Tk;
+    int B, Hq, Hk, G, D, causal;
+    float scale;
+};
+
+// operand of a 32 x 32 x 16 product: lane l holds row (or column) l % 32, and 8 of the 16 k
+template <typename T> struct Frag;
+template <> struct Frag<bf16_t> { bf16x8 v; };
+template <> struct Frag<float> { float v[8]; };
+
+__device__ __forceinline__ f32x16 mma(const Frag<bf16_t>& a, const Frag<bf16_t>& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+// 32 bits: eight instructions of two k each; instruction j takes element j of both lane halves, of A and B alike
+__device__ __forceinline__ f32x16 mma(const Frag<float>& a, const Frag<float>& b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+// index along the result's register side: register i of lane half h
+__device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// eight elements of one row from global memory (zeros where `on` is false)
+__device__ __forceinline__ Frag<bf16_t> frag_global(const bf16_t* p, bool on) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (on) u = *reinterpret_cast<const uint4*>(p);
+    return Frag<bf16_t>{__builtin_bit_cast(bf16x8, u)};
+}
+__device__ __forceinline__ Frag<float> frag_global(const float* p, bool on) {
+    Frag<float> f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (on) {
+        a = *reinterpret_cast<const float4*>(p);
+        b = *reinterpret_cast<const float4*>(p + 4);
+    }
+    f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w;
+    f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
+    return f;
+}
+// registers 8 t .. 8 t + 7 of a result as the k-step t of the next product's second operand
+__device__ __forceinline__ void frag_of(Frag<bf16_t>& f, const float* p) {
+    f.v = __builtin_bit_cast(bf16x8, make_uint4(pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])));
+}
+__device__ __forceinline__ void frag_of(Frag<float>& f, const float* p) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = p[j];
+}
+
+// A tile of rows in LDS: rows of DP elements in chunks of 16 bytes, the chunks of a row permuted by f(row) so that neighbouring rows'
+// same chunk lies in different banks.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int EPC = 16 / sizeof(T);          // elements per chunk
+    static constexpr int CPR = DP / EPC;                // chunks per row
+    static constexpr int ROWB = DP * sizeof(T);
+    static __device__ __forceinline__ int f(int row) {
+        constexpr int rows_per_line = CPR >= 8 ? 1 : 8 / CPR;
+        return (row / rows_per_line) & (CPR < 8 ? CPR - 1 : 7);
+    }
+    static __device__ __forceinline__ int chunk_at(int row, int c) { return row * ROWB + ((c ^ f(row)) << 4); }
+    // k-step s (16 elements) of row `row`: elements 16 s + 8 h .. + 7
+    static __device__ __forceinline__ Frag<T> row_frag(const char* t, int row, int s, int h) {
+        Frag<T> r;
+        if constexpr (sizeof(T) == 2) {
+            r.v = *reinterpret_cast<const bf16x8*>(t + chunk_at(row, 2 * s + h));
+        } else {
+            const float4 a = *reinterpret_cast<const float4*>(t + chunk_at(row, 4 * s + 2 * h));
+            const float4 b = *reinterpret_cast<const float4*>(t + chunk_at(row, 4 * s + 2 * h + 1));
+            r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
+            r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
+        }
+        return r;
+    }
+    // the tile's transpose: lane l = column 32 dt + l % 32, k = rows row0 + reg_row order: {0..3} + 4 h and 8 + {0..3} + 4 h
+    static __device__ __forceinline__ Frag<T> col_frag(const char* t, int row0, int dt, int lane) {
+        Frag<T> r;
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            // 16 lanes read a 4 x 16 block and get its columns: lane i addresses row i / 4, elements 4 (i % 4) .. + 3
+            const int i = lane & 15, c = dt * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), off = (i & 1) * 8;
+            const int ra = row0 + 4 * h + (i >> 2), rb = ra + 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t + chunk_at(ra, c) + off));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t + chunk_at(rb, c) + off));
+            const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            r.v = __builtin_bit_cast(bf16x8, both);
+        } else {
+            const int d = dt * 32 + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                r.v[j] = *reinterpret_cast<const float*>(t + chunk_at(row0 + 4 * h + (j & 3) + 8 * (j >> 2), d >> 2) + (d & 3) * 4);
+        }
+        return r;
+    }
+};
+
+// where a sequence lies; begin / count clamped to the tensors
+struct Span {
+    long long begin;
+    int n;
+};
+__device__ __forceinline__ Span span(const int* cu, const int* len, int b, long long total) {
+    long long s = cu[b], e = len ? s + len[b] : cu[b + 1];
+    s = s < 0 ? 0 : s > total ? total : s;
+    e = e < s ? s : e > total ? total : e;
+    return Span{s, (int)(e - s)};
+}
+// rows of no sequence: [0, cu[0]) and [cu[B], total)
+struct Rest {
+    long long head, tail, n;
+    __device__ __forceinline__ long long row(long long i) const { return i < head ? i : tail + (i - head); }
+};
+__device__ __forceinline__ Rest rest(const int* cu, int B, long long total) {
+    long long s = cu[0], e = cu[B];
+    s = s < 0 ? 0 : s > total ? total : s;
+    e = e < s ? s : e > total ? total : e;
+    return Rest{s, e, s + (total - e)};
+}
+__device__ __forceinline__ int seen_keys(int token, int nq, int nk, int causal) {
+    if (!causal) return nk;
+    const long long j = (long long)token + 1 + nk - nq;
+    return j < 0 ? 0 : j > nk ? nk : (int)j;
+}
+
+// rows of one (sequence, head group) as addresses: row r -> token r / G, head kv * G + r % G
+struct Rows {
+    long long begin, st, sh;
+    int G, head0;
+    __device__ __forceinline__ long long at(int r) const {
+        const int t = r / G;
+        return (begin + t) * st + (long long)(head0 + (r - t * G)) * sh;
+    }
+};
+
+// ROWS rows (n of them there, the others zeros) of DP elements (D of them there) into LDS by 256 threads.
+// CHECK: infinities and NaN become zeros, and the answer says whether there were any.  A product over a tile that some of its rows
+// only see a part of multiplies what they do not see by zero, which a non-finite element would turn into NaN; such tiles are
+// staged with the check, and the rows that do see such an element get its effect afterwards (spoils(), add_nonfinite()).
+__device__ __forceinline__ bool finite_bits(unsigned u, bf16_t) { return (u & 0x7f80u) != 0x7f80u && (u & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ bool finite_bits(unsigned u, float) { return (u & 0x7f800000u) != 0x7f800000u; }
+__device__ __forceinline__ unsigned only_finite(unsigned u, bf16_t) {
+    return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u);
+}
+__device__ __forceinline__ unsigned only_finite(unsigned u, float) { return (u & 0x7f800000u) == 0x7f800000u ? 0u : u; }
+
+template <typename T, int DP, int ROWS, bool CHECK, typename ADDR>
+__device__ __forceinline__ bool stage(char* lds, const T* base, int n, int D, ADDR addr) {
+    typedef Tile<T, DP> L;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < (ROWS * L::CPR + 255) / 256; ++i) {
+        const int p = i * 256 + threadIdx.x, row = p / L::CPR, c = p % L::CPR;
+        if (ROWS * L::CPR % 256 && row >= ROWS) break;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (row < n && c * L::EPC < D) u = *reinterpret_cast<const uint4*>(base + addr(row) + c * L::EPC);
+        if (CHECK && !(finite_bits(u.x, T()) && finite_bits(u.y, T()) && finite_bits(u.z, T()) && finite_bits(u.w, T()))) {
+            bad = true;
+            u = make_uint4(only_finite(u.x, T()), only_finite(u.y, T()), only_finite(u.z, T()), only_finite(u.w, T()));
+        }
+        *reinterpret_cast<uint4*>(lds + L::chunk_at(row, c)) = u;
+    }
+    return bad;
+}
+// does a row hold an infinity or a NaN (rare path)
+template <typename T>
+__device__ bool spoils(const T* row, int D) {
+    bool bad = false;
+    for (int d = 0; d < D; ++d) bad |= !(fabsf(ld1(row + d)) <= 3.402823466e38f);
+    return bad;
+}
+
+// the result's registers of one 32-column block of a row, four neighbours at a time
+template <typename T>
+__device__ __forceinline__ void store_cols(T* row, const f32x16& acc, int dt, int h, int D, float mul) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = dt * 32 + 8 * g + 4 * h;
+        if (d < D) {
+            const float a = acc[4 * g] * mul, b = acc[4 * g + 1] * mul, c = acc[4 * g + 2] * mul, e = acc[4 * g + 3] * mul;
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + d) = make_uint2(pack2(a, b), pack2(c, e));
+            else *reinterpret_cast<float4*>(row + d) = make_float4(a, b, c, e);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void zero_row(T* row, int D, int lane, int lanes) {
+    for (int d = lane * 8; d < D; d += lanes * 8) {
+        Raw8<T> z;
+        const float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        z.set(f);
+        z.store(row + d);
+    }
+}
+
+// the infinities and NaN of n value rows into the results of a row that sees them: whatever their weight, they decide it
+template <typename T, int DT>
+__device__ __forceinline__ void add_nonfinite(f32x16* acc, const T* v, long long st, int n, int D, int h) {
+    for (int j = 0; j < n; ++j)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int e = d * 32 + reg_row(i, h);
+                const float x = e < D ? ld1(v + j * st + e) : 0.f;
+                if (!(fabsf(x) <= 3.402823466e38f)) acc[d][i] += x;
+            }
+}
+
+constexpr int BM = 128;      // rows of a workgroup: 4 waves of 32
+constexpr int BN = 64;       // keys of a step
+
+// ---------------------------------------------------------------------------------------------------------- forward
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attn_fwd(Attn a) {
+    typedef Tile<T, DP> L;
+    constexpr int KS = DP / 16, DT = DP / 32;
+    __shared__ __attribute__((aligned(16))) char lds[2 * BN * L::ROWB];
+    char *lk = lds, *lv = lds + BN * L::ROWB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int kv = blockIdx.y, b = blockIdx.z;
+    T* out = (T*)a.out;
+    if (b == a.B) {         // rows of no sequence
+        const Rest z = rest(a.cu_q, a.B, a.Tq);
+        for (long long i = (long long)blockIdx.x * BM + (threadIdx.x >> 3); i < z.n * a.G; i += (long long)gridDim.x * BM) {
+            for (long long r = i; r < z.n * a.G && r < (i - (threadIdx.x >> 3)) + BM; r += 32) {
+                const long long tok = z.row(r / a.G);
+                const int head = kv * a.G + (int)(r % a.G);
+                zero_row(out + (tok * a.Hq + head) * a.D, a.D, threadIdx.x & 7, 8);
+                if (a.lse && (threadIdx.x & 7) == 0) a.lse[tok * a.Hq + head] = -INFINITY;
+            }
+        }
+        return;
+    }
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, a.len_k, b, a.Tk);
+    const int R = sq.n * a.G;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G};
+    const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const float c2 = a.scale * LOG2E;
+    for (long long rr = (long long)blockIdx.x * BM; rr < R; rr += (long long)gridDim.x * BM) {
+        const int r0 = (int)rr;
+        const int row = r0 + wave * 32 + (lane & 31);
+        const bool live = row < R;
+        const int jmax = live ? seen_keys(row / a.G, sq.n, sk.n, a.causal) : 0;
+        const int last = min(r0 + BM, R) - 1;
+        const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal);      // keys that any row of the tile sees
+        const int jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);        // keys that every row of the tile sees
+        Frag<T> qf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + s * 16 + h * 8, live && s * 16 + h * 8 < a.D);
+        f32x16 acc[DT];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] = zero16();
+        float m = -INFINITY, l = 0.f;
+        for (int k0 = 0; k0 < jend; k0 += BN) {
+            __syncthreads();
+            bool bad = false;
+            stage<T, DP, BN, false>(lk, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+            const auto vrow = [&](int r) { return (long long)r * a.v_st; };
+            if (k0 + BN > jall) bad = stage<T, DP, BN, true>(lv, v + (long long)k0 * a.v_st, sk.n - k0, a.D, vrow);
+            else stage<T, DP, BN, false>(lv, v + (long long)k0 * a.v_st, sk.n - k0, a.D, vrow);
+            bad = __syncthreads_or(bad);
+            if (bad) add_nonfinite<T, DT>(acc, v + (long long)k0 * a.v_st, a.v_st, min(jmax - k0, BN), a.D, h);
+#pragma unroll
+            for (int sub = 0; sub < BN / 32; ++sub) {
+                f32x16 s = zero16();
+#pragma unroll
+                for (int i = 0; i < KS; ++i) s = mma(L::row_frag(lk, sub * 32 + (lane & 31), i, h), qf[i], s);
+                const int j0 = k0 + sub * 32;
+                float p[16];
+                float mx = m;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = j0 + reg_row(i, h) < jmax ? s[i] : -INFINITY;
+                    mx = fmaxf(mx, p[i]);
+                }
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float base = mx == -INFINITY ? 0.f : mx * c2;
+                const float alpha = exp2f(m * c2 - base);
+                m = mx;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = exp2f(p[i] * c2 - base);
+                    sum += p[i];
+                }
+                l = l * alpha + sum;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    Frag<T> pf;
+                    frag_of(pf, p + 8 * t);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lv, sub * 32 + 16 * t, d, lane), pf, acc[d]);
+                }
+            }
+        }
+        l += __shfl_xor(l, 32, 64);
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        if (live) {
+            const int t = row / a.G, head = kv * a.G + row - t * a.G;
+            T* o = out + ((sq.begin + t) * a.Hq + head) * a.D;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) store_cols(o, acc[d], d, h, a.D, inv);
+            if (a.lse && h == 0) a.lse[(sq.begin + t) * a.Hq + head] = inv == 0.f ? -INFINITY : m * a.scale + logf(l);
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------- gradient of q (and D)
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attn_gq(Attn a) {
+    typedef Tile<T, DP> L;
+    constexpr int KS = DP / 16, DT = DP / 32;
+    constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+    __shared__ __attribute__((aligned(16))) char lds[2 * BK * L::ROWB];
+    char *lk = lds, *lv = lds + BK * L::ROWB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int kv = blockIdx.y, b = blockIdx.z;
+    T* gq = (T*)a.gq;
+    if (b == a.B) {
+        const Rest z = rest(a.cu_q, a.B, a.Tq);
+        for (long long i = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); i < z.n * a.G; i += (long long)gridDim.x * 32)
+            zero_row(gq + (z.row(i / a.G) * a.Hq + kv * a.G + (int)(i % a.G)) * a.D, a.D, threadIdx.x & 7, 8);
+        return;
+    }
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
+    const int R = sq.n * a.G;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G},
+        orows{sq.begin, (long long)a.Hq * a.D, a.D, a.G, kv * a.G}, srows{sq.begin, a.Hq, 1, a.G, kv * a.G};
+    const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const float c2 = a.scale * LOG2E;
+    for (long long rr = (long long)blockIdx.x * BM; rr < R; rr += (long long)gridDim.x * BM) {
+        const int r0 = (int)rr;
+        const int row = r0 + wave * 32 + (lane & 31);
+        const bool live = row < R;
+        const int jmax = live ? seen_keys(row / a.G, sq.n, sk.n, a.causal) : 0;
+        const int jend = seen_keys((min(r0 + BM, R) - 1) / a.G, sq.n, sk.n, a.causal);
+        const int jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);
+        bool spoilt = false;        // the row sees a key that is not finite: so is its gradient
+        Frag<T> qf[KS], gf[KS];
+        float delta = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + h * 8;
+            const bool on = live && d < a.D;
+            qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + d, on);
+            gf[s] = frag_global((const T*)a.go + (live ? grows.at(row) : 0) + d, on);
+            if (on) {
+                Raw8<T> x, y;
+                float fx[8], fy[8];
+                x.load((const T*)a.o + orows.at(row) + d);
+                y.load((const T*)a.go + grows.at(row) + d);
+                x.get(fx);
+                y.get(fy);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
+            }
+        }
+        delta += __shfl_xor(delta, 32, 64);
+        if (live && h == 0) a.delta[srows.at(row)] = delta;
+        const float l2 = (live ? a.lse[srows.at(row)] : 0.f) * LOG2E;
+        f32x16 acc[DT];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] = zero16();
+        for (int k0 = 0; k0 < jend; k0 += BK) {
+            __syncthreads();
+            bool bad = false;
+            const auto krow = [&](int r) { return (long long)r * a.k_st; };
+            if (k0 + BK > jall) bad = stage<T, DP, BK, true>(lk, k + (long long)k0 * a.k_st, sk.n - k0, a.D, krow);
+            else stage<T, DP, BK, false>(lk, k + (long long)k0 * a.k_st, sk.n - k0, a.D, krow);
+            stage<T, DP, BK, false>(lv, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
+            bad = __syncthreads_or(bad);
+            if (bad)
+                for (int j = 0; j < min(jmax - k0, BK); ++j) spoilt |= spoils(k + (k0 + j) * a.k_st, a.D);
+#pragma unroll
+            for (int sub = 0; sub < BK / 32; ++sub) {
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    s = mma(L::row_frag(lk, sub * 32 + (lane & 31), i, h), qf[i], s);
+                    dp = mma(L::row_frag(lv, sub * 32 + (lane & 31), i, h), gf[i], dp);
+                }
+                float ds[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    ds[i] = k0 + sub * 32 + reg_row(i, h) < jmax ? exp2f(s[i] * c2 - l2) * (dp[i] - delta) : 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    Frag<T> f;
+                    frag_of(f, ds + 8 * t);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lk, sub * 32 + 16 * t, d, lane), f, acc[d]);
+                }
+            }
+        }
+        if (live) {
+            T* o = gq + orows.at(row);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) store_cols(o, acc[d], d, h, a.D, spoilt ? NAN : a.scale);
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------------------- gradients of k and v
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_attn_gkv(Attn a) {
+    typedef Tile<T, DP> L;
+    constexpr int KS = DP / 16, DT = DP / 32;
+    constexpr int BK = 128, BR = 32;
+    __shared__ __attribute__((aligned(16))) char lds[2 * BR * L::ROWB];
+    __shared__ __attribute__((aligned(16))) float stat[2][BR];
+    char *lq = lds, *lg = lds + BR * L::ROWB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int kv = blockIdx.y, b = blockIdx.z;
+    T *gk = (T*)a.gk, *gv = (T*)a.gv;
+    if (b == a.B) {
+        const Rest z = rest(a.cu_k, a.B, a.Tk);
+        for (long long i = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); i < z.n; i += (long long)gridDim.x * 32) {
+            zero_row(gk + (z.row(i) * a.Hk + kv) * a.D, a.D, threadIdx.x & 7, 8);
+            zero_row(gv + (z.row(i) * a.Hk + kv) * a.D, a.D, threadIdx.x & 7, 8);
+        }
+        return;
+    }
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
+    const int R = sq.n * a.G;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G},
+        srows{sq.begin, a.Hq, 1, a.G, kv * a.G};
+    const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const float c2 = a.scale * LOG2E;
+    for (long long kk = (long long)blockIdx.x * BK; kk < sk.n; kk += (long long)gridDim.x * BK) {
+        const int k0 = (int)kk;
+        const int key = k0 + wave * 32 + (lane & 31);
+        const bool live = key < sk.n;
+        Frag<T> kf[KS], vf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + h * 8;
+            kf[s] = frag_global(k + (live ? key * a.k_st : 0) + d, live && d < a.D);
+            vf[s] = frag_global(v + (live ? key * a.v_st : 0) + d, live && d < a.D);
+        }
+        f32x16 ak[DT], av[DT];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) ak[i] = zero16(), av[i] = zero16();
+        // the first token that sees this key (this tile's first key); rows before it see nothing of it
+        const long long first = a.causal ? (long long)k0 - (sk.n - sq.n) : 0;
+        const int t_first = first < 0 ? 0 : first > sq.n ? sq.n : (int)first;
+        const long long mine = a.causal ? (long long)key - (sk.n - sq.n) : 0;
+        const int t_key = live ? (mine < 0 ? 0 : mine > sq.n ? sq.n : (int)mine) : sq.n;
+        const int r_key = t_key * a.G;          // rows from here on see the key
+        const long long final = a.causal ? (long long)min(k0 + BK, sk.n) - 1 - (sk.n - sq.n) : 0;
+        const int r_all = (final < 0 ? 0 : final > sq.n ? sq.n : (int)final) * a.G;       // rows from here on see all keys of the tile
+        bool spoilt = false;                    // a row that is not finite sees the key: so are its gradients
+        for (int r0 = t_first * a.G; r0 < R; r0 += BR) {
+            __syncthreads();
+            bool bad = false;
+            const auto qrow = [&](int r) { return qrows.at(r0 + r); };
+            const auto grow = [&](int r) { return grows.at(r0 + r); };
+            if (r0 < r_all) {
+                bad = stage<T, DP, BR, true>(lq, (const T*)a.q, R - r0, a.D, qrow);
+                bad |= stage<T, DP, BR, true>(lg, (const T*)a.go, R - r0, a.D, grow);
+            } else {
+                stage<T, DP, BR, false>(lq, (const T*)a.q, R - r0, a.D, qrow);
+                stage<T, DP, BR, false>(lg, (const T*)a.go, R - r0, a.D, grow);
+            }
+            if (threadIdx.x < BR) {
+                const bool on = r0 + (int)threadIdx.x < R;
+                stat[0][threadIdx.x] = on ? a.lse[srows.at(r0 + threadIdx.x)] * LOG2E : 0.f;
+                stat[1][threadIdx.x] = on ? a.delta[srows.at(r0 + threadIdx.x)] : 0.f;
+            }
+            bad = __syncthreads_or(bad);
+            if (bad)
+                for (int r = max(r0, r_key); r < min(r0 + BR, R); ++r)
+                    spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                s = mma(L::row_frag(lq, lane & 31, i, h), kf[i], s);
+                dp = mma(L::row_frag(lg, lane & 31, i, h), vf[i], dp);
+            }
+            float p[16], ds[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = reg_row(i, h);
+                const bool sees = r0 + r >= r_key && r0 + r < R;
+                p[i] = sees ? exp2f(s[i] * c2 - stat[0][r]) : 0.f;
+                ds[i] = sees ? p[i] * (dp[i] - stat[1][r]) : 0.f;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> pf, df;
+                frag_of(pf, p + 8 * t);
+                frag_of(df, ds + 8 * t);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    av[d] = mma(L::col_frag(lg, 16 * t, d, lane), pf, av[d]);
+                    ak[d] = mma(L::col_frag(lq, 16 * t, d, lane), df, ak[d]);
+                }
+            }
+        }
+        if (live) {
+            T *ok = gk + ((sk.begin + key) * a.Hk + kv) * a.D, *ov = gv + ((sk.begin + key) * a.Hk + kv) * a.D;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                store_cols(ok, ak[d], d, h, a.D, spoilt ? NAN : a.scale);
+                store_cols(ov, av[d], d, h, a.D, spoilt ? NAN : 1.f);
+            }
+        }
+    }
+}
+
+bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+bool bad_pitch(int64_t ld, int dtype) { return (ld % (dtype == 0 ? 8 : 4)) != 0; }
+
+int check(int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, float scale, int dtype) {
+    if (dtype != 0 && dtype != 1) return sam3_seq_fail(EINVAL_, "dtype must be 0 (bf16) or 1 (fp32), got %d", dtype);
+    if (Tq < 0 || Tk < 0 || B < 0 || Hq <= 0 || Hk <= 0 || D <= 0 || max_q < 0 || max_k < 0) return sam3_seq_fail(EINVAL_, "attention: bad sizes");
+    if (Hq % Hk) return sam3_seq_fail(EINVAL_, "attention: %d query heads over %d key heads", Hq, Hk);
+    if (D % 8) return sam3_seq_fail(EINVAL_, "attention: head size must be a multiple of 8, got %d", D);
+    if (D > 128) return sam3_seq_fail(ENOTSUP_, "attention: head size at most 128, got %d", D);
+    if (B > 65000 || Hk > 65000) return sam3_seq_fail(ENOTSUP_, "attention: at most 65000 sequences and key heads");
+    if (Tq * Hq > 0x7fff0000ll || Tk > 0x7fff0000ll) return sam3_seq_fail(ENOTSUP_, "attention: too many rows");
+    if (!(scale > 0.f) || scale > 3.0e38f) return sam3_seq_fail(EINVAL_, "attention: scale must be positive and finite");
+    return 0;
+}
+int check_tensor(const char* name, const void* p, int64_t st, int64_t sh, int dtype) {
+    if (!p) return sam3_seq_fail(EINVAL_, "attention: %s is a null pointer", name);
+    if (misaligned(p) || bad_pitch(st, dtype) || bad_pitch(sh, dtype))
+        return sam3_seq_fail(EINVAL_, "attention: %s: pointer and strides must keep 16-byte accesses aligned", name);
+    return 0;
+}
+
+#define BY_HEAD(KERNEL, GRID, ST, ARGS)                                                                         \
+    do {                                                                                                        \
+        if (dtype == 0) {                                                                                       \
+            if (D <= 32) hipLaunchKernelGGL((KERNEL<bf16_t, 32>), GRID, dim3(256), 0, ST, ARGS);                 \
+            else if (D <= 64) hipLaunchKernelGGL((KERNEL<bf16_t, 64>), GRID, dim3(256), 0, ST, ARGS);            \
+            else hipLaunchKernelGGL((KERNEL<bf16_t, 128>), GRID, dim3(256), 0, ST, ARGS);                        \
+        } else {                                                                                                \
+            if (D <= 32) hipLaunchKernelGGL((KERNEL<float, 32>), GRID, dim3(256), 0, ST, ARGS);                  \
+            else if (D <= 64) hipLaunchKernelGGL((KERNEL<float, 64>), GRID, dim3(256), 0, ST, ARGS);             \
+            else hipLaunchKernelGGL((KERNEL<float, 128>), GRID, dim3(256), 0, ST, ARGS);                         \
+        }                                                                                                       \
+    } while (0)
+
+unsigned tiles(int64_t rows, int per) {
+    const int64_t t = (rows + per - 1) / per;
+    return (unsigned)(t < 1 ? 1 : t);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sam3_seq_attn_fwd_workspace_bytes(int64_t Tq, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype) {
+    (void)Tq; (void)B; (void)Hq; (void)Hk; (void)D; (void)max_q; (void)max_k; (void)dtype;
+    return 0;
+}
+
+int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                      int64_t v_st, int64_t v_sh, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, void* out,
+                      float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int causal,
+                      float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    sam3_seq_clear_error();
+    (void)workspace; (void)workspace_bytes;
+    if (int rc = check(Tq, Tk, B, Hq, Hk, D, max_q, max_k, scale, dtype)) return rc;
+    if (Tq == 0) return 0;
+    if (int rc = check_tensor("q", q, q_st, q_sh, dtype)) return rc;
+    if (Tk > 0) {
+        if (int rc = check_tensor("k", k, k_st, k_sh, dtype)) return rc;
+        if (int rc = check_tensor("v", v, v_st, v_sh, dtype)) return rc;
+    }
+    if (!cu_q || !cu_k || !out || misaligned(out)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
+    Attn a{};
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.cu_q = cu_q; a.cu_k = cu_k; a.len_k = len_k;
+    a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
+    a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
+    const int64_t longest = max_q < Tq ? max_q : Tq;
+    const dim3 grid(tiles(longest * a.G, BM), (unsigned)Hk, (unsigned)B + 1);
+    BY_HEAD(k_attn_fwd, grid, (hipStream_t)stream, a);
+    return launched("sam3_seq_attn_fwd");
+}
+
+size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq) { return Tq > 0 && Hq > 0 ? (size_t)Tq * Hq * sizeof(float) : 0; }
+
+int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                      int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const void* out, const float* lse,
+                      const int32_t* cu_q, const int32_t* cu_k, void* gq, void* gk, void* gv, int64_t Tq, int64_t Tk, int B, int Hq,
+                      int Hk, int D, int64_t max_q, int64_t max_k, int causal, float scale, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    sam3_seq_clear_error();
+    if (int rc = check(Tq, Tk, B, Hq, Hk, D, max_q, max_k, scale, dtype)) return rc;
+    if (Tq > 0) {
+        if (int rc = check_tensor("q", q, q_st, q_sh, dtype)) return rc;
+        if (int rc = check_tensor("go", go, go_st, go_sh, dtype)) return rc;
+        if (!out || !lse || !gq || misaligned(out) || misaligned(gq)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
+        if (!workspace || workspace_bytes < sam3_seq_attn_bwd_workspace_bytes(Tq, Hq))
+            return sam3_seq_fail(ENOMEM_, "attention: workspace too small: %zu < %zu", workspace_bytes, sam3_seq_attn_bwd_workspace_bytes(Tq, Hq));
+    }
+    if (Tk > 0) {
+        if (int rc = check_tensor("k", k, k_st, k_sh, dtype)) return rc;
+        if (int rc = check_tensor("v", v, v_st, v_sh, dtype)) return rc;
+        if (!gk || !gv || misaligned(gk) || misaligned(gv)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
+    }
+    if (!cu_q || !cu_k) return sam3_seq_fail(EINVAL_, "attention: null pointer");
+    Attn a{};
+    a.q = q; a.k = k; a.v = v; a.go = go; a.o = out; a.lse = (float*)lse; a.delta = (float*)workspace;
+    a.gq = gq; a.gk = gk; a.gv = gv; a.cu_q = cu_q; a.cu_k = cu_k;
+    a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh; a.go_st = go_st; a.go_sh = go_sh;
+    a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
+    const int64_t longest_q = max_q < Tq ? max_q : Tq, longest_k = max_k < Tk ? max_k : Tk;
+    if (Tq > 0) {
+        const dim3 grid(tiles(longest_q * a.G, BM), (unsigned)Hk, (unsigned)B + 1);
+        BY_HEAD(k_attn_gq, grid, (hipStream_t)stream, a);
+        if (int rc = launched("sam3_seq_attn_bwd")) return rc;
+    }
+    if (Tk > 0) {
+        const dim3 grid(tiles(longest_k, 128), (unsigned)Hk, (unsigned)B + 1);
+        BY_HEAD(k_attn_gkv, grid, (hipStream_t)stream, a);
+    }
+    return launched("sam3_seq_attn_bwd");
+}
+
+}  // extern "C"

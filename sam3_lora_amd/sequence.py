@@ -1,0 +1,408 @@
+"""
+Sequence operators around the adapted Linears: the norm, rotary positions and attention of a pre-norm block over tokens of text,
+images or video, as hand-written HIP kernels (C-ABI ``include/sam3_seq_amd.h``, ``csrc/seq_rows.hip``, ``csrc/seq_attention.hip``).
+
+  rms_norm, rms_norm_q8   root-mean-square norm with the residual's addition, differentiable; the same with an 8-bit output and
+                          its scales in front of a frozen 8-bit GEMM (the counterparts of ``vit.layer_norm`` and its fp8 image)
+  rotary_axes             rotary positions with several axes (time, height, width, ...) on q and k, differentiable (the general
+                          form of the trunk's 2-D tables, ``vit.axial_rope_table``)
+  packed_attention        attention over packed sequences of different lengths, causal or not, with grouped heads, differentiable;
+                          one token against a long cache is the same call
+
+Activations are bf16 or fp32 on an AMD GPU; there is no CPU fallback.  Calls run on the current stream of the tensors' device, never
+wait for the GPU, keep nothing between calls, and can be captured into a graph.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from functools import lru_cache
+from typing import Optional, Sequence, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _ffi
+from ._ffi import LoRAKernelError
+
+__all__ = ["rms_norm", "rms_norm_q8", "rotary_axes", "packed_attention", "FP8_E4M3", "FP8_E5M2"]
+
+FP8_E4M3, FP8_E5M2 = _ffi.FP8_E4M3, _ffi.FP8_E5M2
+_FP8_TYPES = {FP8_E4M3: torch.float8_e4m3fn, FP8_E5M2: torch.float8_e5m2}
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _check(rc: int, what: str) -> None:
+    if rc != 0:
+        raise LoRAKernelError(f"{what} failed (code {rc}): {(_ffi.load().sam3_seq_last_error() or b'').decode()}")
+
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _activation(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> int:
+    """Type code of an activation; its place and type are ``like``'s."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if like is not None and (t.device != like.device or t.dtype != like.dtype):
+        raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise LoRAKernelError(f"sam3_lora_amd: activations must be bfloat16 or float32, got {t.dtype} for {name}")
+    if not t.is_cuda:
+        raise LoRAKernelError(f"sam3_lora_amd: the sequence operators run only on an AMD GPU (got a {t.device} tensor for {name}); "
+                              "there is no CPU fallback.")
+    return _ffi.DT_BF16 if t.dtype == torch.bfloat16 else _ffi.DT_F32
+
+
+def _on(device: torch.device):
+    """The tensors' device as the current one, where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with unit stride inside a row, and its address and other strides in multiples of 16 bytes (a copy where it has not)."""
+    per = 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % per == 0 and s >= 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+# ----------------------------------------------------------------------------------------------------------- RMS norm
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    t = t.detach().reshape(-1, width)
+    t = _aligned(t)
+    return t if t.shape[0] <= 1 or t.stride(0) >= width else t.contiguous()
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _norm_fwd(x, residual, weight, eps, want_y, want_rstd, q8=None):
+    """(y, h, rstd, image, scales) of contiguous outputs; q8 = (group, fmt) or None."""
+    width = x.shape[-1]
+    x2 = _rows(x, width)
+    r2 = None if residual is None else _rows(residual, width)
+    w = _aligned(weight.detach())
+    m = x2.shape[0]
+    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)      # noqa: E731
+    y = new() if want_y else None
+    h = new() if residual is not None else None
+    rstd = torch.empty(m, dtype=torch.float32, device=x.device) if want_rstd else None
+    image = scales = None
+    group, fmt = q8 or (0, FP8_E4M3)
+    if q8 is not None:
+        image = torch.empty(x.shape, dtype=_FP8_TYPES[fmt], device=x.device)
+        scales = torch.empty(x.shape[:-1] + (width // group if group else 1,), dtype=torch.float32, device=x.device)
+    ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+    with _on(x.device):
+        _check(_ffi.load().sam3_seq_rms_norm_fwd(
+            x2.data_ptr(), _pitch(x2), ptr(r2), 0 if r2 is None else _pitch(r2), w.data_ptr(), ptr(y), ptr(h), ptr(rstd), ptr(image),
+            ptr(scales), group, fmt, m, width, eps, _ffi.DT_BF16 if x.dtype == torch.bfloat16 else _ffi.DT_F32, _stream(x.device)),
+            "sam3_seq_rms_norm_fwd")
+    return y, h, rstd, image, scales
+
+
+class _RMSNorm(torch.autograd.Function):
+    """``(y, h)``; saves the stream h (x itself without a residual) and rstd."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, h, rstd, _, _ = _norm_fwd(x, residual, weight, eps, True, True)
+        ctx.save_for_backward(x if residual is None else h, weight, rstd)
+        ctx.with_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.with_residual else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gh=None):
+        h, weight, rstd = ctx.saved_tensors
+        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        if gy is None:      # only the stream was used
+            return gh if ctx.needs_input_grad[0] else None, gh if ctx.needs_input_grad[1] else None, None, None
+        width = h.shape[-1]
+        h2, w = _rows(h, width), _aligned(weight.detach())
+        gy2 = _aligned(gy.contiguous())
+        gh2 = None if gh is None or not need_x else _aligned(gh.contiguous())
+        gx = torch.empty(h.shape, dtype=h.dtype, device=h.device) if need_x else None
+        gw = torch.empty_like(weight, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
+        m = h2.shape[0]
+        if m == 0:
+            return gx if ctx.needs_input_grad[0] else None, gx if ctx.needs_input_grad[1] else None, None if gw is None else gw.zero_(), None
+        lib = _ffi.load()
+        ws = None
+        if gw is not None:
+            ws = torch.empty(lib.sam3_seq_rms_norm_bwd_workspace_bytes(m, width), dtype=torch.uint8, device=h.device)
+        ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+        with _on(h.device):
+            _check(lib.sam3_seq_rms_norm_bwd(
+                gy2.data_ptr(), ptr(gh2), h2.data_ptr(), _pitch(h2), w.data_ptr(), rstd.data_ptr(), ptr(gx), ptr(gw), m, width,
+                _ffi.DT_BF16 if h.dtype == torch.bfloat16 else _ffi.DT_F32, ptr(ws), 0 if ws is None else ws.numel(), _stream(h.device)),
+                "sam3_seq_rms_norm_bwd")
+        return gx if ctx.needs_input_grad[0] else None, gx if ctx.needs_input_grad[1] else None, gw, None
+
+
+def _norm_args(x, weight, residual, eps):
+    _activation("x", x)
+    _activation("weight", weight, x)
+    _need(x.dim() >= 1 and weight.dim() == 1 and x.shape[-1] == weight.shape[0],
+          f"weight must have x's last dimension: got x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    _need(x.shape[-1] > 0 and x.shape[-1] % 8 == 0 and x.shape[-1] <= 16384,
+          f"the normalised dimension must be a multiple of 8 up to 16384, got {x.shape[-1]}")
+    if residual is not None:
+        _activation("residual", residual, x)
+        _need(residual.shape == x.shape, f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    _need(0.0 <= eps < 3e38, f"eps must be finite and not negative, got {eps}")
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, with ``h = x + residual``.
+
+    x, residual: [..., C] (rows may be strided), weight: [C], one type (bf16 or fp32); C a multiple of 8, at most 16384.  Returns y, or
+    ``(y, h)`` with a residual: h, rounded, is the stream that the next block adds to, and its gradient joins the norm's in one pass.
+    The statistics and y come from the unrounded fp32 h.  Differentiable in x, residual and weight.
+    """
+    _norm_args(x, weight, residual, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        return _RMSNorm.apply(x, residual, weight, eps)
+    y, h, _, _, _ = _norm_fwd(x, residual, weight, eps, True, False)
+    return y if residual is None else (y, h)
+
+
+def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6, group: int = 0,
+                fmt: int = FP8_E4M3):
+    """:func:`rms_norm` with an 8-bit output for a frozen 8-bit GEMM: ``(image, scales)``, or ``(image, scales, h)`` with a residual.
+
+    image: [..., C] ``float8_e4m3fn`` (``fmt=FP8_E5M2``: ``float8_e5m2``) of ``y / scale``; scales: fp32 [..., 1], or [..., C / group] with one
+    scale for every ``group`` (32, 64 or 128, a divisor of C) neighbouring columns.  A scale is the largest ``|y|`` of its part, at
+    least 2^-24, over the format's largest value, so nothing is clipped; y is rounded once, to 8 bits.  For inference: tensors that
+    require a gradient are refused where gradients are recorded.
+    """
+    _norm_args(x, weight, residual, eps)
+    _need(fmt in _FP8_TYPES, f"fmt must be FP8_E4M3 or FP8_E5M2, got {fmt}")
+    _need(group == 0 or (group in (32, 64, 128) and x.shape[-1] % group == 0),
+          f"group must be 0, or 32, 64 or 128 and divide {x.shape[-1]}, got {group}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        raise ValueError("rms_norm_q8 has no gradient: call it under torch.no_grad(), or rms_norm for training")
+    _, h, _, image, scales = _norm_fwd(x, residual, weight, eps, False, False, (group, fmt))
+    return (image, scales) if residual is None else (image, scales, h)
+
+
+# --------------------------------------------------------------------------------------------------- rotary positions
+@lru_cache(maxsize=256)
+def _rotation_table(sections: Tuple[int, ...], theta: float, spectrum: str):
+    """(turns per position step, axis) of each pair as the C arrays that a call reads."""
+    pairs = sum(sections)
+    two_pi = 6.283185307179586476925286766559
+    turns, axis = [], []
+    for a, n in enumerate(sections):
+        for i in range(n):
+            exponent = len(axis) / pairs if spectrum == "shared" else i / n
+            turns.append(theta ** -exponent / two_pi)
+            axis.append(a)
+    return (ctypes.c_double * pairs)(*turns), (ctypes.c_ubyte * pairs)(*axis), pairs
+
+
+def _tokens(t: torch.Tensor) -> torch.Tensor:
+    """[..., heads, D] -> [tokens, heads, D], a view where it can be, with strides that the kernel takes."""
+    return _aligned(t.detach().reshape(-1, t.shape[-2], t.shape[-1]))
+
+
+def _rotate(q, k, positions, table, halves, inverse):
+    turns, axis, pairs = table
+    q3 = _tokens(q)
+    k3 = None if k is None else _tokens(k)
+    pos = positions.reshape(positions.shape[0], -1)
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    t, hq, d = q3.shape
+    with _on(q.device):
+        _check(_ffi.load().sam3_seq_rotary(
+            q3.data_ptr(), q3.stride(0), q3.stride(1), None if k is None else k3.data_ptr(), 0 if k is None else k3.stride(0),
+            0 if k is None else k3.stride(1), qo.data_ptr(), None if k is None else ko.data_ptr(), pos.data_ptr(), pos.stride(0),
+            pos.stride(1), _POSITION_TYPES[pos.dtype], pos.shape[0], turns, axis, pairs, int(halves), int(inverse), t, hq,
+            0 if k is None else k3.shape[1], d, _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32, _stream(q.device)),
+            "sam3_seq_rotary")
+    return qo, ko
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, table, halves):
+        qo, ko = _rotate(q, k, positions, table, halves, False)
+        ctx.save_for_backward(positions)
+        ctx.table, ctx.halves = table, halves
+        ctx.set_materialize_grads(False)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk=None):
+        positions, = ctx.saved_tensors
+        gq = gq if ctx.needs_input_grad[0] else None
+        gk = gk if ctx.needs_input_grad[1] else None
+        if gq is None and gk is None:
+            return None, None, None, None, None
+        if gq is None:
+            return None, _rotate(gk, None, positions, ctx.table, ctx.halves, True)[0], None, None, None
+        return _rotate(gq, gk, positions, ctx.table, ctx.halves, True) + (None, None, None)
+
+
+def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, sections: Sequence[int], theta: float = 10000.0,
+                pairing: str = "adjacent", spectrum: str = "shared"):
+    """Rotary positions with one or several axes on the heads of q and k; returns ``(q', k')``, or q' where k is None.
+
+    q: [..., Hq, D], k: [..., Hk, D], the same leading (token) dimensions and type, any strides; D a multiple of 8, at most 256.
+    positions: [axes, ...] of the tokens' positions on each axis: int32, int64, or fp32 (fractions for interpolated grids).
+    sections: how many pairs of elements each axis turns; ``2 * sum(sections) <= D``, and the elements behind stay as they are.
+    spectrum: ``"shared"``: pair i of n in all turns by ``theta ** (-i / n)`` per step, whatever its axis; ``"per_axis"``: each axis
+    starts its own spectrum (``vit.axial_rope_table`` is ``sections=(D/4, D/4)``, per axis).
+    pairing: ``"adjacent"``: elements (2i, 2i + 1), the trunk's convention; ``"halves"``: elements (i, i + n).
+    Angles are reduced in 64 bits, so far positions keep their precision.  Differentiable in q and k.
+    """
+    _activation("q", q)
+    _need(q.dim() >= 2 and q.shape[-1] > 0 and q.shape[-1] % 8 == 0 and q.shape[-1] <= 256,
+          f"q must be [..., heads, D] with D a multiple of 8 up to 256, got {tuple(q.shape)}")
+    if k is not None:
+        _activation("k", k, q)
+        _need(k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == q.shape[-1],
+              f"k must have q's tokens and head size: got q {tuple(q.shape)}, k {tuple(k.shape)}")
+    _need(q.shape[-2] > 0 and (k is None or k.shape[-2] > 0), "q and k must have heads")
+    sections = tuple(int(n) for n in sections)
+    _need(len(sections) > 0 and all(n >= 0 for n in sections) and 0 < 2 * sum(sections) <= q.shape[-1],
+          f"sections {sections} do not fit a head of {q.shape[-1]}")
+    _need(pairing in ("adjacent", "halves"), f"pairing must be 'adjacent' or 'halves', got {pairing!r}")
+    _need(spectrum in ("shared", "per_axis"), f"spectrum must be 'shared' or 'per_axis', got {spectrum!r}")
+    theta = float(theta)
+    _need(0.0 < theta < float("inf"), f"theta must be positive and finite, got {theta}")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_TYPES:
+        raise TypeError("positions must be an int32, int64 or float32 tensor")
+    _need(positions.device == q.device and positions.shape == (len(sections),) + q.shape[:-2],
+          f"positions must be {(len(sections),) + tuple(q.shape[:-2])} on {q.device}, got {tuple(positions.shape)} on {positions.device}")
+    _need(not positions.requires_grad, "positions have no gradient")
+    table = _rotation_table(sections, theta, spectrum)
+    halves = pairing == "halves"
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryAxes.apply(q, k, positions, table, halves)
+    qo, ko = _rotate(q, k, positions, table, halves, False)
+    return qo if k is None else (qo, ko)
+
+
+# ---------------------------------------------------------------------------------------------------------- attention
+def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse):
+    tq, hq, d = q.shape
+    tk, hk = k.shape[:2]
+    q, k, v = _aligned(q.detach()), _aligned(k.detach()), _aligned(v.detach())
+    out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
+    lse = torch.empty(tq, hq, dtype=torch.float32, device=q.device) if want_lse else None
+    dt = _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32
+    lib = _ffi.load()
+    b = cu_q.numel() - 1
+    nbytes = lib.sam3_seq_attn_fwd_workspace_bytes(tq, b, hq, hk, d, max_q, max_k, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    with _on(q.device):
+        _check(lib.sam3_seq_attn_fwd(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+            cu_q.data_ptr(), cu_k.data_ptr(), None if len_k is None else len_k.data_ptr(), out.data_ptr(),
+            None if lse is None else lse.data_ptr(), tq, tk, b, hq, hk, d, max_q, max_k, int(causal), scale, dt,
+            None if ws is None else ws.data_ptr(), nbytes, _stream(q.device)), "sam3_seq_attn_fwd")
+    return out, lse
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale):
+        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, None, max_q, max_k, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.how = max_q, max_k, causal, scale
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go, _):
+        if go is None:
+            return (None,) * 9
+        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        max_q, max_k, causal, scale = ctx.how
+        tq, hq, d = q.shape
+        tk, hk = k.shape[:2]
+        q, k, v, go = (_aligned(t.detach()) for t in (q, k, v, go))
+        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        lib = _ffi.load()
+        nbytes = lib.sam3_seq_attn_bwd_workspace_bytes(tq, hq)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        with _on(q.device):
+            _check(lib.sam3_seq_attn_bwd(
+                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                go.data_ptr(), go.stride(0), go.stride(1), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+                gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq, tk, cu_q.numel() - 1, hq, hk, d, max_q, max_k, int(causal), scale,
+                _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32, ws.data_ptr(), nbytes, _stream(q.device)),
+                "sam3_seq_attn_bwd")
+        need = ctx.needs_input_grad
+        return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None) + (None,) * 6
+
+
+def _index(name: str, t: torch.Tensor, n: int, device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor")
+    _need(t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.device == device,
+          f"{name} must be a contiguous [{n}] on {device}, got {tuple(t.shape)} on {t.device}")
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: Optional[torch.Tensor] = None, *,
+                     max_q: Optional[int] = None, max_k: Optional[int] = None, len_k: Optional[torch.Tensor] = None, causal: bool = True,
+                     scale: Optional[float] = None, return_lse: bool = False):
+    """Softmax attention over sequences of different lengths that lie one behind the other; returns out [Tq, Hq, D].
+
+    q: [Tq, Hq, D], k, v: [Tk, Hk, D], one type (bf16 or fp32), any strides (views of a fused projection or of a cache); Hq a multiple
+    of Hk: head h of q reads head ``h // (Hq / Hk)`` of k and v.  D a multiple of 8, at most 128.
+    cu_q, cu_k: int32 [B + 1] on the GPU; sequence b is rows ``cu_q[b]:cu_q[b + 1]`` of q and ``cu_k[b]:cu_k[b + 1]`` of k and v
+    (cu_k None: the same rows).  Sequences may be empty.  Rows in front of the first and behind the last sequence give zeros.
+    causal: the last query of a sequence sees all its keys, the one before it all but the last, and so on; False: all see all.  A query
+    that sees no key gives zeros.  One new token per request over its cache is ``cu_q = arange(B + 1)``.
+    len_k: int32 [B], for caches with room behind each request: only the first ``len_k[b]`` of the rows from ``cu_k[b]`` count (without
+    gradients).  max_q, max_k: the longest lengths where the caller knows them: they size the launch (longer ones still come out right).
+    scale: of the scores, 1 / sqrt(D) if None.  return_lse: also the logarithm of each row's sum, fp32 [Tq, Hq], without a gradient.
+
+    Keys and values that a query does not see do not enter its result, whatever they hold.  Sums and statistics are fp32; for bf16 the
+    probabilities are rounded to bf16 for the product with v.  Gradients come out the same in every run.
+    """
+    _activation("q", q)
+    _activation("k", k, q)
+    _activation("v", v, q)
+    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.shape[2] == k.shape[2],
+          f"q must be [Tq, Hq, D] and k, v [Tk, Hk, D]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    (tq, hq, d), (tk, hk) = q.shape, k.shape[:2]
+    _need(hq > 0 and hk > 0 and hq % hk == 0, f"{hq} query heads do not share {hk} key heads")
+    _need(d > 0 and d % 8 == 0 and d <= 128, f"the head size must be a multiple of 8 up to 128, got {d}")
+    if not isinstance(cu_q, torch.Tensor) or cu_q.dim() != 1 or cu_q.numel() < 1:
+        raise TypeError("cu_q must be an int32 tensor [B + 1]")
+    n = cu_q.numel()
+    _index("cu_q", cu_q, n, q.device)
+    if cu_k is None:
+        _need(tk == tq, f"without cu_k, k and v must have q's {tq} rows, got {tk}")
+        cu_k = cu_q
+    else:
+        _index("cu_k", cu_k, n, q.device)
+    if len_k is not None:
+        _index("len_k", len_k, n - 1, q.device)
+    for name, m in (("max_q", max_q), ("max_k", max_k)):
+        _need(m is None or (isinstance(m, int) and 0 <= m < 2 ** 31), f"{name} must be a length, got {m}")
+    max_q, max_k = tq if max_q is None else max_q, tk if max_k is None else max_k
+    scale = d ** -0.5 if scale is None else float(scale)
+    _need(0.0 < scale < 3e38, f"scale must be positive and finite, got {scale}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        _need(len_k is None, "len_k has no gradient: call packed_attention under torch.no_grad()")
+        out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, bool(causal), scale)
+    else:
+        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, bool(causal), scale, return_lse)
+    return (out, lse) if return_lse else out

@@ -1,0 +1,468 @@
+"""
+Sequence operators (sam3_lora_amd/sequence.py, include/sam3_seq_amd.h) against their definitions in 64 bits.
+
+Tolerances are sums of the roundings that a result passes through.  u = finfo(type).eps / 2 is the relative error of one rounding to
+the activations' type (bf16 2^-8, fp32 2^-24), F = 2^-24 of one fp32 operation; a sum of n products in fp32 is off by at most
+(n + 1) F times the sum of the products' absolute values, whatever its order.
+"""
+import math
+
+import pytest
+import torch
+
+from sam3_lora_amd import _ffi, sequence
+from sam3_lora_amd._ffi import LoRAKernelError
+
+F = 2.0 ** -24
+DT = [torch.bfloat16, torch.float32]
+ids = lambda t: str(t).replace("torch.", "")      # noqa: E731
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rand(g, *shape, dtype, scale=1.0):
+    """Values that the type holds exactly, on the CPU in 64 bits."""
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).double()
+
+
+def close(got, want, tol, what=""):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.isfinite(got).all(), what
+    over = (got - want).abs() - tol
+    assert (over <= 0).all(), f"{what}: off by {(got - want).abs().max().item():.3e}, {int((over > 0).sum())} beyond the bound, worst by {over.max().item():.3e}"
+
+
+# ----------------------------------------------------------------------------------------------------------- refusals
+def test_header_exports_and_error_text():
+    import ctypes
+    import os
+    import re
+    from sam3_lora_amd import build
+    hdr = open(os.path.join(build.INCLUDE, "sam3_seq_amd.h")).read()
+    assert set(re.findall(r"\b(sam3_seq_[a-z_0-9]+)\s*\(", hdr)) == set(_ffi.SEQ_EXPORTS)
+    lib = _ffi.load()
+    assert lib.sam3_seq_rms_norm_bwd_workspace_bytes(0, 64) == 0 == lib.sam3_seq_rms_norm_bwd_workspace_bytes(8, 63)
+    assert lib.sam3_seq_rms_norm_bwd_workspace_bytes(3, 1024) == 1024 * 4
+    assert lib.sam3_seq_attn_bwd_workspace_bytes(5, 4) == 80
+    p = ctypes.c_void_p(64)
+
+    def norm(M=1, C=64, dtype=0, x=p, w=p, y=p, q8=None, scales=None, group=0, fmt=0, eps=1e-6, ldx=64):
+        return lib.sam3_seq_rms_norm_fwd(x, ldx, None, 0, w, y, None, None, q8, scales, group, fmt, M, C, eps, dtype, None)
+    for bad, text in ((dict(dtype=2), "dtype"), (dict(C=60), "multiples of 8"), (dict(M=-1), "sizes"), (dict(x=None), "null"), (dict(y=None), "null"),
+                      (dict(q8=p), "scales"), (dict(q8=p, scales=p, group=48), "groups"), (dict(q8=p, scales=p, fmt=3), "format"),
+                      (dict(eps=-1.0), "eps"), (dict(ldx=32), "pitch"), (dict(x=ctypes.c_void_p(68)), "aligned")):
+        assert norm(**bad) == -22, bad
+        assert text in lib.sam3_seq_last_error().decode(), (bad, lib.sam3_seq_last_error())
+    assert norm(C=16392, ldx=16392) == -95 and norm(M=0) == 0
+
+    turns, axis = (ctypes.c_double * 16)(), (ctypes.c_ubyte * 16)()
+
+    def rope(q=p, T=1, Hq=1, D=32, pairs=16, pos_type=0, axes=1, st=32, dtype=0):
+        return lib.sam3_seq_rotary(q, st, 32, None, 0, 0, p, None, p, 0, 1, pos_type, axes, turns, axis, pairs, 0, 0, T, Hq, 0, D, dtype, None)
+    for bad in (dict(q=None), dict(D=36), dict(pairs=17), dict(pairs=0), dict(pos_type=3), dict(axes=0), dict(st=33), dict(dtype=5), dict(Hq=0)):
+        assert rope(**bad) == -22, bad
+    assert rope(T=0) == 0 and rope(Hq=2000) == -95
+    axis[3] = 1
+    assert rope() == -22 and "axis" in lib.sam3_seq_last_error().decode()
+
+    def attn(q=p, B=1, Hq=4, Hk=2, D=64, Tq=8, Tk=8, scale=0.1, dtype=0, st=64, cu=p):
+        return lib.sam3_seq_attn_fwd(q, st, 64, p, 64, 64, p, 64, 64, cu, p, None, p, None, Tq, Tk, B, Hq, Hk, D, 8, 8, 1, scale, dtype, None, 0, None)
+    for bad in (dict(q=None), dict(Hk=3), dict(D=60), dict(scale=0.0), dict(scale=float("nan")), dict(dtype=2), dict(st=62), dict(cu=None), dict(Hq=0),
+                dict(Tq=-1)):
+        assert attn(**bad) == -22, bad
+    assert attn(D=136) == -95 and attn(Tq=1 << 30, Hq=4) == -95 and attn(Tq=0) == 0
+    assert lib.sam3_seq_attn_bwd(*([p, 64, 64] * 4), p, p, p, p, p, p, p, 8, 8, 1, 4, 2, 64, 8, 8, 1, 0.1, 0, None, 0, None) == -12
+
+
+def test_calls_are_refused_before_they_reach_the_gpu():
+    x, w = torch.zeros(4, 64), torch.ones(64)
+    with pytest.raises(LoRAKernelError, match="AMD GPU"):
+        sequence.rms_norm(x, w)
+    with pytest.raises(LoRAKernelError, match="bfloat16 or float32"):
+        sequence.rms_norm(x.half(), w.half())
+    with pytest.raises(LoRAKernelError, match="AMD GPU"):
+        sequence.rotary_axes(torch.zeros(2, 3, 64), None, torch.zeros(1, 2, dtype=torch.int32), (32,))
+    q = torch.zeros(4, 2, 64)
+    with pytest.raises(LoRAKernelError, match="AMD GPU"):
+        sequence.packed_attention(q, q, q, torch.tensor([0, 4], dtype=torch.int32))
+    with pytest.raises(TypeError):
+        sequence.rms_norm([1.0], w)
+
+
+@pytest.mark.gpu
+def test_arguments_are_checked():
+    dev = "cuda"
+    x, w = torch.zeros(4, 64, device=dev), torch.ones(64, device=dev)
+    for bad in (lambda: sequence.rms_norm(x, w[:32]), lambda: sequence.rms_norm(x[:, :60], w[:60]), lambda: sequence.rms_norm(x, w.bfloat16()),
+                lambda: sequence.rms_norm(x, w, residual=x[:2]), lambda: sequence.rms_norm(x, w, eps=-1.0), lambda: sequence.rms_norm(x, w.cpu()),
+                lambda: sequence.rms_norm_q8(x, w, group=16), lambda: sequence.rms_norm_q8(x, w, group=128), lambda: sequence.rms_norm_q8(x, w, fmt=7),
+                lambda: sequence.rms_norm_q8(x.clone().requires_grad_(True), w)):
+        with pytest.raises(ValueError):
+            bad()
+    q, k = torch.zeros(4, 4, 64, device=dev), torch.zeros(4, 2, 64, device=dev)
+    pos = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+    for bad in (lambda: sequence.rotary_axes(q, k, pos, (33,)), lambda: sequence.rotary_axes(q, k, pos, ()), lambda: sequence.rotary_axes(q, k, pos, (16, 16)),
+                lambda: sequence.rotary_axes(q, k[:3], pos, (32,)), lambda: sequence.rotary_axes(q, k, pos, (32,), pairing="x"),
+                lambda: sequence.rotary_axes(q, k, pos, (32,), spectrum="x"), lambda: sequence.rotary_axes(q, k, pos, (32,), theta=0.0),
+                lambda: sequence.rotary_axes(q, k, pos.cpu(), (32,)), lambda: sequence.rotary_axes(q[..., :60], k[..., :60], pos, (16,))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        sequence.rotary_axes(q, k, pos.double(), (32,))
+    cu = torch.tensor([0, 4], dtype=torch.int32, device=dev)
+    for bad in (lambda: sequence.packed_attention(q, k[:3], k[:3], cu), lambda: sequence.packed_attention(q, k, k[..., :32], cu),
+                lambda: sequence.packed_attention(q[:, :3], k, k, cu), lambda: sequence.packed_attention(q, k, k, cu, cu[:1]),
+                lambda: sequence.packed_attention(q, k, k, cu.cpu()), lambda: sequence.packed_attention(q, k, k, cu, scale=0.0),
+                lambda: sequence.packed_attention(q, k, k, cu, max_q=-1), lambda: sequence.packed_attention(q, k, k, cu, len_k=cu),
+                lambda: sequence.packed_attention(q.clone().requires_grad_(True), k, k, cu, len_k=cu[1:]),
+                lambda: sequence.packed_attention(q.bfloat16(), k, k, cu)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: sequence.packed_attention(q, k, k, cu.long()), lambda: sequence.packed_attention(q, k, k, [0, 4])):
+        with pytest.raises(TypeError):
+            bad()
+
+
+# ----------------------------------------------------------------------------------------------------------- RMS norm
+def norm_ref(x, w, r, eps, gy=None, gh=None):
+    h = x if r is None else x + r
+    rstd = (h.square().mean(-1, keepdim=True) + eps).rsqrt()
+    xhat = h * rstd
+    out = dict(h=h, y=xhat * w, xhat=xhat, rstd=rstd)
+    if gy is not None:
+        u = gy * w
+        out["mean"] = (u * xhat).mean(-1, keepdim=True)
+        out["gx"] = rstd * (u - xhat * out["mean"]) + (0 if gh is None else gh)
+        out["gw"] = (gy * xhat).sum(0)
+        out["u"] = u
+    return out
+
+
+# fp32 operations on the way to y: the sum of squares (a lane adds at most 64 of them, then 8 levels), the mean, eps, the root (2),
+# the products (3), half of the sum's part reaching y through the root
+NORM_OPS = 48
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,width", [(1, 8), (1, 1024), (3, 64), (37, 72), (130, 128), (65, 264), (5, 512), (9, 520), (33, 1024), (7, 2040),
+                                        (5, 4096), (3, 4104), (2, 6152), (3, 16384), (2050, 96)])
+def test_rms_norm_and_gradients(rows, width, residual, dtype):
+    g = gen(rows * 7 + width)
+    gain = torch.exp(0.5 * torch.randn(width, generator=g))
+    x = (torch.randn(rows, width, generator=g) * gain).to(dtype).double()
+    r = (torch.randn(rows, width, generator=g) * gain * 2).to(dtype).double() if residual else None
+    w = rand(g, width, dtype=dtype, scale=0.3) + 1
+    w = w.to(dtype).double()
+    gy, gh = rand(g, rows, width, dtype=dtype), rand(g, rows, width, dtype=dtype) if residual else None
+    ref = norm_ref(x, w, r, 1e-6, gy, gh)
+    u = unit(dtype)
+    dev = lambda t: None if t is None else t.to("cuda", dtype)      # noqa: E731
+    xs = dev(x).requires_grad_(True)
+    rs = dev(r).requires_grad_(True) if residual else None
+    ws = dev(w).requires_grad_(True)
+    got = sequence.rms_norm(xs, ws, residual=rs)
+    y = got[0] if residual else got
+    assert y.dtype == dtype
+    close(y, ref["y"], (u + NORM_OPS * F) * ref["y"].abs(), "y")
+    if residual:
+        close(got[1], ref["h"], (u + F) * ref["h"].abs(), "h")
+        grads = torch.autograd.grad(got, (xs, rs, ws), (dev(gy), dev(gh)))
+        assert torch.equal(grads[0], grads[1])
+    else:
+        grads = torch.autograd.grad(y, (xs, ws), dev(gy))
+    # the saved stream is rounded once (u, with a residual): it reaches xhat, and through the mean of u xhat the result
+    us = u if residual else 0.0
+    absmean = (ref["u"] * ref["xhat"]).abs().mean(-1, keepdim=True)
+    tol = ref["rstd"] * (2 * NORM_OPS * F * (ref["u"].abs() + ref["xhat"].abs() * absmean) + 2 * us * ref["xhat"].abs() * absmean)
+    close(grads[0], ref["gx"], tol + (u + 2 * F) * ref["gx"].abs() + 2 * F * (0 if gh is None else gh.abs()), "gx")
+    sums = (gy * ref["xhat"]).abs().sum(0)
+    close(grads[-1], ref["gw"], u * ref["gw"].abs() + (us + (rows + NORM_OPS) * F) * sums, "gw")
+    with torch.no_grad():       # without a gradient: the same kernel
+        again = sequence.rms_norm(dev(x), dev(w), residual=dev(r))
+    assert torch.equal(again[0] if residual else again, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("fmt", [sequence.FP8_E4M3, sequence.FP8_E5M2], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("rows,width,group", [(1, 32, 32), (3, 1024, 0), (17, 128, 128), (33, 64, 64), (5, 1056, 32), (2, 4224, 128), (4, 8192, 0), (129, 512, 64)])
+def test_rms_norm_q8(rows, width, group, fmt, dtype):
+    g = gen(rows + width + group)
+    x, r = rand(g, rows, width, dtype=dtype), rand(g, rows, width, dtype=dtype, scale=3)
+    if rows > 2:
+        x[1], r[1] = 0, 0                       # a row without content
+    w = rand(g, width, dtype=dtype)
+    ref = norm_ref(x, w, r, 1e-6)
+    image, scales, h = sequence.rms_norm_q8(x.to("cuda", dtype), w.to("cuda", dtype), residual=r.to("cuda", dtype), group=group, fmt=fmt)
+    close(h, ref["h"], (unit(dtype) + F) * ref["h"].abs(), "h")
+    parts = ref["y"].reshape(rows, -1, group or width)
+    top, half, tiny = (448.0, 2.0 ** -4, 2.0 ** -10) if fmt == sequence.FP8_E4M3 else (57344.0, 2.0 ** -3, 2.0 ** -17)
+    want = parts.abs().amax(-1).clamp(min=2.0 ** -24) / top
+    assert image.dtype == (torch.float8_e4m3fn if fmt == sequence.FP8_E4M3 else torch.float8_e5m2) and scales.dtype == torch.float32
+    close(scales, want, (NORM_OPS + 2) * F * want, "scales")
+    # against the scale that came out: one rounding to 8 bits (half a step of the value, or of the smallest exponent), the fp32 errors before it
+    value = parts / scales.cpu().double()[..., None]
+    back = image.cpu().float().double().reshape(parts.shape)
+    close(back, value, torch.clamp(half * value.abs(), min=tiny) * (1 + 2.0 ** -12) + (NORM_OPS + 4) * F * value.abs(), "image")
+    alone = sequence.rms_norm_q8(x.to("cuda", dtype), w.to("cuda", dtype), group=group, fmt=fmt)
+    assert len(alone) == 2
+
+
+@pytest.mark.gpu
+def test_rms_norm_rows_of_a_wider_tensor_other_shapes_and_no_rows():
+    g = gen(3)
+    big = torch.randn(6, 5, 3 * 256, generator=g).to("cuda", torch.bfloat16)
+    x, r, w = big[..., 256:512], big[..., 512:], torch.ones(256, device="cuda", dtype=torch.bfloat16)
+    y, h = sequence.rms_norm(x, w, residual=r)
+    y2, h2 = sequence.rms_norm(x.contiguous(), w, residual=r.contiguous())
+    assert y.shape == x.shape and torch.equal(y, y2) and torch.equal(h, h2)
+    odd = torch.randn(7 * 64 + 1, generator=g).to("cuda", torch.bfloat16)[1:].view(7, 64)       # not 16-byte aligned
+    assert torch.equal(sequence.rms_norm(odd, w[:64]), sequence.rms_norm(odd.clone(), w[:64]))
+    assert torch.equal(sequence.rms_norm(x[0, 0], w), y.new_tensor(sequence.rms_norm(x[:1, :1], w).tolist())[0, 0])
+    empty = torch.empty(0, 64, device="cuda", requires_grad=True)
+    wt = torch.ones(64, device="cuda", requires_grad=True)
+    out = sequence.rms_norm(empty, wt)
+    gx, gw = torch.autograd.grad(out, (empty, wt), torch.empty_like(out))
+    assert out.shape == (0, 64) and gx.shape == (0, 64) and torch.equal(gw, torch.zeros_like(gw))
+    spread = torch.randn(64, generator=g).cuda().expand(5, 64).requires_grad_(True)             # a broadcast input
+    out = sequence.rms_norm(spread, wt)
+    assert torch.equal(out, sequence.rms_norm(spread.contiguous(), wt))
+
+
+@pytest.mark.gpu
+def test_rms_norm_partial_gradients():
+    g = gen(4)
+    x, r, w = (torch.randn(*s, generator=g).cuda() for s in ((9, 64), (9, 64), (64,)))
+    gy, gh = torch.randn(9, 64, generator=g).cuda(), torch.randn(9, 64, generator=g).cuda()
+    xs = x.clone().requires_grad_(True)
+    y, h = sequence.rms_norm(xs, w, residual=r)
+    full = torch.autograd.grad((y, h), xs, (gy, gh), retain_graph=True)[0]
+    only_y = torch.autograd.grad(y, xs, gy, retain_graph=True)[0]
+    only_h = torch.autograd.grad(h, xs, gh)[0]
+    assert torch.equal(only_h, gh)
+    assert (full - (only_y + gh)).abs().max() <= 4 * F * (only_y.abs() + gh.abs()).max()
+    ws = w.clone().requires_grad_(True)
+    y, h = sequence.rms_norm(x, ws, residual=r)
+    ref = norm_ref(x.cpu().double(), w.cpu().double(), r.cpu().double(), 1e-6, gy.cpu().double())
+    close(torch.autograd.grad(y, ws, gy)[0], ref["gw"], (9 + NORM_OPS) * F * (gy.cpu().double() * ref["xhat"]).abs().sum(0), "gw")
+
+
+@pytest.mark.gpu
+def test_rms_norm_keeps_rows_apart_and_non_finite_rows_to_themselves():
+    x = torch.randn(70, 128, generator=gen(5)).cuda()
+    w = torch.ones(128, device="cuda")
+    good = sequence.rms_norm_q8(x, w)
+    bad = x.clone()
+    bad[3, 5], bad[40, 0] = float("nan"), float("inf")
+    image, scales = sequence.rms_norm_q8(bad, w)
+    keep = torch.ones(70, dtype=torch.bool)
+    keep[[3, 40]] = False
+    assert torch.equal(image.view(torch.uint8)[keep], good[0].view(torch.uint8)[keep]) and torch.equal(scales[keep], good[1][keep])
+    assert torch.isnan(image.float()[3]).all() and torch.isnan(scales[3]).all() and not torch.isfinite(image.float()[40, 0])
+
+
+# --------------------------------------------------------------------------------------------------- rotary positions
+def rope_ref(x, pos, sections, theta, pairing, spectrum, sign=1.0):
+    n = sum(sections)
+    axis = [a for a, m in enumerate(sections) for _ in range(m)]
+    rate = [theta ** (-i / n) for i in range(n)] if spectrum == "shared" else [theta ** (-i / m) for m in sections for i in range(m)]
+    angle = pos.double()[axis].movedim(0, -1) * torch.tensor(rate, dtype=torch.float64) * sign
+    cos, sin = angle.cos()[..., None, :], angle.sin()[..., None, :]
+    first = torch.arange(n) * 2 if pairing == "adjacent" else torch.arange(n)
+    second = first + 1 if pairing == "adjacent" else first + n
+    out, size = x.clone(), torch.zeros_like(x)
+    a, b = x[..., first], x[..., second]
+    out[..., first], out[..., second] = a * cos - b * sin, a * sin + b * cos
+    size[..., first] = size[..., second] = a.abs() + b.abs()
+    return out, size
+
+
+# cos and sin: the fraction of a turn is rounded to fp32 (2^-25 of half a turn: an angle of 2 pi 2^-26), the functions are good to 2 ulp;
+# then two products and a sum
+ROPE_OPS = 2 * math.pi / 4 + 4 + 3
+ROPE = [  # heads, kv heads, D, sections, pairing, spectrum
+    (1, 1, 8, (4,), "adjacent", "shared"), (3, 1, 64, (32,), "halves", "shared"), (4, 2, 64, (8, 12, 12), "adjacent", "per_axis"),
+    (16, 4, 128, (16, 24, 24), "halves", "shared"), (2, 2, 96, (7, 0, 6), "halves", "shared"), (5, 1, 40, (3, 2), "adjacent", "per_axis"),
+    (2, 1, 256, (32, 32, 32, 32), "halves", "per_axis"), (8, 8, 64, (16, 8), "halves", "per_axis"), (7, 7, 32, (5, 4, 3), "halves", "shared")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("tokens,kind", [(1, "i32"), (7, "i64"), (65, "f32"), (1030, "i32"), (4099, "f32")])
+@pytest.mark.parametrize("case", ROPE, ids=lambda c: "-".join(str(v) for v in c))
+def test_rotary_axes_and_gradients(case, tokens, kind, dtype):
+    hq, hk, d, sections, pairing, spectrum = case
+    if tokens * hq * d > 2_000_000:
+        tokens = 4099 // 8
+    g = gen(tokens + d)
+    qkv = rand(g, tokens, hq + 2 * hk, d, dtype=dtype)
+    far = torch.randint(-(1 << 20), 1 << 20, (len(sections), tokens), generator=g)
+    pos = far.int() if kind == "i32" else far * 1024 if kind == "i64" else far.float() / 64
+    fused = qkv.to("cuda", dtype).requires_grad_(True)
+    q, k = fused[:, :hq], fused[:, hq:hq + hk]
+    got = sequence.rotary_axes(q, k, pos.cuda(), sections, theta=10000.0, pairing=pairing, spectrum=spectrum)
+    go = [rand(g, tokens, n, d, dtype=dtype) for n in (hq, hk)]
+    grad = torch.autograd.grad(got, fused, [t.to("cuda", dtype) for t in go])[0]
+    u = unit(dtype)
+    for out, lo, n in ((got[0], 0, hq), (got[1], hq, hk)):
+        want, size = rope_ref(qkv[:, lo:lo + n], pos, sections, 10000.0, pairing, spectrum)
+        close(out, want, u * want.abs() + ROPE_OPS * F * size, "out")
+    for t, lo, n in ((go[0], 0, hq), (go[1], hq, hk)):
+        want, size = rope_ref(t, pos, sections, 10000.0, pairing, spectrum, -1.0)
+        close(grad[:, lo:lo + n], want, u * want.abs() + ROPE_OPS * F * size, "grad")
+    assert torch.equal(grad[:, hq + hk:], torch.zeros_like(grad[:, hq + hk:]))
+    alone = sequence.rotary_axes(q.detach(), None, pos.cuda(), sections, theta=10000.0, pairing=pairing, spectrum=spectrum)
+    assert torch.equal(alone, got[0])
+
+
+@pytest.mark.gpu
+def test_rotary_axes_matches_the_trunks_tables():
+    """The trunk's 2-D tables and kernel are one setting of the general operator."""
+    from sam3_lora_amd import vit
+    att = vit.Attention(128, 2, True, (6, 5), rope_theta=10000.0).cuda()
+    qkv = torch.randn(2, 30, 3, 2, 64, generator=gen(8)).cuda()
+    cos, sin = att._cos_sin(qkv.device)
+    q, k, _ = vit._QKVRope.apply(qkv.reshape(60, 384), cos, sin, 2, 30, 2, 64)
+    t = torch.arange(30, device="cuda")
+    pos = torch.stack([t % 6, t // 6]).int()[:, None].expand(2, 2, 30)
+    q2, k2 = sequence.rotary_axes(qkv[:, :, 0], qkv[:, :, 1], pos, (16, 16), spectrum="per_axis")
+    # both round cos and sin to fp32; the table's angles are fp32 products (up to 6 of 2^-24 of an angle up to 5)
+    assert (q - q2).abs().max() <= 40 * F * 8 and (k - k2).abs().max() <= 40 * F * 8
+
+
+@pytest.mark.gpu
+def test_rotary_axes_edges():
+    q = torch.randn(5, 2, 64, generator=gen(9)).cuda()
+    pos = torch.arange(5, device="cuda")[None]
+    assert torch.equal(sequence.rotary_axes(q, None, torch.zeros_like(pos), (32,)), q)
+    q2 = q.clone()
+    q2[2, 1, 40:] = float("inf")                # behind the turned part: copied as it is
+    out = sequence.rotary_axes(q2, None, pos, (19,))
+    assert torch.equal(out[..., 38:], q2[..., 38:]) and torch.isfinite(out[..., :38]).all()
+    out = sequence.rotary_axes(q2, None, pos, (19,), pairing="halves")
+    assert torch.equal(out[..., 38:], q2[..., 38:]) and torch.isfinite(out[..., :38]).all()
+    assert sequence.rotary_axes(q[:0], q[:0], pos[:, :0], (32,))[0].shape == (0, 2, 64)
+    odd = torch.randn(5 * 2 * 64 + 1, generator=gen(10)).cuda()[1:].view(5, 2, 64)
+    assert torch.equal(sequence.rotary_axes(odd, None, pos, (32,)), sequence.rotary_axes(odd.clone(), None, pos, (32,)))
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(sequence.rotary_axes(heads_first, None, pos, (32,)), sequence.rotary_axes(q, None, pos, (32,)))
+    qs, ks = q.clone().requires_grad_(True), q.clone().requires_grad_(True)
+    a, b = sequence.rotary_axes(qs, ks, pos, (32,))
+    assert torch.equal(torch.autograd.grad(b.sum(), ks, retain_graph=True)[0], torch.autograd.grad(a.sum(), qs)[0])
+
+
+# ---------------------------------------------------------------------------------------------------------- attention
+def attn_ref(q, k, v, lq, lk, causal, scale, u, go=None, len_k=None):
+    """Results and error bounds in 64 bits: the bounds follow the roundings named at each line."""
+    hq, hk, d = q.shape[1], k.shape[1], q.shape[2]
+    r = {n: torch.zeros_like(t) for n, t in (("o", q), ("to", q), ("gq", q), ("tgq", q), ("gk", k), ("tgk", k), ("gv", v), ("tgv", v))}
+    r["lse"] = torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+    r["tlse"] = torch.zeros(q.shape[:2], dtype=torch.float64)
+    a = b = 0
+    for i, (m, n) in enumerate(zip(lq, lk)):
+        nn = n if len_k is None else len_k[i]
+        for h in range(hq):
+            kh = h // (hq // hk)
+            Q, K, V = q[a:a + m, h], k[b:b + nn, kh], v[b:b + nn, kh]
+            seen = torch.ones(m, nn, dtype=torch.bool).tril(nn - m) if causal else torch.ones(m, nn, dtype=torch.bool)
+            s = (Q @ K.T * scale).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, 1).nan_to_num(0.0) if nn else torch.zeros(m, 0, dtype=torch.float64)
+            o = p @ V
+            # scores: a sum of d products, scale log2(e) and the maximum joined in one fused step, the exponential good to 2 ulp; both
+            # the row's sum and the weight carry it
+            es = ((d + 6) * F * (Q.abs() @ K.abs().T) * scale + 6 * F * s.abs().masked_fill(~seen, 0.0) + 4 * F).masked_fill(~seen, 0.0)
+            worst = es.amax(1, keepdim=True) if nn else es.new_zeros(m, 1)
+            ep = es + worst + (nn + 16) * F            # relative, of a weight; the sum of nn terms and its rescalings
+            to = ((ep + u) * p) @ V.abs() + (nn + 16) * F * (p @ V.abs()) + u * o.abs()      # u: the weight's rounding, the result's
+            r["o"][a:a + m, h], r["to"][a:a + m, h] = o, to
+            if nn:
+                r["lse"][a:a + m, h] = torch.logsumexp(s, 1)
+                fin = torch.isfinite(r["lse"][a:a + m, h])
+                r["tlse"][a:a + m, h] = torch.where(fin, worst[:, 0] + (nn + 16) * F + 4 * F * r["lse"][a:a + m, h].abs().masked_fill(~fin, 0.0), 0.0)
+            if go is not None:
+                G = go[a:a + m, h]
+                dp = G @ V.T
+                delta = (G * o).sum(1, keepdim=True)
+                ds = p * (dp - delta)
+                # the forward's rounded result in delta, its sum of d products, and those of dp
+                ed = (G.abs() * to).sum(1, keepdim=True) + (d + 2) * F * (G.abs() * o.abs()).sum(1, keepdim=True)
+                ep2 = 2 * ep + 4 * F                   # weights recomputed from the stored fp32 lse
+                eds = p * ((d + 2) * F * (G.abs() @ V.abs().T) + ed) + (ep2 + 4 * F) * ds.abs() + u * ds.abs()
+                r["gq"][a:a + m, h] = ds @ K * scale
+                r["tgq"][a:a + m, h] = (eds @ K.abs() + (nn + 2) * F * (ds.abs() @ K.abs())) * scale + (u + 2 * F) * r["gq"][a:a + m, h].abs()
+                rows = m * (hq // hk)
+                r["gk"][b:b + nn, kh] += ds.T @ Q * scale
+                r["tgk"][b:b + nn, kh] += (eds.T @ Q.abs() + (rows + 2) * F * (ds.abs().T @ Q.abs())) * scale
+                r["gv"][b:b + nn, kh] += p.T @ G
+                r["tgv"][b:b + nn, kh] += ((ep2 + u) * p).T @ G.abs() + (rows + 2) * F * (p.T @ G.abs())
+        a, b = a + m, b + n
+    r["tgk"] += (u + 2 * F) * r["gk"].abs()
+    r["tgv"] += (u + 2 * F) * r["gv"].abs()
+    return r
+
+
+def ends(lengths, dev="cuda"):
+    return torch.tensor([0] + list(lengths)).cumsum(0).int().to(dev)
+
+
+def check_attention(lq, lk, hq, hk, d, causal, dtype, seed=0, scale=None, train=True, hints=True, qscale=1.5):
+    g = gen(seed)
+    q = rand(g, sum(lq), hq, d, dtype=dtype, scale=qscale)
+    k, v = rand(g, sum(lk), hk, d, dtype=dtype), rand(g, sum(lk), hk, d, dtype=dtype)
+    go = rand(g, sum(lq), hq, d, dtype=dtype)
+    ref = attn_ref(q, k, v, lq, lk, causal, scale or d ** -0.5, unit(dtype), go if train else None)
+    qs, ks, vs = (t.to("cuda", dtype).requires_grad_(train) for t in (q, k, v))
+    how = dict(max_q=max(lq, default=0), max_k=max(lk, default=0)) if hints else {}
+    out, lse = sequence.packed_attention(qs, ks, vs, ends(lq), ends(lk), causal=causal, scale=scale, return_lse=True, **how)
+    close(out, ref["o"], ref["to"], "out")
+    fin = torch.isfinite(ref["lse"])
+    assert torch.equal(torch.isfinite(lse.cpu()), fin) and (lse.cpu()[~fin] == -math.inf).all()
+    close(lse.cpu()[fin], ref["lse"][fin], ref["tlse"][fin], "lse")
+    if train:
+        grads = torch.autograd.grad(out, (qs, ks, vs), go.to("cuda", dtype))
+        for n, t in zip(("gq", "gk", "gv"), grads):
+            close(t, ref[n], ref["t" + n], n)
+        again = torch.autograd.grad(sequence.packed_attention(qs, ks, vs, ends(lq), ends(lk), causal=causal, scale=scale, **how), (qs, ks, vs), go.to("cuda", dtype))
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+ATTN = [  # query lengths, key lengths, heads, kv heads, D, causal
+    ([1], [1], 1, 1, 8, True), ([2, 1, 5], [2, 1, 5], 2, 1, 32, True), ([33], [33], 1, 1, 64, True), ([64, 64], [64, 64], 4, 4, 64, True),
+    ([65, 1, 31], [65, 1, 31], 4, 2, 64, True), ([129], [129], 2, 1, 128, True), ([200, 3], [200, 3], 3, 3, 40, True),
+    ([130, 70], [130, 70], 6, 1, 96, True), ([17, 90], [17, 90], 7, 1, 128, True), ([5, 0, 9], [5, 0, 9], 2, 2, 64, True),
+    ([0, 0], [0, 0], 2, 1, 64, True), ([4], [300], 4, 2, 64, True), ([40, 3], [10, 3], 2, 1, 64, True), ([10, 5], [0, 7], 2, 1, 64, True),
+    ([100], [35], 2, 2, 128, True), ([1, 1, 1], [1, 257, 64], 8, 2, 128, True), ([3, 2], [1000, 130], 4, 1, 64, True),
+    ([70], [70], 2, 2, 64, False), ([1], [200], 2, 1, 64, False), ([150, 20], [33, 97], 4, 2, 32, False), ([64], [128], 2, 1, 128, False),
+    ([12, 0, 4], [0, 5, 9], 2, 1, 24, False), ([260], [260], 2, 1, 64, True), ([300], [300], 1, 1, 128, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("case", ATTN, ids=lambda c: "-".join(str(v).replace(" ", "") for v in c))
+def test_packed_attention_and_gradients(case, dtype):
+    check_attention(*case, dtype, seed=len(case[0]) + case[4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+def test_packed_attention_hints_and_scale(dtype):
+    check_attention([150, 40], [150, 40], 4, 2, 64, True, dtype, hints=False)
+    check_attention([50], [50], 2, 2, 64, True, dtype, scale=0.5)
+    # a hint that is too small costs time, not the result
+    g = gen(1)
+    q, k = rand(g, 300, 2, 64, dtype=dtype).to("cuda", dtype), rand(g, 300, 2, 64, dtype=dtype).to("cuda", dtype)
+    full = sequence.packed_attention(q, k, k, ends([300]))
+    assert torch.equal(sequence.packed_attention(q, k, k, ends([300]), max_q=1, max_k=300), full)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, k)]
+    a = torch.autograd.grad(sequence.packed_attention(*leaves, ends([300])), leaves, q)
+    b = torch.autograd.grad(sequence.packed_attention(*leaves, ends([300]), max_q=1, max_k=1), leaves, q)
+    assert all((x.float() - y.float()).abs().max() <= 2 * unit(dtype) * x.float().abs().max() for x, y in zip(a, b))
