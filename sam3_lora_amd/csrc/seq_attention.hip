@@ -246,105 +246,201 @@ __device__ __forceinline__ void add_nonfinite(f32x16* acc, const T* v, long long
 }
 
 constexpr int BM = 128;      // rows of a workgroup: 4 waves of 32
-constexpr int BN = 64;       // keys of a step
+
+// Which (sequence, key head) and which of its tiles a workgroup takes.  Workgroups go round the 8 XCDs in turn, and each XCD has its own
+// L2: the tiles of one pair, which read the same keys, stay on one XCD where the number of pairs is a multiple of 8, and on 2, 4 or 8
+// of them otherwise, so that all are busy.  The last tiles of a causal sequence have the most keys and go first.
+struct Place {
+    int pair, tile;
+};
+__host__ __device__ inline int xcds_per_pair(int pairs) { return pairs % 8 == 0 ? 1 : pairs % 4 == 0 ? 2 : pairs % 2 == 0 ? 4 : 8; }
+__host__ __device__ inline long long places(int pairs, int tiles) {
+    const int s = xcds_per_pair(pairs);
+    return (long long)pairs * ((tiles + s - 1) / s) * s;
+}
+__device__ __forceinline__ Place place(unsigned id, int pairs, int tiles) {
+    const int s = xcds_per_pair(pairs), lanes = 8 / s, per = (tiles + s - 1) / s;
+    const int xcd = id & 7, slot = id >> 3;
+    const int tile = (slot % per) * s + xcd / lanes;
+    return Place{xcd % lanes + lanes * (slot / per), tiles - 1 - tile};        // tile < 0: none
+}
+
+// 16 bytes per lane straight into LDS: lane l's go to lds + 16 l.  The instruction is written out because the compiler would wait for
+// every such load before any later read of LDS, and the loads of the next tile have to stay in flight; whoever reads waits at the
+// barrier in front (vmcnt(0)).
+__device__ __forceinline__ void load_to_lds(const void* p, char* lds) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
+}
+// A tile of whole rows into LDS by 256 threads without passing through registers.  The chunks' permutation is on the address that a
+// lane reads; chunks behind the head's end are left alone (they were cleared once).
+template <typename T, int DP, int ROWS>
+struct Dma {
+    typedef Tile<T, DP> L;
+    static constexpr int RPI = 256 / L::CPR;        // rows of one round of the workgroup
+    static constexpr int N = ROWS / RPI;
+    static_assert(ROWS % RPI == 0 && (RPI % 8 == 0 || N == 1), "the permutation must not depend on the round");
+    long long off;      // bytes from the tile's first row
+    bool on;
+    __device__ __forceinline__ Dma(long long st, int D) {
+        const int row = threadIdx.x / L::CPR, c = (threadIdx.x % L::CPR) ^ L::f(row);
+        off = ((long long)row * st + c * L::EPC) * (long long)sizeof(T);
+        on = c * L::EPC < D;
+    }
+    __device__ __forceinline__ void load(const T* tile, long long st, char* lds) const {
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                load_to_lds(reinterpret_cast<const char*>(tile + i * RPI * st) + off, lds + i * 4096 + (threadIdx.x >> 6) * 1024);
+        }
+    }
+};
 
 // ---------------------------------------------------------------------------------------------------------- forward
+// One pass over the keys with a running maximum and sum per row.  The maximum in use only follows when a row's new one is 2^8 above
+// it: weights stay below 2^8 (their relative precision does not change), and the accumulators are hardly ever rescaled.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attn_fwd(Attn a) {
+struct FwdCfg {
+    static constexpr int BN = sizeof(T) * DP > 256 ? 32 : 64;       // keys of a step
+};
+
+template <typename T, int DP, int BN>
+struct FwdState {
     typedef Tile<T, DP> L;
-    constexpr int KS = DP / 16, DT = DP / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BN * L::ROWB];
-    char *lk = lds, *lv = lds + BN * L::ROWB;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int kv = blockIdx.y, b = blockIdx.z;
-    T* out = (T*)a.out;
-    if (b == a.B) {         // rows of no sequence
-        const Rest z = rest(a.cu_q, a.B, a.Tq);
-        for (long long i = (long long)blockIdx.x * BM + (threadIdx.x >> 3); i < z.n * a.G; i += (long long)gridDim.x * BM) {
-            for (long long r = i; r < z.n * a.G && r < (i - (threadIdx.x >> 3)) + BM; r += 32) {
-                const long long tok = z.row(r / a.G);
-                const int head = kv * a.G + (int)(r % a.G);
-                zero_row(out + (tok * a.Hq + head) * a.D, a.D, threadIdx.x & 7, 8);
-                if (a.lse && (threadIdx.x & 7) == 0) a.lse[tok * a.Hq + head] = -INFINITY;
+    static constexpr int KS = DP / 16, DT = DP / 32, SUBS = BN / 32;
+    Frag<T> qf[KS];
+    f32x16 acc[DT];
+    float base, l;      // exponent base in powers of two, this half-wave's part of the sum
+
+    template <bool MASK>
+    __device__ __forceinline__ void step(const char* lk, const char* lv, int lane, float c2, int left) {
+        const int h = lane >> 5;
+        f32x16 s[SUBS];
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub) {
+            s[sub] = zero16();
+#pragma unroll
+            for (int i = 0; i < KS; ++i) s[sub] = mma(L::row_frag(lk, sub * 32 + (lane & 31), i, h), qf[i], s[sub]);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (MASK && sub * 32 + reg_row(i, h) >= left) s[sub][i] = -INFINITY;
+                mx = fmaxf(mx, s[sub][i]);
             }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
+        if (__any(mx > base + 8.f)) {
+            const float next = fmaxf(base, mx), alpha = __builtin_amdgcn_exp2f(base - next);
+            base = next;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub) {
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(s[sub][i], c2, -base));
+                l += p[i];
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> pf;
+                frag_of(pf, p + 8 * t);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lv, sub * 32 + 16 * t, d, lane), pf, acc[d]);
+            }
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void k_attn_fwd(Attn a, int tiles, unsigned first_rest) {
+    typedef Tile<T, DP> L;
+    constexpr int BN = FwdCfg<T, DP>::BN, TB = BN * L::ROWB;
+    constexpr int KS = DP / 16, DT = DP / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TB];        // two tiles of keys and values
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    T* out = (T*)a.out;
+    if (blockIdx.x >= first_rest) {         // rows of no sequence
+        const Rest z = rest(a.cu_q, a.B, a.Tq);
+        for (long long i = (long long)(blockIdx.x - first_rest) * 32 + (threadIdx.x >> 3); i < z.n * a.Hq; i += (long long)(gridDim.x - first_rest) * 32) {
+            const long long r = z.row(i / a.Hq) * a.Hq + i % a.Hq;
+            zero_row(out + r * a.D, a.D, threadIdx.x & 7, 8);
+            if (a.lse && (threadIdx.x & 7) == 0) a.lse[r] = -INFINITY;
         }
         return;
     }
+    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    if (pl.tile < 0) return;
+    const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, a.len_k, b, a.Tk);
     const int R = sq.n * a.G;
+    if ((long long)pl.tile * BM >= R) return;
     const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G};
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
     const float c2 = a.scale * LOG2E;
-    for (long long rr = (long long)blockIdx.x * BM; rr < R; rr += (long long)gridDim.x * BM) {
+    const Dma<T, DP, BN> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    if (a.D < DP) {
+        for (int i = threadIdx.x; i < 4 * TB / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    for (long long rr = (long long)pl.tile * BM; rr < R; rr += (long long)tiles * BM) {
         const int r0 = (int)rr;
         const int row = r0 + wave * 32 + (lane & 31);
         const bool live = row < R;
         const int jmax = live ? seen_keys(row / a.G, sq.n, sk.n, a.causal) : 0;
         const int last = min(r0 + BM, R) - 1;
-        const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal);      // keys that any row of the tile sees
-        const int jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);        // keys that every row of the tile sees
-        Frag<T> qf[KS];
+        const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal);           // keys that any row of the tile sees
+        const int jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);             // keys that every row of the tile sees
+        const int jwave = r0 + wave * 32 < R ? seen_keys(min(r0 + wave * 32 + 31, last) / a.G, sq.n, sk.n, a.causal) : 0;
+        FwdState<T, DP, BN> st;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
-            qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + s * 16 + h * 8, live && s * 16 + h * 8 < a.D);
-        f32x16 acc[DT];
+            st.qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + s * 16 + h * 8, live && s * 16 + h * 8 < a.D);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i] = zero16();
-        float m = -INFINITY, l = 0.f;
-        for (int k0 = 0; k0 < jend; k0 += BN) {
+        for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
+        st.base = -3.0e38f;
+        st.l = 0.f;
+        const int nfull = jall / BN;        // steps whose keys are all there and all seen: no mask, and loaded while the one before computes
+        if (nfull > 0) {
             __syncthreads();
-            bool bad = false;
-            stage<T, DP, BN, false>(lk, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
-            const auto vrow = [&](int r) { return (long long)r * a.v_st; };
-            if (k0 + BN > jall) bad = stage<T, DP, BN, true>(lv, v + (long long)k0 * a.v_st, sk.n - k0, a.D, vrow);
-            else stage<T, DP, BN, false>(lv, v + (long long)k0 * a.v_st, sk.n - k0, a.D, vrow);
-            bad = __syncthreads_or(bad);
-            if (bad) add_nonfinite<T, DT>(acc, v + (long long)k0 * a.v_st, a.v_st, min(jmax - k0, BN), a.D, h);
-#pragma unroll
-            for (int sub = 0; sub < BN / 32; ++sub) {
-                f32x16 s = zero16();
-#pragma unroll
-                for (int i = 0; i < KS; ++i) s = mma(L::row_frag(lk, sub * 32 + (lane & 31), i, h), qf[i], s);
-                const int j0 = k0 + sub * 32;
-                float p[16];
-                float mx = m;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    p[i] = j0 + reg_row(i, h) < jmax ? s[i] : -INFINITY;
-                    mx = fmaxf(mx, p[i]);
+            dk.load(k, a.k_st, lds);
+            dv.load(v, a.v_st, lds + TB);
+            for (int t = 0; t < nfull; ++t) {
+                char* now = lds + (t & 1) * 2 * TB;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();            // tile t is there, and nobody reads the other buffer any more
+                if (t + 1 < nfull) {
+                    char* next = lds + ((t + 1) & 1) * 2 * TB;
+                    dk.load(k + (long long)(t + 1) * BN * a.k_st, a.k_st, next);
+                    dv.load(v + (long long)(t + 1) * BN * a.v_st, a.v_st, next + TB);
                 }
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float base = mx == -INFINITY ? 0.f : mx * c2;
-                const float alpha = exp2f(m * c2 - base);
-                m = mx;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    p[i] = exp2f(p[i] * c2 - base);
-                    sum += p[i];
-                }
-                l = l * alpha + sum;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    Frag<T> pf;
-                    frag_of(pf, p + 8 * t);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lv, sub * 32 + 16 * t, d, lane), pf, acc[d]);
-                }
+                st.template step<false>(now, now + TB, lane, c2, BN);
             }
         }
-        l += __shfl_xor(l, 32, 64);
+        for (int k0 = nfull * BN; k0 < jend; k0 += BN) {
+            __syncthreads();
+            stage<T, DP, BN, false>(lds, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+            bool bad = stage<T, DP, BN, true>(lds + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
+            bad = __syncthreads_or(bad);
+            if (k0 < jwave) st.template step<true>(lds, lds + TB, lane, c2, jmax - k0);
+            if (bad) add_nonfinite<T, DT>(st.acc, v + (long long)k0 * a.v_st, a.v_st, min(jmax - k0, BN), a.D, h);
+        }
+        const float l = st.l + __shfl_xor(st.l, 32, 64);
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         if (live) {
             const int t = row / a.G, head = kv * a.G + row - t * a.G;
-            T* o = out + ((sq.begin + t) * a.Hq + head) * a.D;
+            const long long at = (sq.begin + t) * a.Hq + head;
+            T* o = out + at * a.D;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) store_cols(o, acc[d], d, h, a.D, inv);
-            if (a.lse && h == 0) a.lse[(sq.begin + t) * a.Hq + head] = inv == 0.f ? -INFINITY : m * a.scale + logf(l);
+            for (int d = 0; d < DT; ++d) store_cols(o, st.acc[d], d, h, a.D, inv);
+            if (a.lse && h == 0) a.lse[at] = inv == 0.f ? -INFINITY : st.base * LN2 + logf(l);
         }
     }
 }
@@ -560,6 +656,7 @@ int check(int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, i
     if (Hq % Hk) return sam3_seq_fail(EINVAL_, "attention: %d query heads over %d key heads", Hq, Hk);
     if (D % 8) return sam3_seq_fail(EINVAL_, "attention: head size must be a multiple of 8, got %d", D);
     if (D > 128) return sam3_seq_fail(ENOTSUP_, "attention: head size at most 128, got %d", D);
+    if ((int64_t)B * Hk > 0x7ffffff) return sam3_seq_fail(ENOTSUP_, "attention: too many sequences and heads");
     if (B > 65000 || Hk > 65000) return sam3_seq_fail(ENOTSUP_, "attention: at most 65000 sequences and key heads");
     if (Tq * Hq > 0x7fff0000ll || Tk > 0x7fff0000ll) return sam3_seq_fail(ENOTSUP_, "attention: too many rows");
     if (!(scale > 0.f) || scale > 3.0e38f) return sam3_seq_fail(EINVAL_, "attention: scale must be positive and finite");
@@ -572,16 +669,18 @@ int check_tensor(const char* name, const void* p, int64_t st, int64_t sh, int dt
     return 0;
 }
 
-#define BY_HEAD(KERNEL, GRID, ST, ARGS)                                                                         \
+constexpr unsigned REST = 32;       // workgroups that clear the rows of no sequence (mostly there are none)
+
+#define BY_HEAD(KERNEL, GRID, ST, ...)                                                                         \
     do {                                                                                                        \
         if (dtype == 0) {                                                                                       \
-            if (D <= 32) hipLaunchKernelGGL((KERNEL<bf16_t, 32>), GRID, dim3(256), 0, ST, ARGS);                 \
-            else if (D <= 64) hipLaunchKernelGGL((KERNEL<bf16_t, 64>), GRID, dim3(256), 0, ST, ARGS);            \
-            else hipLaunchKernelGGL((KERNEL<bf16_t, 128>), GRID, dim3(256), 0, ST, ARGS);                        \
+            if (D <= 32) hipLaunchKernelGGL((KERNEL<bf16_t, 32>), GRID, dim3(256), 0, ST, __VA_ARGS__);                 \
+            else if (D <= 64) hipLaunchKernelGGL((KERNEL<bf16_t, 64>), GRID, dim3(256), 0, ST, __VA_ARGS__);            \
+            else hipLaunchKernelGGL((KERNEL<bf16_t, 128>), GRID, dim3(256), 0, ST, __VA_ARGS__);                        \
         } else {                                                                                                \
-            if (D <= 32) hipLaunchKernelGGL((KERNEL<float, 32>), GRID, dim3(256), 0, ST, ARGS);                  \
-            else if (D <= 64) hipLaunchKernelGGL((KERNEL<float, 64>), GRID, dim3(256), 0, ST, ARGS);             \
-            else hipLaunchKernelGGL((KERNEL<float, 128>), GRID, dim3(256), 0, ST, ARGS);                         \
+            if (D <= 32) hipLaunchKernelGGL((KERNEL<float, 32>), GRID, dim3(256), 0, ST, __VA_ARGS__);                  \
+            else if (D <= 64) hipLaunchKernelGGL((KERNEL<float, 64>), GRID, dim3(256), 0, ST, __VA_ARGS__);             \
+            else hipLaunchKernelGGL((KERNEL<float, 128>), GRID, dim3(256), 0, ST, __VA_ARGS__);                         \
         }                                                                                                       \
     } while (0)
 
@@ -618,8 +717,11 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest = max_q < Tq ? max_q : Tq;
-    const dim3 grid(tiles(longest * a.G, BM), (unsigned)Hk, (unsigned)B + 1);
-    BY_HEAD(k_attn_fwd, grid, (hipStream_t)stream, a);
+    const int nt = (int)tiles(longest * a.G, BM);
+    const long long first_rest = places(B * Hk, nt);
+    if (first_rest > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+    const dim3 grid((unsigned)first_rest + REST);
+    BY_HEAD(k_attn_fwd, grid, (hipStream_t)stream, a, nt, (unsigned)first_rest);
     return launched("sam3_seq_attn_fwd");
 }
 
