@@ -60,23 +60,23 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
  *   n = len_k[b], or cu_k[b+1] - cu_k[b] where len_k is NULL (int32, device; values outside the tensors are clamped to them).
  *   causal: query i of n_q sees the keys j <= i + n - n_q (the last query sees all); otherwise every key.
  *   out [Tq, Hq, D] contiguous;  lse [Tq, Hq] fp32 (natural logarithm; NULL: not wanted).  A row that sees no key gives zeros and
- *   lse = -inf, and so do rows of no sequence.
+ *   lse = -inf, and so do rows of no sequence.  stats [Tq, Hq, 2] fp32 is what the backward takes (NULL: not wanted).
  * max_q, max_k: the longest lengths if known (they size the grid; longer sequences are still computed), or Tq and Tk.
  * Key and value rows that a query does not see never enter its result, whatever they hold.
  */
 size_t sam3_seq_attn_fwd_workspace_bytes(int64_t Tq, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype);
 int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                       int64_t v_st, int64_t v_sh, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, void* out,
-                      float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int causal,
+                      float* lse, float* stats, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int causal,
                       float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Its gradients, each sum in a fixed order: gq [Tq, Hq, D], gk, gv [Tk, Hk, D] contiguous, from go [Tq, Hq, D] (strides as q's), out and
- * lse of the forward (contiguous) and the forward's inputs.  Rows of no sequence get zeros.  The workspace holds fp32 [Tq, Hq].
+ * stats of the forward (contiguous) and the forward's inputs.  Rows of no sequence get zeros.  The workspace holds fp32 [Tq, Hq].
  */
 size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq);
 int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
-                      int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const void* out, const float* lse,
+                      int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const void* out, const float* stats,
                       const int32_t* cu_q, const int32_t* cu_k, void* gq, void* gk, void* gv, int64_t Tq, int64_t Tk, int B, int Hq,
                       int Hk, int D, int64_t max_q, int64_t max_k, int causal, float scale, int dtype, void* workspace,
                       size_t workspace_bytes, void* stream);

@@ -211,7 +211,7 @@ def _declare(lib):
     lib.sam3_seq_attn_fwd_workspace_bytes.argtypes = [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]
     shape = [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int, c_float, c_int]      # Tq, Tk, B, Hq, Hk, D, max_q, max_k, ...
     lib.sam3_seq_attn_fwd.restype = c_int
-    lib.sam3_seq_attn_fwd.argtypes = strided * 3 + [c_void_p] * 5 + shape + [c_void_p, c_size_t, c_void_p]
+    lib.sam3_seq_attn_fwd.argtypes = strided * 3 + [c_void_p] * 6 + shape + [c_void_p, c_size_t, c_void_p]
     lib.sam3_seq_attn_bwd_workspace_bytes.restype = c_size_t
     lib.sam3_seq_attn_bwd_workspace_bytes.argtypes = [c_int64, c_int]
     lib.sam3_seq_attn_bwd.restype = c_int

@@ -12,6 +12,8 @@
 // from LDS by transposing reads, follows that order.
 #include "seq_common.inc"
 
+#include <type_traits>
+
 #include "sam3_seq_amd.h"
 
 using namespace seq;
@@ -30,6 +32,7 @@ struct Attn {
     const void *q, *k, *v, *go, *o;
     void *out, *gq, *gk, *gv;
     float *lse, *delta;         // [Tq, Hq]
+    float2* stats;              // [Tq, Hq]: exponent base (powers of two) and 1 / sum of each row; 0 for a row that sees no key
     const int *cu_q, *cu_k, *len_k;
     long long q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
     long long Tq, Tk;
@@ -270,7 +273,7 @@ __device__ __forceinline__ Place place(unsigned id, int pairs, int tiles) {
 // barrier in front (vmcnt(0)).
 __device__ __forceinline__ void load_to_lds(const void* p, char* lds) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory", "m0");
 }
 // A tile of whole rows into LDS by 256 threads without passing through registers.  The chunks' permutation is on the address that a
 // lane reads; chunks behind the head's end are left alone (they were cleared once).
@@ -440,54 +443,108 @@ __global__ __launch_bounds__(256, 2) void k_attn_fwd(Attn a, int tiles, unsigned
             T* o = out + at * a.D;
 #pragma unroll
             for (int d = 0; d < DT; ++d) store_cols(o, st.acc[d], d, h, a.D, inv);
+            if (a.stats && h == 0) a.stats[at] = make_float2(st.base, inv);
             if (a.lse && h == 0) a.lse[at] = inv == 0.f ? -INFINITY : st.base * LN2 + logf(l);
         }
     }
 }
 
 // -------------------------------------------------------------------------------------------------- gradient of q (and D)
+// The forward's layout with two scores per key: s = q k and go v.  The weights keep the forward's exponent base and stay unnormalised;
+// the row's 1 / sum goes into the result with the scale, so what the base lost in rounding cancels as it does in the forward.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attn_gq(Attn a) {
+struct GqCfg {
+    static constexpr int BN = sizeof(T) * DP > 256 ? 32 : 64;
+};
+
+template <typename T, int DP, int BN>
+struct GqState {
     typedef Tile<T, DP> L;
+    static constexpr int KS = DP / 16, DT = DP / 32;
+    Frag<T> qf[KS], gf[KS];
+    f32x16 acc[DT];
+    float base, delta;
+
+    template <bool MASK>
+    __device__ __forceinline__ void step(const char* lk, const char* lv, int lane, float c2, int left) {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int sub = 0; sub < BN / 32; ++sub) {
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                s = mma(L::row_frag(lk, sub * 32 + (lane & 31), i, h), qf[i], s);
+                dp = mma(L::row_frag(lv, sub * 32 + (lane & 31), i, h), gf[i], dp);
+            }
+            float ds[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -base)) * (dp[i] - delta);
+                if (MASK && sub * 32 + reg_row(i, h) >= left) ds[i] = 0.f;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag<T> f;
+                frag_of(f, ds + 8 * t);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lk, sub * 32 + 16 * t, d, lane), f, acc[d]);
+            }
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void k_attn_gq(Attn a, int tiles, unsigned first_rest) {
+    typedef Tile<T, DP> L;
+    constexpr int BN = GqCfg<T, DP>::BN, TB = BN * L::ROWB;
     constexpr int KS = DP / 16, DT = DP / 32;
-    constexpr int BK = sizeof(T) == 2 ? 64 : 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BK * L::ROWB];
-    char *lk = lds, *lv = lds + BK * L::ROWB;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int kv = blockIdx.y, b = blockIdx.z;
     T* gq = (T*)a.gq;
-    if (b == a.B) {
+    if (blockIdx.x >= first_rest) {
         const Rest z = rest(a.cu_q, a.B, a.Tq);
-        for (long long i = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); i < z.n * a.G; i += (long long)gridDim.x * 32)
-            zero_row(gq + (z.row(i / a.G) * a.Hq + kv * a.G + (int)(i % a.G)) * a.D, a.D, threadIdx.x & 7, 8);
+        for (long long i = (long long)(blockIdx.x - first_rest) * 32 + (threadIdx.x >> 3); i < z.n * a.Hq; i += (long long)(gridDim.x - first_rest) * 32)
+            zero_row(gq + (z.row(i / a.Hq) * a.Hq + i % a.Hq) * a.D, a.D, threadIdx.x & 7, 8);
         return;
     }
+    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    if (pl.tile < 0) return;
+    const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
     const int R = sq.n * a.G;
-    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G},
-        orows{sq.begin, (long long)a.Hq * a.D, a.D, a.G, kv * a.G}, srows{sq.begin, a.Hq, 1, a.G, kv * a.G};
+    if ((long long)pl.tile * BM >= R) return;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G};
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
     const float c2 = a.scale * LOG2E;
-    for (long long rr = (long long)blockIdx.x * BM; rr < R; rr += (long long)gridDim.x * BM) {
+    const Dma<T, DP, BN> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    if (a.D < DP) {
+        for (int i = threadIdx.x; i < 4 * TB / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    for (long long rr = (long long)pl.tile * BM; rr < R; rr += (long long)tiles * BM) {
         const int r0 = (int)rr;
         const int row = r0 + wave * 32 + (lane & 31);
         const bool live = row < R;
-        const int jmax = live ? seen_keys(row / a.G, sq.n, sk.n, a.causal) : 0;
-        const int jend = seen_keys((min(r0 + BM, R) - 1) / a.G, sq.n, sk.n, a.causal);
+        const int tok = live ? row / a.G : 0;
+        const long long at = live ? (sq.begin + tok) * a.Hq + kv * a.G + (row - tok * a.G) : 0;     // row of [Tq, Hq]
+        const int jmax = live ? seen_keys(tok, sq.n, sk.n, a.causal) : 0;
+        const int last = min(r0 + BM, R) - 1;
+        const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal);
         const int jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);
+        const int jwave = r0 + wave * 32 < R ? seen_keys(min(r0 + wave * 32 + 31, last) / a.G, sq.n, sk.n, a.causal) : 0;
         bool spoilt = false;        // the row sees a key that is not finite: so is its gradient
-        Frag<T> qf[KS], gf[KS];
+        GqState<T, DP, BN> st;
         float delta = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = s * 16 + h * 8;
             const bool on = live && d < a.D;
-            qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + d, on);
-            gf[s] = frag_global((const T*)a.go + (live ? grows.at(row) : 0) + d, on);
+            st.qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + d, on);
+            st.gf[s] = frag_global((const T*)a.go + (live ? grows.at(row) : 0) + d, on);
             if (on) {
                 Raw8<T> x, y;
                 float fx[8], fy[8];
-                x.load((const T*)a.o + orows.at(row) + d);
+                x.load((const T*)a.o + at * a.D + d);
                 y.load((const T*)a.go + grows.at(row) + d);
                 x.get(fx);
                 y.get(fy);
@@ -495,147 +552,251 @@ __global__ __launch_bounds__(256) void k_attn_gq(Attn a) {
                 for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
             }
         }
-        delta += __shfl_xor(delta, 32, 64);
-        if (live && h == 0) a.delta[srows.at(row)] = delta;
-        const float l2 = (live ? a.lse[srows.at(row)] : 0.f) * LOG2E;
-        f32x16 acc[DT];
+        st.delta = delta + __shfl_xor(delta, 32, 64);
+        if (live && h == 0) a.delta[at] = st.delta;
+        const float2 stat = live ? a.stats[at] : make_float2(0.f, 0.f);
+        st.base = stat.x;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i] = zero16();
-        for (int k0 = 0; k0 < jend; k0 += BK) {
+        for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
+        const int nfull = jall / BN;
+        if (nfull > 0) {
             __syncthreads();
-            bool bad = false;
-            const auto krow = [&](int r) { return (long long)r * a.k_st; };
-            if (k0 + BK > jall) bad = stage<T, DP, BK, true>(lk, k + (long long)k0 * a.k_st, sk.n - k0, a.D, krow);
-            else stage<T, DP, BK, false>(lk, k + (long long)k0 * a.k_st, sk.n - k0, a.D, krow);
-            stage<T, DP, BK, false>(lv, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
-            bad = __syncthreads_or(bad);
-            if (bad)
-                for (int j = 0; j < min(jmax - k0, BK); ++j) spoilt |= spoils(k + (k0 + j) * a.k_st, a.D);
-#pragma unroll
-            for (int sub = 0; sub < BK / 32; ++sub) {
-                f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    s = mma(L::row_frag(lk, sub * 32 + (lane & 31), i, h), qf[i], s);
-                    dp = mma(L::row_frag(lv, sub * 32 + (lane & 31), i, h), gf[i], dp);
+            dk.load(k, a.k_st, lds);
+            dv.load(v, a.v_st, lds + TB);
+            for (int t = 0; t < nfull; ++t) {
+                char* now = lds + (t & 1) * 2 * TB;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (t + 1 < nfull) {
+                    char* next = lds + ((t + 1) & 1) * 2 * TB;
+                    dk.load(k + (long long)(t + 1) * BN * a.k_st, a.k_st, next);
+                    dv.load(v + (long long)(t + 1) * BN * a.v_st, a.v_st, next + TB);
                 }
-                float ds[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    ds[i] = k0 + sub * 32 + reg_row(i, h) < jmax ? exp2f(s[i] * c2 - l2) * (dp[i] - delta) : 0.f;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    Frag<T> f;
-                    frag_of(f, ds + 8 * t);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lk, sub * 32 + 16 * t, d, lane), f, acc[d]);
-                }
+                st.template step<false>(now, now + TB, lane, c2, BN);
             }
         }
+        for (int k0 = nfull * BN; k0 < jend; k0 += BN) {
+            __syncthreads();
+            bool bad = stage<T, DP, BN, true>(lds, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+            stage<T, DP, BN, false>(lds + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
+            bad = __syncthreads_or(bad);
+            if (k0 < jwave) st.template step<true>(lds, lds + TB, lane, c2, jmax - k0);
+            if (bad)
+                for (int j = 0; j < min(jmax - k0, BN); ++j) spoilt |= spoils(k + (k0 + j) * a.k_st, a.D);
+        }
         if (live) {
-            T* o = gq + orows.at(row);
+            T* o = gq + at * a.D;
+            const float mul = spoilt ? NAN : a.scale * stat.y;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) store_cols(o, acc[d], d, h, a.D, spoilt ? NAN : a.scale);
+            for (int d = 0; d < DT; ++d) store_cols(o, st.acc[d], d, h, a.D, mul);
         }
     }
 }
 
 // --------------------------------------------------------------------------------------------- gradients of k and v
+// One key per lane, the rows that see it in registers; rows pass through LDS, so no sum leaves the workgroup and none is atomic.
+// For 128 elements of 16 bits the value rows stay in LDS instead of registers: two waves share a SIMD's registers then.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attn_gkv(Attn a) {
+struct GkvCfg {
+    static constexpr int BR = sizeof(T) * DP >= 256 ? 32 : 64;         // rows of a step
+    static constexpr bool V_LDS = sizeof(T) * DP >= 256;
+    static constexpr int WAVES = sizeof(T) * DP > 256 ? 1 : 2;         // per SIMD
+};
+
+// the rows of a step, for a lane's part of each round of loads: token and head of row r0 + i RPI + threadIdx / CPR
+template <typename T, int DP, int BR>
+struct RowDma {
     typedef Tile<T, DP> L;
-    constexpr int KS = DP / 16, DT = DP / 32;
-    constexpr int BK = 128, BR = 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BR * L::ROWB];
-    __shared__ __attribute__((aligned(16))) float stat[2][BR];
-    char *lq = lds, *lg = lds + BR * L::ROWB;
+    static constexpr int RPI = 256 / L::CPR, N = (BR + RPI - 1) / RPI;
+    static_assert((RPI % 8 == 0 && BR % RPI == 0) || N == 1, "the permutation must not depend on the round");
+    int tok[N], g[N], c;
+    bool on;
+    __device__ __forceinline__ RowDma(int r0, int G, int D) {
+        const int row = threadIdx.x / L::CPR;
+        c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC;
+        on = c < D && row < BR;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            tok[i] = (r0 + i * RPI + row) / G;
+            g[i] = r0 + i * RPI + row - tok[i] * G;
+        }
+    }
+    __device__ __forceinline__ void advance(int G, int dt, int dg) {       // BR = dt G + dg
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            tok[i] += dt;
+            g[i] += dg;
+            if (g[i] >= G) g[i] -= G, ++tok[i];
+        }
+    }
+    __device__ __forceinline__ void load(const T* base, long long st, long long sh, char* lds) const {
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) load_to_lds(base + tok[i] * st + g[i] * sh + c, lds + i * 4096 + (threadIdx.x >> 6) * 1024);
+        }
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a, int tiles, unsigned first_rest) {
+    typedef Tile<T, DP> L;
+    typedef GkvCfg<T, DP> C;
+    constexpr int KS = DP / 16, DT = DP / 32, BK = 128, BR = C::BR, TB = BR * L::ROWB;
+    constexpr bool F32 = sizeof(T) == 4;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TB + (C::V_LDS ? BK * L::ROWB : 0)];
+    __shared__ __attribute__((aligned(16))) float stat[2][3][BR];      // exponent base (16 bits: with the sum's logarithm), D, 1 / sum
+    char* lvt = lds + 4 * TB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int kv = blockIdx.y, b = blockIdx.z;
     T *gk = (T*)a.gk, *gv = (T*)a.gv;
-    if (b == a.B) {
+    if (blockIdx.x >= first_rest) {
         const Rest z = rest(a.cu_k, a.B, a.Tk);
-        for (long long i = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); i < z.n; i += (long long)gridDim.x * 32) {
-            zero_row(gk + (z.row(i) * a.Hk + kv) * a.D, a.D, threadIdx.x & 7, 8);
-            zero_row(gv + (z.row(i) * a.Hk + kv) * a.D, a.D, threadIdx.x & 7, 8);
+        for (long long i = (long long)(blockIdx.x - first_rest) * 32 + (threadIdx.x >> 3); i < z.n * a.Hk; i += (long long)(gridDim.x - first_rest) * 32) {
+            const long long r = z.row(i / a.Hk) * a.Hk + i % a.Hk;
+            zero_row(gk + r * a.D, a.D, threadIdx.x & 7, 8);
+            zero_row(gv + r * a.D, a.D, threadIdx.x & 7, 8);
         }
         return;
     }
+    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    if (pl.tile < 0) return;
+    const int tile = tiles - 1 - pl.tile;       // the first keys have the most rows
+    const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
+    if ((long long)tile * BK >= sk.n) return;
     const int R = sq.n * a.G;
     const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G},
         srows{sq.begin, a.Hq, 1, a.G, kv * a.G};
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const T *q0 = (const T*)a.q + sq.begin * a.q_st + (long long)kv * a.G * a.q_sh, *g0 = (const T*)a.go + sq.begin * a.go_st + (long long)kv * a.G * a.go_sh;
     const float c2 = a.scale * LOG2E;
-    for (long long kk = (long long)blockIdx.x * BK; kk < sk.n; kk += (long long)gridDim.x * BK) {
+    const int adv_t = BR / a.G, adv_g = BR - adv_t * a.G;
+    if (a.D < DP) {
+        for (int i = threadIdx.x; i < 4 * TB / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    // this thread's row of statistics of the step at r0
+    const auto load_stat = [&](int r0, float* to) {
+        to[0] = to[1] = to[2] = 0.f;
+        if ((int)threadIdx.x < BR && r0 + (int)threadIdx.x < R) {
+            const long long at = srows.at(r0 + threadIdx.x);
+            const float2 s = a.stats[at];
+            to[0] = F32 ? s.x : s.x - __builtin_amdgcn_logf(s.y);
+            to[1] = a.delta[at];
+            to[2] = s.y;
+        }
+    };
+    const auto put_stat = [&](const float* from, int buf) {
+        if ((int)threadIdx.x < BR) {
+            stat[buf][0][threadIdx.x] = from[0];
+            stat[buf][1][threadIdx.x] = from[1];
+            if (F32) stat[buf][2][threadIdx.x] = from[2];
+        }
+    };
+    for (long long kk = (long long)tile * BK; kk < sk.n; kk += (long long)tiles * BK) {
         const int k0 = (int)kk;
         const int key = k0 + wave * 32 + (lane & 31);
         const bool live = key < sk.n;
-        Frag<T> kf[KS], vf[KS];
+        Frag<T> kf[KS], vf[C::V_LDS ? 1 : KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = s * 16 + h * 8;
             kf[s] = frag_global(k + (live ? key * a.k_st : 0) + d, live && d < a.D);
-            vf[s] = frag_global(v + (live ? key * a.v_st : 0) + d, live && d < a.D);
+            if (!C::V_LDS) vf[s] = frag_global(v + (live ? key * a.v_st : 0) + d, live && d < a.D);
         }
+        __syncthreads();
+        if (C::V_LDS) stage<T, DP, BK, false>(lvt, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
         f32x16 ak[DT], av[DT];
 #pragma unroll
         for (int i = 0; i < DT; ++i) ak[i] = zero16(), av[i] = zero16();
-        // the first token that sees this key (this tile's first key); rows before it see nothing of it
-        const long long first = a.causal ? (long long)k0 - (sk.n - sq.n) : 0;
-        const int t_first = first < 0 ? 0 : first > sq.n ? sq.n : (int)first;
-        const long long mine = a.causal ? (long long)key - (sk.n - sq.n) : 0;
-        const int t_key = live ? (mine < 0 ? 0 : mine > sq.n ? sq.n : (int)mine) : sq.n;
-        const int r_key = t_key * a.G;          // rows from here on see the key
-        const long long final = a.causal ? (long long)min(k0 + BK, sk.n) - 1 - (sk.n - sq.n) : 0;
-        const int r_all = (final < 0 ? 0 : final > sq.n ? sq.n : (int)final) * a.G;       // rows from here on see all keys of the tile
+        // rows before first see no key of the tile; from r_all on they see all of them; from r_key on, this lane's
+        const auto first_row = [&](int j) {
+            const long long t = a.causal ? (long long)j - (sk.n - sq.n) : 0;
+            return (t < 0 ? 0 : t > sq.n ? sq.n : (int)t) * a.G;
+        };
+        const int first = first_row(k0), r_all = first_row(min(k0 + BK, sk.n) - 1), r_key = live ? first_row(key) : R;
         bool spoilt = false;                    // a row that is not finite sees the key: so are its gradients
-        for (int r0 = t_first * a.G; r0 < R; r0 += BR) {
+
+        const auto step = [&](auto mask, const char* lq, const char* lg, const float (*st)[BR], int r0) {
+            constexpr bool MASK = decltype(mask)::value;
+#pragma unroll
+            for (int sub = 0; sub < BR / 32; ++sub) {
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    s = mma(L::row_frag(lq, sub * 32 + (lane & 31), i, h), kf[i], s);
+                    if constexpr (C::V_LDS) dp = mma(L::row_frag(lg, sub * 32 + (lane & 31), i, h), L::row_frag(lvt, wave * 32 + (lane & 31), i, h), dp);
+                    else dp = mma(L::row_frag(lg, sub * 32 + (lane & 31), i, h), vf[i], dp);
+                }
+                float p[16], ds[16];
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const int r4 = sub * 32 + 8 * q4 + 4 * h;
+                    const float4 ba = *reinterpret_cast<const float4*>(&st[0][r4]), de = *reinterpret_cast<const float4*>(&st[1][r4]);
+                    float4 in = make_float4(1.f, 1.f, 1.f, 1.f);
+                    if (F32) in = *reinterpret_cast<const float4*>(&st[2][r4]);
+                    const float bb[4] = {ba.x, ba.y, ba.z, ba.w}, dd[4] = {de.x, de.y, de.z, de.w}, ii[4] = {in.x, in.y, in.z, in.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = 4 * q4 + j;
+                        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -bb[j]));
+                        if (F32) p[i] *= ii[j];
+                        ds[i] = p[i] * (dp[i] - dd[j]);
+                        if (MASK && !(r0 + r4 + j >= r_key && r0 + r4 + j < R)) p[i] = ds[i] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    Frag<T> pf, df;
+                    frag_of(pf, p + 8 * t);
+                    frag_of(df, ds + 8 * t);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        av[d] = mma(L::col_frag(lg, sub * 32 + 16 * t, d, lane), pf, av[d]);
+                        ak[d] = mma(L::col_frag(lq, sub * 32 + 16 * t, d, lane), df, ak[d]);
+                    }
+                }
+            }
+        };
+        const auto border = [&](int r0) {
+            float mine[3];
+            load_stat(r0, mine);
             __syncthreads();
-            bool bad = false;
-            const auto qrow = [&](int r) { return qrows.at(r0 + r); };
-            const auto grow = [&](int r) { return grows.at(r0 + r); };
-            if (r0 < r_all) {
-                bad = stage<T, DP, BR, true>(lq, (const T*)a.q, R - r0, a.D, qrow);
-                bad |= stage<T, DP, BR, true>(lg, (const T*)a.go, R - r0, a.D, grow);
-            } else {
-                stage<T, DP, BR, false>(lq, (const T*)a.q, R - r0, a.D, qrow);
-                stage<T, DP, BR, false>(lg, (const T*)a.go, R - r0, a.D, grow);
-            }
-            if (threadIdx.x < BR) {
-                const bool on = r0 + (int)threadIdx.x < R;
-                stat[0][threadIdx.x] = on ? a.lse[srows.at(r0 + threadIdx.x)] * LOG2E : 0.f;
-                stat[1][threadIdx.x] = on ? a.delta[srows.at(r0 + threadIdx.x)] : 0.f;
-            }
+            bool bad = stage<T, DP, BR, true>(lds, (const T*)a.q, R - r0, a.D, [&](int r) { return qrows.at(r0 + r); });
+            bad |= stage<T, DP, BR, true>(lds + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
+            put_stat(mine, 0);
             bad = __syncthreads_or(bad);
+            step(std::true_type{}, lds, lds + TB, stat[0], r0);
             if (bad)
                 for (int r = max(r0, r_key); r < min(r0 + BR, R); ++r)
                     spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
-            f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                s = mma(L::row_frag(lq, lane & 31, i, h), kf[i], s);
-                dp = mma(L::row_frag(lg, lane & 31, i, h), vf[i], dp);
-            }
-            float p[16], ds[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int r = reg_row(i, h);
-                const bool sees = r0 + r >= r_key && r0 + r < R;
-                p[i] = sees ? exp2f(s[i] * c2 - stat[0][r]) : 0.f;
-                ds[i] = sees ? p[i] * (dp[i] - stat[1][r]) : 0.f;
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                Frag<T> pf, df;
-                frag_of(pf, p + 8 * t);
-                frag_of(df, ds + 8 * t);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    av[d] = mma(L::col_frag(lg, 16 * t, d, lane), pf, av[d]);
-                    ak[d] = mma(L::col_frag(lq, 16 * t, d, lane), df, ak[d]);
+        };
+        int r0 = first;
+        for (; r0 < R && r0 < r_all; r0 += BR) border(r0);
+        const int nfull = r0 < R ? (R - r0) / BR : 0;
+        if (nfull > 0) {
+            RowDma<T, DP, BR> dma(r0, a.G, a.D);
+            float mine[3];
+            load_stat(r0, mine);
+            __syncthreads();
+            dma.load(q0, a.q_st, a.q_sh, lds);
+            dma.load(g0, a.go_st, a.go_sh, lds + TB);
+            put_stat(mine, 0);
+            for (int t = 0; t < nfull; ++t, r0 += BR) {
+                char* now = lds + (t & 1) * 2 * TB;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (t + 1 < nfull) {
+                    char* next = lds + ((t + 1) & 1) * 2 * TB;
+                    load_stat(r0 + BR, mine);
+                    dma.advance(a.G, adv_t, adv_g);
+                    dma.load(q0, a.q_st, a.q_sh, next);
+                    dma.load(g0, a.go_st, a.go_sh, next + TB);
                 }
+                step(std::false_type{}, now, now + TB, stat[t & 1], r0);
+                if (t + 1 < nfull) put_stat(mine, (t + 1) & 1);
             }
         }
+        if (r0 < R) border(r0);
         if (live) {
             T *ok = gk + ((sk.begin + key) * a.Hk + kv) * a.D, *ov = gv + ((sk.begin + key) * a.Hk + kv) * a.D;
 #pragma unroll
@@ -700,7 +861,7 @@ size_t sam3_seq_attn_fwd_workspace_bytes(int64_t Tq, int B, int Hq, int Hk, int 
 
 int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                       int64_t v_st, int64_t v_sh, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, void* out,
-                      float* lse, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int causal,
+                      float* lse, float* stats, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int causal,
                       float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
     sam3_seq_clear_error();
     (void)workspace; (void)workspace_bytes;
@@ -713,7 +874,7 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     }
     if (!cu_q || !cu_k || !out || misaligned(out)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
     Attn a{};
-    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.cu_q = cu_q; a.cu_k = cu_k; a.len_k = len_k;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.stats = (float2*)stats; a.cu_q = cu_q; a.cu_k = cu_k; a.len_k = len_k;
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest = max_q < Tq ? max_q : Tq;
@@ -728,7 +889,7 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
 size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq) { return Tq > 0 && Hq > 0 ? (size_t)Tq * Hq * sizeof(float) : 0; }
 
 int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
-                      int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const void* out, const float* lse,
+                      int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const void* out, const float* stats,
                       const int32_t* cu_q, const int32_t* cu_k, void* gq, void* gk, void* gv, int64_t Tq, int64_t Tk, int B, int Hq,
                       int Hk, int D, int64_t max_q, int64_t max_k, int causal, float scale, int dtype, void* workspace,
                       size_t workspace_bytes, void* stream) {
@@ -737,7 +898,7 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     if (Tq > 0) {
         if (int rc = check_tensor("q", q, q_st, q_sh, dtype)) return rc;
         if (int rc = check_tensor("go", go, go_st, go_sh, dtype)) return rc;
-        if (!out || !lse || !gq || misaligned(out) || misaligned(gq)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
+        if (!out || !stats || !gq || misaligned(out) || misaligned(gq)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
         if (!workspace || workspace_bytes < sam3_seq_attn_bwd_workspace_bytes(Tq, Hq))
             return sam3_seq_fail(ENOMEM_, "attention: workspace too small: %zu < %zu", workspace_bytes, sam3_seq_attn_bwd_workspace_bytes(Tq, Hq));
     }
@@ -748,20 +909,19 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     }
     if (!cu_q || !cu_k) return sam3_seq_fail(EINVAL_, "attention: null pointer");
     Attn a{};
-    a.q = q; a.k = k; a.v = v; a.go = go; a.o = out; a.lse = (float*)lse; a.delta = (float*)workspace;
+    a.q = q; a.k = k; a.v = v; a.go = go; a.o = out; a.stats = (float2*)stats; a.delta = (float*)workspace;
     a.gq = gq; a.gk = gk; a.gv = gv; a.cu_q = cu_q; a.cu_k = cu_k;
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh; a.go_st = go_st; a.go_sh = go_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest_q = max_q < Tq ? max_q : Tq, longest_k = max_k < Tk ? max_k : Tk;
+    const int qt = (int)tiles(longest_q * a.G, BM), kt = (int)tiles(longest_k, 128);
+    const long long q_rest = places(B * Hk, qt), k_rest = places(B * Hk, kt);
+    if (q_rest > 0x7ffffff0ll || k_rest > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
     if (Tq > 0) {
-        const dim3 grid(tiles(longest_q * a.G, BM), (unsigned)Hk, (unsigned)B + 1);
-        BY_HEAD(k_attn_gq, grid, (hipStream_t)stream, a);
+        BY_HEAD(k_attn_gq, dim3((unsigned)q_rest + REST), (hipStream_t)stream, a, qt, (unsigned)q_rest);
         if (int rc = launched("sam3_seq_attn_bwd")) return rc;
     }
-    if (Tk > 0) {
-        const dim3 grid(tiles(longest_k, 128), (unsigned)Hk, (unsigned)B + 1);
-        BY_HEAD(k_attn_gkv, grid, (hipStream_t)stream, a);
-    }
+    if (Tk > 0) BY_HEAD(k_attn_gkv, dim3((unsigned)k_rest + REST), (hipStream_t)stream, a, kt, (unsigned)k_rest);
     return launched("sam3_seq_attn_bwd");
 }
 

@@ -296,12 +296,13 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
 
 
 # ---------------------------------------------------------------------------------------------------------- attention
-def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse):
+def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse, want_stats=False):
     tq, hq, d = q.shape
     tk, hk = k.shape[:2]
     q, k, v = _aligned(q.detach()), _aligned(k.detach()), _aligned(v.detach())
     out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
     lse = torch.empty(tq, hq, dtype=torch.float32, device=q.device) if want_lse else None
+    stats = torch.empty(tq, hq, 2, dtype=torch.float32, device=q.device) if want_stats else None
     dt = _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32
     lib = _ffi.load()
     b = cu_q.numel() - 1
@@ -311,27 +312,30 @@ def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse)
         _check(lib.sam3_seq_attn_fwd(
             q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
             cu_q.data_ptr(), cu_k.data_ptr(), None if len_k is None else len_k.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), tq, tk, b, hq, hk, d, max_q, max_k, int(causal), scale, dt,
-            None if ws is None else ws.data_ptr(), nbytes, _stream(q.device)), "sam3_seq_attn_fwd")
-    return out, lse
+            None if lse is None else lse.data_ptr(), None if stats is None else stats.data_ptr(), tq, tk, b, hq, hk, d, max_q, max_k,
+            int(causal), scale, dt, None if ws is None else ws.data_ptr(), nbytes, _stream(q.device)), "sam3_seq_attn_fwd")
+    return out, lse, stats
 
 
 class _PackedAttention(torch.autograd.Function):
+    """``(out, lse)``, lse None where it is not wanted."""
+
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale):
-        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, None, max_q, max_k, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+    def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, want_lse):
+        out, lse, stats = _attn_fwd(q, k, v, cu_q, cu_k, None, max_q, max_k, causal, scale, want_lse, True)
+        ctx.save_for_backward(q, k, v, out, stats, cu_q, cu_k)
         ctx.how = max_q, max_k, causal, scale
-        ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
+        if lse is not None:
+            ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go, _):
         if go is None:
-            return (None,) * 9
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+            return (None,) * 10
+        q, k, v, out, stats, cu_q, cu_k = ctx.saved_tensors
         max_q, max_k, causal, scale = ctx.how
         tq, hq, d = q.shape
         tk, hk = k.shape[:2]
@@ -343,12 +347,12 @@ class _PackedAttention(torch.autograd.Function):
         with _on(q.device):
             _check(lib.sam3_seq_attn_bwd(
                 q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                go.data_ptr(), go.stride(0), go.stride(1), out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+                go.data_ptr(), go.stride(0), go.stride(1), out.data_ptr(), stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
                 gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq, tk, cu_q.numel() - 1, hq, hk, d, max_q, max_k, int(causal), scale,
                 _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32, ws.data_ptr(), nbytes, _stream(q.device)),
                 "sam3_seq_attn_bwd")
         need = ctx.needs_input_grad
-        return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None) + (None,) * 6
+        return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None) + (None,) * 7
 
 
 def _index(name: str, t: torch.Tensor, n: int, device) -> None:
@@ -402,7 +406,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     _need(0.0 < scale < 3e38, f"scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         _need(len_k is None, "len_k has no gradient: call packed_attention under torch.no_grad()")
-        out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, bool(causal), scale)
+        out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, bool(causal), scale, return_lse)
     else:
-        out, lse = _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, bool(causal), scale, return_lse)
+        out, lse, _ = _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, bool(causal), scale, return_lse)
     return (out, lse) if return_lse else out

@@ -73,7 +73,7 @@ def test_header_exports_and_error_text():
     assert rope() == -22 and "axis" in lib.sam3_seq_last_error().decode()
 
     def attn(q=p, B=1, Hq=4, Hk=2, D=64, Tq=8, Tk=8, scale=0.1, dtype=0, st=64, cu=p):
-        return lib.sam3_seq_attn_fwd(q, st, 64, p, 64, 64, p, 64, 64, cu, p, None, p, None, Tq, Tk, B, Hq, Hk, D, 8, 8, 1, scale, dtype, None, 0, None)
+        return lib.sam3_seq_attn_fwd(q, st, 64, p, 64, 64, p, 64, 64, cu, p, None, p, None, None, Tq, Tk, B, Hq, Hk, D, 8, 8, 1, scale, dtype, None, 0, None)
     for bad in (dict(q=None), dict(Hk=3), dict(D=60), dict(scale=0.0), dict(scale=float("nan")), dict(dtype=2), dict(st=62), dict(cu=None), dict(Hq=0),
                 dict(Tq=-1)):
         assert attn(**bad) == -22, bad
