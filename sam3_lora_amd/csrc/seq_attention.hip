@@ -174,7 +174,7 @@ struct Rows {
     }
 };
 
-// ROWS rows (n of them there, the others zeros) of DP elements (D of them there) into LDS by 256 threads.
+// ROWS rows (n of them there, the others zeros) of DP elements (D of them there) into LDS by NT threads.
 // CHECK: infinities and NaN become zeros, and the answer says whether there were any.  A product over a tile that some of its rows
 // only see a part of multiplies what they do not see by zero, which a non-finite element would turn into NaN; such tiles are
 // staged with the check, and the rows that do see such an element get its effect afterwards (spoils(), add_nonfinite()).
@@ -185,14 +185,14 @@ __device__ __forceinline__ unsigned only_finite(unsigned u, bf16_t) {
 }
 __device__ __forceinline__ unsigned only_finite(unsigned u, float) { return (u & 0x7f800000u) == 0x7f800000u ? 0u : u; }
 
-template <typename T, int DP, int ROWS, bool CHECK, typename ADDR>
+template <typename T, int DP, int ROWS, bool CHECK, int NT = 256, typename ADDR>
 __device__ __forceinline__ bool stage(char* lds, const T* base, int n, int D, ADDR addr) {
     typedef Tile<T, DP> L;
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < (ROWS * L::CPR + 255) / 256; ++i) {
-        const int p = i * 256 + threadIdx.x, row = p / L::CPR, c = p % L::CPR;
-        if (ROWS * L::CPR % 256 && row >= ROWS) break;
+    for (int i = 0; i < (ROWS * L::CPR + NT - 1) / NT; ++i) {
+        const int p = i * NT + threadIdx.x % NT, row = p / L::CPR, c = p % L::CPR;
+        if (ROWS * L::CPR % NT && row >= ROWS) break;
         uint4 u = make_uint4(0, 0, 0, 0);
         if (row < n && c * L::EPC < D) u = *reinterpret_cast<const uint4*>(base + addr(row) + c * L::EPC);
         if (CHECK && !(finite_bits(u.x, T()) && finite_bits(u.y, T()) && finite_bits(u.z, T()) && finite_bits(u.w, T()))) {
@@ -335,7 +335,7 @@ struct FwdState {
             }
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
         if (__any(mx > base + 8.f)) {
-            const float next = fmaxf(base, mx), alpha = __builtin_amdgcn_exp2f(base - next);
+            const float next = mx > base + 8.f ? mx : base, alpha = __builtin_amdgcn_exp2f(base - next);
             base = next;
             l *= alpha;
 #pragma unroll
@@ -446,6 +446,205 @@ __global__ __launch_bounds__(256, 2) void k_attn_fwd(Attn a, int tiles, unsigned
             if (a.stats && h == 0) a.stats[at] = make_float2(st.base, inv);
             if (a.lse && h == 0) a.lse[at] = inv == 0.f ? -INFINITY : st.base * LN2 + logf(l);
         }
+    }
+}
+
+// ------------------------------------------------------------------------------------- forward for few rows, split over the keys
+// With few rows (one new token of each request: the heads of one group) the keys are what has to be read, once, and nothing else
+// counts.  A workgroup takes 32 rows and a chunk of keys; its waves take blocks of 32 keys in turn, each with tiles of its own that
+// the next block's loads fill while it computes (no barrier: a wave waits for its own loads).  The waves' results meet in LDS, the
+// chunks' in k_attn_join.
+template <typename T, int DP>
+struct FewCfg {
+    static constexpr int NW = sizeof(T) * DP > 256 ? 2 : 4;
+    static constexpr int TB = 32 * DP * (int)sizeof(T), LDS = NW * 4 * TB;
+};
+
+template <typename T, int DP>
+struct WaveDma {
+    typedef Tile<T, DP> L;
+    static constexpr int RPI = 64 / L::CPR, N = 32 / RPI;
+    int row, c;
+    __device__ __forceinline__ WaveDma() : row((threadIdx.x & 63) / L::CPR), c(((threadIdx.x & 63) % L::CPR) ^ L::f((threadIdx.x & 63) / L::CPR)) {}
+    // (the rows of a round and the round's first row have no bit in common, so the permutation is the exclusive or of both)
+    __device__ __forceinline__ void load(const T* tile, long long st, int D, char* lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = (c ^ L::f(i * RPI)) * L::EPC;
+            if (e < D) load_to_lds(tile + (i * RPI + row) * st + e, lds + i * 1024);
+        }
+    }
+};
+
+struct Few {
+    int tiles, splits, chunk;       // row tiles of a pair, chunks of the longest sequence, keys of a chunk
+    float* part;                    // [splits, Tq * Hq, D] unnormalised results, and
+    float2* pstat;                  // [splits, Tq * Hq] their bases and sums; unused with one split
+    unsigned first_rest;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__((FewCfg<T, DP>::NW * 64), (FewCfg<T, DP>::LDS > 81920 ? 1 : 2)) void k_attn_few(Attn a, Few f) {
+    typedef Tile<T, DP> L;
+    typedef FewCfg<T, DP> C;
+    constexpr int KS = DP / 16, DT = DP / 32, NW = C::NW, TB = C::TB, NT = NW * 64;
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    __shared__ float2 wstat[NW][32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    T* out = (T*)a.out;
+    if (blockIdx.x >= f.first_rest) {
+        const Rest z = rest(a.cu_q, a.B, a.Tq);
+        for (long long i = (long long)(blockIdx.x - f.first_rest) * (NT / 8) + (threadIdx.x >> 3); i < z.n * a.Hq;
+             i += (long long)(gridDim.x - f.first_rest) * (NT / 8)) {
+            const long long r = z.row(i / a.Hq) * a.Hq + i % a.Hq;
+            zero_row(out + r * a.D, a.D, threadIdx.x & 7, 8);
+            if (a.lse && (threadIdx.x & 7) == 0) a.lse[r] = -INFINITY;
+        }
+        return;
+    }
+    const Place pl = place(blockIdx.x, a.B * a.Hk * f.splits, f.tiles);
+    if (pl.tile < 0) return;
+    const int pair = pl.pair / f.splits, split = pl.pair - pair * f.splits;
+    const int b = pair / a.Hk, kv = pair - b * a.Hk;
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, a.len_k, b, a.Tk);
+    const int R = sq.n * a.G;
+    if ((long long)pl.tile * 32 >= R) return;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G};
+    const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const float c2 = a.scale * LOG2E;
+    char* mine = lds + wave * 4 * TB;
+    const WaveDma<T, DP> dma;
+    for (long long rr = (long long)pl.tile * 32; rr < R; rr += (long long)f.tiles * 32) {
+        const int r0 = (int)rr, row = r0 + (lane & 31);
+        const bool live = row < R;
+        const int jmax = live ? seen_keys(row / a.G, sq.n, sk.n, a.causal) : 0;
+        const int last = min(r0 + 32, R) - 1;
+        const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal), jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);
+        if (f.splits > 1 && (long long)split * f.chunk >= jend && (split > 0 || jend > 0)) continue;      // (chunk 0 answers for a row without keys)
+        __syncthreads();
+        if (a.D < DP) {
+            for (int i = lane; i < 4 * TB / 16; i += 64) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        FwdState<T, DP, 32> st;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            st.qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + s * 16 + h * 8, live && s * 16 + h * 8 < a.D);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
+        st.base = -3.0e38f;
+        st.l = 0.f;
+        for (long long c0 = (long long)split * f.chunk; c0 < jend; c0 += (long long)f.splits * f.chunk) {
+            const int begin = (int)c0, end = (int)(c0 + f.chunk < jend ? c0 + f.chunk : jend);
+            const int full = min(end, jall) >= begin ? (min(end, jall) - begin) / 32 : 0;       // blocks that need no mask
+            int blk = wave, buf = 0;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (blk < full) {
+                dma.load(k + (long long)(begin + blk * 32) * a.k_st, a.k_st, a.D, mine);
+                dma.load(v + (long long)(begin + blk * 32) * a.v_st, a.v_st, a.D, mine + TB);
+            }
+            for (; blk < full; blk += NW, buf ^= 1) {
+                char *now = mine + buf * 2 * TB, *next = mine + (buf ^ 1) * 2 * TB;
+                // what was read of the other buffer has arrived; then its new loads, and the wait for all but those
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (blk + NW < full) {
+                    dma.load(k + (long long)(begin + (blk + NW) * 32) * a.k_st, a.k_st, a.D, next);
+                    dma.load(v + (long long)(begin + (blk + NW) * 32) * a.v_st, a.v_st, a.D, next + TB);
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * WaveDma<T, DP>::N) : "memory");
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+                st.template step<false>(now, now + TB, lane, c2, 32);
+            }
+            for (int i = full + (wave + NW - full % NW) % NW; begin + i * 32 < end; i += NW) {
+                const int k0 = begin + i * 32;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                stage<T, DP, 32, false, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+                const bool bad = __any(stage<T, DP, 32, true, 64>(mine + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; }));
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                st.template step<true>(mine, mine + TB, lane, c2, min(jmax, end) - k0);
+                if (bad) add_nonfinite<T, DT>(st.acc, v + (long long)k0 * a.v_st, a.v_st, min(min(jmax, end) - k0, 32), a.D, h);
+            }
+        }
+        // the waves' results: [NW][32 rows][DP] fp32, in the tiles' place
+        __syncthreads();
+        float* pool = reinterpret_cast<float*>(lds);
+        const float l = st.l + __shfl_xor(st.l, 32, 64);
+        if (h == 0) wstat[wave][lane & 31] = make_float2(st.base, l);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4*>(pool + (wave * 32 + (lane & 31)) * DP + ((d * 32 + 8 * g + 4 * h) ^ ((lane & 7) << 2))) =
+                    make_float4(st.acc[d][4 * g], st.acc[d][4 * g + 1], st.acc[d][4 * g + 2], st.acc[d][4 * g + 3]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < 32 * (DP / 4); i += NT) {
+            const int r = i / (DP / 4), d = (i % (DP / 4)) * 4;
+            if (r0 + r >= R || d >= a.D) continue;
+            float base = wstat[0][r].x;
+#pragma unroll
+            for (int w = 1; w < NW; ++w) base = fmaxf(base, wstat[w][r].x);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float2 ws = wstat[w][r];
+                if (ws.y == 0.f) continue;          // (saw nothing)
+                const float e = __builtin_amdgcn_exp2f(ws.x - base);
+                const float4 x = *reinterpret_cast<const float4*>(pool + (w * 32 + r) * DP + (d ^ ((r & 7) << 2)));
+                o.x += x.x * e; o.y += x.y * e; o.z += x.z * e; o.w += x.w * e;
+                sum += ws.y * e;
+            }
+            const int t = (r0 + r) / a.G;
+            const long long at = (sq.begin + t) * a.Hq + kv * a.G + (r0 + r - t * a.G);
+            if (f.splits > 1) {
+                *reinterpret_cast<float4*>(f.part + ((long long)split * a.Tq * a.Hq + at) * a.D + d) = o;
+                if (d == 0) f.pstat[(long long)split * a.Tq * a.Hq + at] = make_float2(base, sum);
+            } else {
+                const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + at * a.D + d) = make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+                else *reinterpret_cast<float4*>(out + at * a.D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                if (d == 0 && a.stats) a.stats[at] = make_float2(base, inv);
+                if (d == 0 && a.lse) a.lse[at] = inv == 0.f ? -INFINITY : base * LN2 + logf(sum);
+            }
+        }
+    }
+}
+
+// the chunks' results of a row, in order; one thread has four elements
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(Attn a, Few f) {
+    const int b = blockIdx.y;
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, a.len_k, b, a.Tk);
+    const int per = a.D / 4;
+    T* out = (T*)a.out;
+    const long long all = a.Tq * a.Hq;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)sq.n * a.Hq * per; i += (long long)gridDim.x * 256) {
+        const int d = (int)(i % per) * 4;
+        const long long row = i / per;
+        const int head = (int)(row % a.Hq), t = (int)(row / a.Hq);
+        const long long at = (sq.begin + t) * a.Hq + head;
+        // the keys of this row's tile, as k_attn_few counted them
+        const int r = t * a.G + head % a.G, last = min((r / 32 + 1) * 32, sq.n * a.G) - 1;
+        const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal);
+        const int n = jend > 0 ? min(f.splits, (jend - 1) / f.chunk + 1) : 1;
+        float base = -3.0e38f;
+        for (int s = 0; s < n; ++s) base = fmaxf(base, f.pstat[s * all + at].x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        for (int s = 0; s < n; ++s) {
+            const float2 ps = f.pstat[s * all + at];
+            if (ps.y == 0.f) continue;
+            const float e = __builtin_amdgcn_exp2f(ps.x - base);
+            const float4 x = *reinterpret_cast<const float4*>(f.part + (s * all + at) * a.D + d);
+            o.x += x.x * e; o.y += x.y * e; o.z += x.z * e; o.w += x.w * e;
+            sum += ps.y * e;
+        }
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + at * a.D + d) = make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+        else *reinterpret_cast<float4*>(out + at * a.D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (d == 0 && a.stats) a.stats[at] = make_float2(base, inv);
+        if (d == 0 && a.lse) a.lse[at] = inv == 0.f ? -INFINITY : base * LN2 + logf(sum);
     }
 }
 
@@ -850,13 +1049,38 @@ unsigned tiles(int64_t rows, int per) {
     return (unsigned)(t < 1 ? 1 : t);
 }
 
+// The forward for few rows: where the tiles of 128 rows would leave most of the chip idle, and there are keys to split.
+struct Plan {
+    bool few;
+    int tiles, splits, chunk;
+};
+Plan plan(int64_t Tq, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
+    const int64_t rows = (max_q < Tq ? max_q : Tq) * (Hq / Hk), pairs = (int64_t)B * Hk;
+    Plan p{};
+    p.few = (rows <= 32 && max_k >= 128) || (max_k >= 1024 && pairs * tiles(rows, BM) <= 64);
+    if (!p.few) return p;
+    p.tiles = (int)tiles(rows, 32);
+    const int64_t wanted = 4096 / (pairs * p.tiles < 1 ? 1 : pairs * p.tiles);       // chunks, for about 16 workgroups per CU
+    int64_t chunk = wanted > 1 ? (max_k + wanted - 1) / wanted : max_k;
+    chunk = (chunk + 127) / 128 * 128;
+    if (chunk < 256) chunk = 256;
+    p.chunk = (int)(chunk > 0x40000000 ? 0x40000000 : chunk);
+    p.splits = (int)((max_k + p.chunk - 1) / p.chunk);
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+size_t part_bytes(int64_t Tq, int Hq, int D, int splits) {
+    return splits > 1 ? (size_t)splits * Tq * Hq * (D * sizeof(float) + sizeof(float2)) : 0;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t sam3_seq_attn_fwd_workspace_bytes(int64_t Tq, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype) {
-    (void)Tq; (void)B; (void)Hq; (void)Hk; (void)D; (void)max_q; (void)max_k; (void)dtype;
-    return 0;
+    if (check(Tq, 0, B, Hq, Hk, D, max_q, max_k, 1.f, dtype) || Tq == 0) return 0;
+    const Plan p = plan(Tq, B, Hq, Hk, max_q, max_k);
+    return p.few ? part_bytes(Tq, Hq, D, p.splits) : 0;
 }
 
 int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
@@ -864,7 +1088,6 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
                       float* lse, float* stats, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int causal,
                       float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
     sam3_seq_clear_error();
-    (void)workspace; (void)workspace_bytes;
     if (int rc = check(Tq, Tk, B, Hq, Hk, D, max_q, max_k, scale, dtype)) return rc;
     if (Tq == 0) return 0;
     if (int rc = check_tensor("q", q, q_st, q_sh, dtype)) return rc;
@@ -873,10 +1096,35 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
         if (int rc = check_tensor("v", v, v_st, v_sh, dtype)) return rc;
     }
     if (!cu_q || !cu_k || !out || misaligned(out)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
+    if (B == 0) max_q = max_k = 0;
     Attn a{};
     a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.stats = (float2*)stats; a.cu_q = cu_q; a.cu_k = cu_k; a.len_k = len_k;
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
+    const Plan p = plan(Tq, B, Hq, Hk, max_q, max_k);
+    if (p.few) {
+        const size_t need = part_bytes(Tq, Hq, D, p.splits);
+        if (need && (!workspace || workspace_bytes < need || misaligned(workspace)))
+            return sam3_seq_fail(ENOMEM_, "attention: workspace too small or misaligned: %zu < %zu", workspace_bytes, need);
+        const long long items = (long long)B * Hk * p.splits;
+        if (items > 0x3fffffffll || places((int)items, p.tiles) > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+        Few f{p.tiles, p.splits, p.chunk, (float*)workspace, nullptr, (unsigned)places((int)items, p.tiles)};
+        f.pstat = reinterpret_cast<float2*>(f.part + (p.splits > 1 ? (size_t)p.splits * Tq * Hq * D : 0));
+        const dim3 grid(f.first_rest + REST);
+        hipStream_t st = (hipStream_t)stream;
+#define FEW(TY, W) hipLaunchKernelGGL((k_attn_few<TY, W>), grid, dim3(FewCfg<TY, W>::NW * 64), 0, st, a, f)
+        if (dtype == 0) { if (D <= 32) FEW(bf16_t, 32); else if (D <= 64) FEW(bf16_t, 64); else FEW(bf16_t, 128); }
+        else { if (D <= 32) FEW(float, 32); else if (D <= 64) FEW(float, 64); else FEW(float, 128); }
+#undef FEW
+        if (int rc = launched("sam3_seq_attn_fwd")) return rc;
+        if (p.splits > 1 && B > 0) {
+            const int64_t work = (max_q < Tq ? max_q : Tq) * Hq * (D / 4);
+            const dim3 jgrid(tiles(work, 256) < 4096 ? tiles(work, 256) : 4096, (unsigned)B);
+            if (dtype == 0) hipLaunchKernelGGL(k_attn_join<bf16_t>, jgrid, dim3(256), 0, st, a, f);
+            else hipLaunchKernelGGL(k_attn_join<float>, jgrid, dim3(256), 0, st, a, f);
+        }
+        return launched("sam3_seq_attn_fwd");
+    }
     const int64_t longest = max_q < Tq ? max_q : Tq;
     const int nt = (int)tiles(longest * a.G, BM);
     const long long first_rest = places(B * Hk, nt);

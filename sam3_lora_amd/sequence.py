@@ -401,7 +401,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         _index("len_k", len_k, n - 1, q.device)
     for name, m in (("max_q", max_q), ("max_k", max_k)):
         _need(m is None or (isinstance(m, int) and 0 <= m < 2 ** 31), f"{name} must be a length, got {m}")
-    max_q, max_k = tq if max_q is None else max_q, tk if max_k is None else max_k
+    max_q, max_k = tq if max_q is None else min(max_q, tq), tk if max_k is None else min(max_k, tk)
     scale = d ** -0.5 if scale is None else float(scale)
     _need(0.0 < scale < 3e38, f"scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -457,12 +457,330 @@ def test_packed_attention_and_gradients(case, dtype):
 def test_packed_attention_hints_and_scale(dtype):
     check_attention([150, 40], [150, 40], 4, 2, 64, True, dtype, hints=False)
     check_attention([50], [50], 2, 2, 64, True, dtype, scale=0.5)
-    # a hint that is too small costs time, not the result
+    # a hint that is too small costs time, not the result (it may choose another order of the sums)
     g = gen(1)
-    q, k = rand(g, 300, 2, 64, dtype=dtype).to("cuda", dtype), rand(g, 300, 2, 64, dtype=dtype).to("cuda", dtype)
-    full = sequence.packed_attention(q, k, k, ends([300]))
-    assert torch.equal(sequence.packed_attention(q, k, k, ends([300]), max_q=1, max_k=300), full)
-    leaves = [t.clone().requires_grad_(True) for t in (q, k, k)]
-    a = torch.autograd.grad(sequence.packed_attention(*leaves, ends([300])), leaves, q)
-    b = torch.autograd.grad(sequence.packed_attention(*leaves, ends([300]), max_q=1, max_k=1), leaves, q)
-    assert all((x.float() - y.float()).abs().max() <= 2 * unit(dtype) * x.float().abs().max() for x, y in zip(a, b))
+    q, k = rand(g, 300, 2, 64, dtype=dtype), rand(g, 300, 2, 64, dtype=dtype)
+    ref = attn_ref(q, k, k, [300], [300], True, 0.125, unit(dtype), q)
+    leaves = [t.to("cuda", dtype).requires_grad_(True) for t in (q, k, k)]
+    for hint in (dict(max_q=1, max_k=300), dict(max_q=1, max_k=1), dict(max_q=0, max_k=0), {}):
+        out = sequence.packed_attention(*leaves, ends([300]), **hint)
+        close(out, ref["o"], ref["to"], "out")
+        for n, t in zip(("gq", "gk", "gv"), torch.autograd.grad(out, leaves, q.to("cuda", dtype))):
+            close(t, ref[n], ref["t" + n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("lq,lk,hq,hk,d", [([1, 1, 1], [300, 1, 5000], 8, 2, 128), ([1] * 5, [129, 2000, 31, 0, 257], 4, 1, 64), ([3, 1], [1500, 700], 4, 4, 32),
+                                           ([40], [3000], 4, 2, 64), ([70, 9], [1100, 2050], 2, 2, 96), ([8], [129], 4, 1, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_attention_few_rows_over_many_keys(lq, lk, hq, hk, d, causal, dtype):
+    check_attention(lq, lk, hq, hk, d, causal, dtype, seed=d)
+    check_attention(lq, lk, hq, hk, d, causal, dtype, seed=d + 1, train=False, hints=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("nq", [1, 3, 50])
+def test_packed_attention_over_caches_with_room(nq, dtype):
+    """Caches [B, room, 2, Hk, D], of which len_k rows are in use; what lies behind them is not touched, NaN or not."""
+    g = gen(nq)
+    B, room, hq, hk, d = 4, 700, 4, 2, 64
+    used = [700, 333, 0, nq]
+    cache = rand(g, B, room, 2, hk, d, dtype=dtype).to("cuda", dtype)
+    for b, n in enumerate(used):
+        cache[b, n:] = float("nan")
+    q = rand(g, B * nq, hq, d, dtype=dtype)
+    flat = cache.view(B * room, 2, hk, d)
+    cu_q, cu_k = ends([nq] * B), ends([room] * B)
+    out = sequence.packed_attention(q.to("cuda", dtype), flat[:, 0], flat[:, 1], cu_q, cu_k, max_q=nq, max_k=room,
+                                    len_k=torch.tensor(used, dtype=torch.int32, device="cuda"))
+    clean = torch.nan_to_num(cache, nan=0.0).cpu().double().view(B * room, 2, hk, d)
+    ref = attn_ref(q, clean[:, 0], clean[:, 1], [nq] * B, [room] * B, True, d ** -0.5, unit(dtype), len_k=used)
+    close(out, ref["o"], ref["to"], "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+def test_packed_attention_rows_of_no_sequence_and_bad_bounds(dtype):
+    g = gen(11)
+    q, k = rand(g, 90, 4, 64, dtype=dtype), rand(g, 70, 2, 64, dtype=dtype)
+    qs, ks, vs = (t.to("cuda", dtype).requires_grad_(True) for t in (q, k, k))
+    cu_q, cu_k = torch.tensor([5, 25, 61], dtype=torch.int32, device="cuda"), torch.tensor([3, 23, 60], dtype=torch.int32, device="cuda")
+    out, lse = sequence.packed_attention(qs, ks, vs, cu_q, cu_k, return_lse=True)
+    go = rand(g, 90, 4, 64, dtype=dtype)
+    grads = torch.autograd.grad(out, (qs, ks, vs), go.to("cuda", dtype))
+    ref = attn_ref(q[5:61], k[3:60], k[3:60], [20, 36], [20, 37], True, 0.125, unit(dtype), go[5:61])
+    close(out[5:61], ref["o"], ref["to"], "out")
+    for t, n, (a, b) in zip(grads, ("gq", "gk", "gv"), ((5, 61), (3, 60), (3, 60))):
+        close(t[a:b], ref[n], ref["t" + n], n)
+        assert not t[:a].any() and not t[b:].any()
+    assert not out[:5].any() and not out[61:].any() and (lse[:5] == -math.inf).all() and (lse[61:] == -math.inf).all()
+    # bounds outside the tensors or in no order are clamped: the call stays inside its tensors
+    wild = torch.tensor([-7, 1000, 3, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    out = sequence.packed_attention(qs, ks, vs, wild, wild)
+    assert all(t.shape == u.shape for t, u in zip(torch.autograd.grad(out, (qs, ks, vs), go.to("cuda", dtype)), (qs, ks, vs)))
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert not sequence.packed_attention(qs, ks, vs, none, none).any()
+    empty = sequence.packed_attention(qs[:0], ks, vs, ends([0]), ends([70]))
+    assert empty.shape == (0, 4, 64)
+    gk = torch.autograd.grad(empty, ks, empty)[0]
+    assert not gk.any()
+    out = sequence.packed_attention(qs, ks[:0], vs[:0], ends([90]), ends([0]))
+    assert not out.any() and not torch.autograd.grad(out, qs, go.to("cuda", dtype))[0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("n,hq,hk,d", [(100, 2, 1, 64), (200, 4, 4, 128), (300, 3, 1, 32)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_packed_attention_what_a_query_does_not_see_stays_out(value, n, hq, hk, d, dtype):
+    """A token that is not finite spoils the results that depend on it and no others, forward and backward."""
+    g = gen(n)
+    q, k, v, go = (rand(g, n, h, d, dtype=dtype).to("cuda", dtype) for h in (hq, hk, hk, hq))
+    cu = ends([n])
+    at, el = n // 2 + 3, 5
+
+    def grads(q, k, v, go):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out = sequence.packed_attention(*leaves, cu)
+        return (out,) + torch.autograd.grad(out, leaves, go)
+    good = grads(q, k, v, go)
+    bad_v = v.clone()
+    bad_v[at, :, el] = value
+    out, gq, gk, gv = grads(q, k, bad_v, go)
+    assert torch.equal(out[:at], good[0][:at]) and not torch.isfinite(out[at:, :, el]).any()
+    others = [i for i in range(d) if i != el]
+    assert torch.equal(out[at:][..., others], good[0][at:][..., others])
+    if not math.isnan(value):
+        assert (out[at:, :, el] == value).all()
+    assert torch.equal(gq[:at], good[1][:at]) and not torch.isfinite(gq[at:]).all(-1).any()
+    bad_k = k.clone()
+    bad_k[at, :, el] = value
+    out, gq, gk, gv = grads(q, bad_k, v, go)
+    assert torch.equal(out[:at], good[0][:at]) and torch.equal(gq[:at], good[1][:at])
+    # a query or an incoming gradient that is not finite reaches the keys that it sees, not the later ones
+    for i in (0, 3):
+        args = [q, k, v, go]
+        args[i] = args[i].clone()
+        args[i][at, :, el] = value
+        out, gq, gk, gv = grads(*args)
+        assert torch.equal(gk[at + 1:], good[2][at + 1:]) and torch.equal(gv[at + 1:], good[3][at + 1:])
+        keep = torch.arange(n, device="cuda") != at
+        assert torch.equal(out[keep], good[0][keep]) and torch.equal(gq[keep], good[1][keep])
+        assert not torch.isfinite(gk[:at + 1]).all(-1).any()
+
+
+@pytest.mark.gpu
+def test_packed_attention_views_of_a_fused_projection_and_shared_inputs():
+    g = gen(12)
+    qkv = rand(g, 150, 8, 64, dtype=torch.bfloat16).to("cuda", torch.bfloat16)      # 4 + 2 + 2 heads
+    cu = ends([100, 50])
+    leaf = qkv.clone().requires_grad_(True)
+    out = sequence.packed_attention(leaf[:, :4], leaf[:, 4:6], leaf[:, 6:], cu)
+    parts = [t.contiguous().requires_grad_(True) for t in (qkv[:, :4], qkv[:, 4:6], qkv[:, 6:])]
+    out2 = sequence.packed_attention(*parts, cu)
+    assert torch.equal(out, out2)
+    go = rand(g, 150, 4, 64, dtype=torch.bfloat16).to("cuda", torch.bfloat16)
+    whole = torch.autograd.grad(out, leaf, go.transpose(0, 1).contiguous().transpose(0, 1))[0]      # a gradient with other strides
+    assert torch.equal(whole, torch.cat(torch.autograd.grad(out2, parts, go), 1))
+    assert torch.equal(torch.autograd.grad(sequence.packed_attention(*parts, cu).sum(), parts[0])[0],       # a broadcast gradient
+                       torch.autograd.grad(sequence.packed_attention(*parts, cu), parts[0], torch.ones_like(out))[0])
+    one = parts[1].detach().clone().requires_grad_(True)        # keys that are the values too
+    got = torch.autograd.grad(sequence.packed_attention(parts[0], one, one, cu), one, go)[0]
+    apart = [one.detach().clone().requires_grad_(True) for _ in range(2)]
+    gk, gv = torch.autograd.grad(sequence.packed_attention(parts[0], *apart, cu), apart, go)
+    assert torch.equal(got, gk + gv)
+    odd = torch.randn(150 * 4 * 24 + 3, generator=g).to("cuda", torch.bfloat16)[3:].view(150, 4, 24)      # not aligned
+    assert torch.equal(sequence.packed_attention(odd, odd, odd, cu), sequence.packed_attention(odd.clone(), odd.clone(), odd.clone(), cu))
+    spread = parts[1].detach()[:, :1].expand(150, 2, 64)        # one key head for both groups, as a broadcast view
+    assert torch.equal(sequence.packed_attention(parts[0].detach(), spread, spread, cu),
+                       sequence.packed_attention(parts[0].detach(), spread.contiguous(), spread.contiguous(), cu))
+
+
+@pytest.mark.gpu
+def test_packed_attention_cache_rows_beyond_32_bits():
+    """Rows so far apart that their offsets in bytes, and in elements, pass 2^32."""
+    g = gen(13)
+    rows, pitch = 2300, 2_000_000
+    big = torch.empty(rows * pitch, device="cuda", dtype=torch.bfloat16)          # 9.2 GB, used in strips
+    k = big.as_strided((rows, 1, 64), (pitch, 64, 1))
+    v = big.as_strided((rows, 1, 64), (pitch, 64, 1), 64)
+    kk, vv = (rand(g, rows, 1, 64, dtype=torch.bfloat16).to("cuda", torch.bfloat16) for _ in range(2))
+    k.copy_(kk)
+    v.copy_(vv)
+    for nq in (1, 200):
+        q = rand(g, nq, 2, 64, dtype=torch.bfloat16).to("cuda", torch.bfloat16)
+        cu_q, cu_k = ends([nq]), ends([rows])
+        assert torch.equal(sequence.packed_attention(q, k, v, cu_q, cu_k), sequence.packed_attention(q, kk, vv, cu_q, cu_k))
+        far = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        near = [t.detach().requires_grad_(True) for t in (q, kk, vv)]
+        got, want = (torch.autograd.grad(sequence.packed_attention(*t, cu_q, cu_k), t, q) for t in (far, near))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del big
+
+
+def two_streams(call, make):
+    """The same call on two streams at once and on the default one: equal results."""
+    a, b = make(1), make(2)
+    want = [call(*a), call(*b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i, (s, args) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[i].append(call(*args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(g, want[i]))
+
+
+def train_call(kind):
+    if kind == "norm":
+        def call(x, w, r, g):
+            leaves = [t.detach().requires_grad_(True) for t in (x, w, r)]
+            y, h = sequence.rms_norm(leaves[0], leaves[1], residual=leaves[2])
+            return (y, h) + torch.autograd.grad((y, h), leaves, (g, g))
+        make = lambda s: (lambda g: [torch.randn(*d, generator=g).cuda() for d in ((300, 256), (256,), (300, 256), (300, 256))])(gen(s))      # noqa: E731
+    elif kind == "rope":
+        def call(q, k, pos, g):
+            leaves = [q.detach().requires_grad_(True), k.detach().requires_grad_(True)]
+            out = sequence.rotary_axes(*leaves, pos, (16, 8, 8))
+            return out + torch.autograd.grad(out, leaves, (g, g[:, :1].contiguous()))
+        make = lambda s: (lambda g: [torch.randn(300, 2, 64, generator=g).cuda(), torch.randn(300, 1, 64, generator=g).cuda(),      # noqa: E731
+                                     torch.randint(0, 5000, (3, 300), generator=g).cuda(), torch.randn(300, 2, 64, generator=g).cuda()])(gen(s))
+    else:
+        nq, nk, hk = (300, 300, 1) if kind == "attention" else (2, 3000, 2)
+
+        def call(q, k, v, g, cu_q, cu_k):
+            leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            out = sequence.packed_attention(*leaves, cu_q, cu_k, max_q=nq, max_k=nk)
+            return (out,) + torch.autograd.grad(out, leaves, g)
+        make = lambda s: (lambda g: [torch.randn(2 * nq, 2, 64, generator=g).cuda().bfloat16(), torch.randn(2 * nk, hk, 64, generator=g).cuda().bfloat16(),      # noqa: E731
+                                     torch.randn(2 * nk, hk, 64, generator=g).cuda().bfloat16(), torch.randn(2 * nq, 2, 64, generator=g).cuda().bfloat16(),
+                                     ends([nq, nq]), ends([nk, nk])])(gen(s))
+    return call, make
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["norm", "rope", "attention", "attention_few"])
+def test_calls_on_two_streams_at_once(kind):
+    two_streams(*train_call(kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["norm", "rope", "attention", "attention_few"])
+def test_captured_forward_and_backward_replay(kind):
+    """Two graphs of the same call, replayed in turn with other inputs and eager work in between, against the eager call."""
+    call, make = train_call(kind)
+    inputs = [make(1), make(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for args in inputs:
+            call(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for args in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(*args))
+        graphs.append(graph)
+    for step in range(4):
+        fresh = [make(10 + 2 * step + i) for i in range(2)]
+        for old, new in zip(inputs, fresh):
+            for a, b in zip(old, new):
+                a.copy_(b)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for out, args in zip(outs, fresh):
+            want = call(*args)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["norm", "rope", "attention"])
+def test_gradients_against_differences(kind):
+    """<gradient, d> against (f(x + e d) - f(x - e d)) / 2 e for a random direction d, in fp32 with sums in 64 bits.  The difference is off by
+    e^2 / 6 times the third derivative along d and by the forward's fp32 error over e: with e = 2^-6 and derivatives of the order of
+    f itself both stay below 1e-3 of the terms that are summed."""
+    g = gen(21)
+    if kind == "norm":
+        x = [torch.randn(6, 64, generator=g).cuda(), torch.randn(64, generator=g).cuda(), torch.randn(6, 64, generator=g).cuda()]
+        f = lambda x, w, r: sequence.rms_norm(x, w, residual=r)      # noqa: E731
+    elif kind == "rope":
+        x = [torch.randn(6, 2, 32, generator=g).cuda(), torch.randn(6, 1, 32, generator=g).cuda()]
+        pos = torch.randint(0, 100, (2, 6), generator=g).cuda()
+        f = lambda q, k: sequence.rotary_axes(q, k, pos, (6, 4), pairing="halves")      # noqa: E731
+    else:
+        x = [torch.randn(40, 4, 32, generator=g).cuda(), torch.randn(40, 2, 32, generator=g).cuda(), torch.randn(40, 2, 32, generator=g).cuda()]
+        f = lambda q, k, v: (sequence.packed_attention(q, k, v, ends([25, 15])),)      # noqa: E731
+    x = [t.requires_grad_(True) for t in x]
+    outs = f(*x)
+    weights = [torch.randn(o.shape, generator=g).cuda() for o in outs]
+    grads = torch.autograd.grad(outs, x, weights)
+    value = lambda ts: sum((o.double() * w.double()).sum().item() for o, w in zip(f(*ts), weights))      # noqa: E731
+    e = 2.0 ** -6
+    for i, t in enumerate(x):
+        d = torch.randn(t.shape, generator=g).cuda()
+        with torch.no_grad():
+            up, down = ([u + s * e * d if j == i else u for j, u in enumerate(x)] for s in (1, -1))
+            diff = (value(up) - value(down)) / (2 * e)
+        terms = grads[i].double() * d.double()
+        assert abs(terms.sum().item() - diff) <= 1e-3 * max(terms.abs().sum().item(), 1.0), (kind, i, terms.sum().item(), diff)
+
+
+@pytest.mark.gpu
+def test_a_block_of_the_operators_together():
+    """norm -> fused projection with a LoRA adapter -> rotary positions -> attention -> projection, and back: the run of a pre-norm block, in
+    fp32, against the same block in 64 bits on the CPU.  Every operator adds a few 2^-24 of its terms; through three projections of 128 terms
+    each the bound of 2^-24 (3 * 128 + 1000) < 1e-4 of the largest result holds."""
+    import lora_layers as L
+    g = gen(31)
+    width, hq, hk, d, lens = 128, 4, 2, 32, [37, 1, 60]
+    T = sum(lens)
+    x, r, gy = (torch.randn(T, width, generator=g) for _ in range(3))
+    w = 1 + 0.1 * torch.randn(width, generator=g)
+    wq, wo = torch.randn((hq + 2 * hk) * d, width, generator=g) / width ** 0.5, torch.randn(width, hq * d, generator=g) / width ** 0.5
+    A, B = torch.randn(width, 4, generator=g) * 0.1, torch.randn(4, (hq + 2 * hk) * d, generator=g) * 0.1
+    pos = torch.stack([torch.cat([torch.arange(n) for n in lens]) * s for s in (1, 3)]).int()
+
+    lin = torch.nn.Linear(width, (hq + 2 * hk) * d, bias=False)
+    lin.weight.data.copy_(wq)
+    mod = L.LoRALinear(lin, rank=4, alpha=4)
+    mod.lora.lora_A.data.copy_(A)
+    mod.lora.lora_B.data.copy_(B)
+    mod = mod.cuda()
+    xs, rs, ws = (t.cuda().requires_grad_(True) for t in (x, r, w))
+    cu = ends(lens)
+    y, h = sequence.rms_norm(xs, ws, residual=rs)
+    qkv = mod(y).view(T, hq + 2 * hk, d)
+    q, k = sequence.rotary_axes(qkv[:, :hq], qkv[:, hq:hq + hk], pos.cuda(), (10, 6), pairing="halves")
+    o = sequence.packed_attention(q, k, qkv[:, hq + hk:], cu, max_q=max(lens), max_k=max(lens))
+    out = h + o.reshape(T, -1) @ wo.cuda().t()
+    got = (out,) + torch.autograd.grad(out, (xs, rs, ws, mod.lora.lora_A, mod.lora.lora_B), gy.cuda())
+
+    X, R, W, a, b = (t.double().requires_grad_(True) for t in (x, r, w, A, B))
+    H = X + R
+    Y = H * (H.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * W
+    QKV = (Y @ wq.double().t() + Y @ a @ b).view(T, hq + 2 * hk, d)
+    angle = pos.double()[[0] * 10 + [1] * 6].t() * torch.tensor([10000.0 ** (-i / 16) for i in range(16)], dtype=torch.float64)
+
+    def turn(t):
+        p, q = t[..., :16], t[..., 16:32]
+        c, s = angle.cos()[:, None], angle.sin()[:, None]
+        return torch.cat([p * c - q * s, p * s + q * c, t[..., 32:]], -1)
+    Q, K, V = turn(QKV[:, :hq]), turn(QKV[:, hq:hq + hk]), QKV[:, hq + hk:]
+    outs, at = [], 0
+    for n in lens:
+        s = torch.einsum("ihd,jhd->hij", Q[at:at + n], K[at:at + n].repeat_interleave(2, 1)) * d ** -0.5
+        p = s.masked_fill(~torch.ones(n, n, dtype=torch.bool).tril(), -math.inf).softmax(-1)
+        outs.append(torch.einsum("hij,jhd->ihd", p, V[at:at + n].repeat_interleave(2, 1)))
+        at += n
+    OUT = H + torch.cat(outs).reshape(T, -1) @ wo.double().t()
+    want = (OUT,) + torch.autograd.grad(OUT, (X, R, W, a, b), gy.double())
+    for name, t, u in zip(("out", "x", "r", "w", "A", "B"), got, want):
+        assert (t.cpu().double() - u).abs().max() <= 1e-4 * u.abs().max(), name
