@@ -35,7 +35,7 @@ struct NormFwd {
     unsigned char* q8;
     float* scales;
     long long ldx, ldr, M;
-    int C, group;
+    int C, group;       // group: log2 of the columns that share a scale, 0: the whole row
     float eps, fmax;
 };
 
@@ -50,14 +50,19 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
     __syncthreads();
     return v;
 }
+// magnitudes as their bit patterns: they order like the numbers, and a NaN is above all of them
+__device__ __forceinline__ unsigned mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ unsigned lane_max(unsigned v, int lanes) {
+    for (int o = lanes / 2; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    return v;
+}
 template <int LPR>
-__device__ __forceinline__ float row_max(float v, float* lds) {
-#pragma unroll
-    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v = nan_max(v, __shfl_xor(v, o, 64));
+__device__ __forceinline__ unsigned row_max(unsigned v, unsigned* lds) {
+    v = lane_max(v, LPR < 64 ? LPR : 64);
     if (LPR <= 64) return v;
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = nan_max(nan_max(lds[0], lds[1]), nan_max(lds[2], lds[3]));
+    v = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
     __syncthreads();
     return v;
 }
@@ -115,7 +120,6 @@ __global__ __launch_bounds__(256) void k_rms_fwd(NormFwd a) {
         }
         const float rs = rsqrtf(row_sum<LPR>(s, lds) / (float)a.C + a.eps);
         if (live && lane == 0 && a.rstd) a.rstd[row] = rs;
-        float m = 0.f;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
             const int c = (i * LPR + lane) * 8;
@@ -136,34 +140,35 @@ __global__ __launch_bounds__(256) void k_rms_fwd(NormFwd a) {
             }
         }
         if (Q8) {
-            if (!a.group) {
+            unsigned m[CPL];
 #pragma unroll
-                for (int i = 0; i < CPL; ++i)
+            for (int i = 0; i < CPL; ++i) {
+                m[i] = 0u;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) m = nan_max(fabsf(h[i][j]), m);
-                m = row_max<LPR>(m, lds);
+                for (int j = 0; j < 8; ++j) m[i] = max(m[i], mag(h[i][j]));
+            }
+            if (a.group) {              // a group is group / 8 neighbouring lanes of one chunk row
+#pragma unroll
+                for (int i = 0; i < CPL; ++i) m[i] = lane_max(m[i], 1 << (a.group - 3));
+            } else {
+#pragma unroll
+                for (int i = 1; i < CPL; ++i) m[0] = max(m[0], m[i]);
+                m[0] = row_max<LPR>(m[0], reinterpret_cast<unsigned*>(lds));
+#pragma unroll
+                for (int i = 1; i < CPL; ++i) m[i] = m[0];
             }
 #pragma unroll
             for (int i = 0; i < CPL; ++i) {
                 const int c = (i * LPR + lane) * 8;
-                if (a.group) {          // a group is group / 8 neighbouring lanes of one chunk row
-                    m = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) m = nan_max(fabsf(h[i][j]), m);
-                    m = nan_max(m, __shfl_xor(m, 1, 64));
-                    m = nan_max(m, __shfl_xor(m, 2, 64));
-                    if (a.group >= 64) m = nan_max(m, __shfl_xor(m, 4, 64));
-                    if (a.group >= 128) m = nan_max(m, __shfl_xor(m, 8, 64));
-                }
-                // (an infinity in y makes the scale infinite and the image NaN: the row is lost either way)
-                const float am = nan_max(m, 5.9604645e-8f), inv = a.fmax / am;
+                // (an infinity in y makes the scale infinite and the image NaN: the group is lost either way)
+                const float am = __uint_as_float(max(m[i], 0x33800000u)), inv = a.fmax / am;
                 if (live && c < a.C) {
                     constexpr int F = Q8 == 1 ? SAM3_FP8_E4M3 : SAM3_FP8_E5M2;
                     *reinterpret_cast<uint2*>(a.q8 + row * a.C + c) =
                         make_uint2(to_fp8x4<F>(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv),
                                    to_fp8x4<F>(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv));
-                    if (a.group ? c % a.group == 0 : c == 0)
-                        a.scales[a.group ? row * (a.C / a.group) + c / a.group : row] = am / a.fmax;
+                    if (a.group ? (c & ((1 << a.group) - 1)) == 0 : c == 0)
+                        a.scales[a.group ? row * (a.C >> a.group) + (c >> a.group) : row] = am / a.fmax;
                 }
             }
         }
@@ -271,8 +276,17 @@ __global__ __launch_bounds__(1024) void k_rms_gw(const float* __restrict__ part,
     __shared__ float s[32][33];
     const int col = threadIdx.x & 31, grp = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
     float v = 0.f;
-    if (c < C)
-        for (int k = grp; k < n; k += 32) v += part[(long long)k * C + c];
+    if (c < C) {
+        int k = grp;
+        for (; k + 7 * 32 < n; k += 8 * 32) {       // eight loads at a time
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = part[(long long)(k + 32 * j) * C + c];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v += x[j];
+        }
+        for (; k < n; k += 32) v += part[(long long)k * C + c];
+    }
     s[grp][col] = v;
     __syncthreads();
     if (grp == 0 && c < C) {
@@ -283,7 +297,9 @@ __global__ __launch_bounds__(1024) void k_rms_gw(const float* __restrict__ part,
     }
 }
 
-// lanes per row and chunks per lane of a row of C elements
+// lanes per row and chunks per lane of a row of C elements.  A wave per row up to 1024 columns, a workgroup per row above: with a wave,
+// 4096 columns of bf16 took 111 us forward and 180 us backward (16411 rows: 4.85 and 2.99 TB/s), with a workgroup 99 and 91 us (5.44 and
+// 5.93 TB/s); at 1024 columns both read 5.4 TB/s and the wave needs no barrier.
 struct RowShape {
     int lpr, cpl;
 };
@@ -294,7 +310,7 @@ RowShape row_shape(int C) {
         while (l < chunks) l *= 2;
         return {l, 1};
     }
-    if (chunks <= 512) return {64, (chunks + 63) / 64};
+    if (chunks <= 128) return {64, (chunks + 63) / 64};
     return {256, (chunks + 255) / 256};
 }
 // workgroups of the backward: its partial sums of the weight gradient are read back by one more launch
@@ -305,8 +321,8 @@ int norm_bwd_blocks(long long M, int C) {
 }
 
 #define NORM_SHAPES(CASE) \
-    CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2) CASE(64, 3) CASE(64, 4) CASE(64, 5) CASE(64, 6) CASE(64, 7) CASE(64, 8) \
-    CASE(256, 3) CASE(256, 4) CASE(256, 5) CASE(256, 6) CASE(256, 7) CASE(256, 8)
+    CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2) \
+    CASE(256, 1) CASE(256, 2) CASE(256, 3) CASE(256, 4) CASE(256, 5) CASE(256, 6) CASE(256, 7) CASE(256, 8)
 
 template <typename T>
 int launch_norm_fwd(const NormFwd& a, int q8, hipStream_t st) {
@@ -373,7 +389,18 @@ __device__ __forceinline__ double position(const void* p, long long i, int type)
     return type == 0 ? (double)((const int*)p)[i] : type == 1 ? (double)((const long long*)p)[i] : (double)((const float*)p)[i];
 }
 
-// FORM 0: adjacent pairs, 1: halves in chunks of 8 (pairs % 8 == 0), 2: halves, single elements
+// 16 bytes from an address that is only aligned to an element
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_any(const T* p) {
+    Raw8<T> v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+}
+
+// FORM 0: adjacent pairs; 1: halves, pairs % 8 == 0: a thread has 8 pairs; 2: halves, any number: a thread has 8 elements and reads their
+// partners, which are not aligned (and which its neighbours read as their own: they come from the cache).
+// 340 MB of bf16 (41472 tokens, 16 + 16 heads of 64, adjacent) in 69 us = 4.9 TB/s; halves 5.0 (heads of 128); halves of 13 pairs 3.1, the
+// chunks across a middle or an end being read by elements.  Loading 2 to 4 chunks per thread before turning the first gained nothing.
 template <typename T, int FORM>
 __global__ __launch_bounds__(256) void k_rotary(Rope a, RopeTable tab, int pos_type) {
     extern __shared__ float2 cs[];      // [TT, pairs]
@@ -392,17 +419,15 @@ __global__ __launch_bounds__(256) void k_rotary(Rope a, RopeTable tab, int pos_t
         const unsigned t = a.row_items > 1 ? (unsigned)(((unsigned long long)it * a.mul_row) >> 32) : it;
         const unsigned rem = it - t * a.row_items;
         const unsigned head = a.head_items > 1 ? (unsigned)(((unsigned long long)rem * a.mul_head) >> 32) : rem;
-        const unsigned e = rem - head * a.head_items;
-        const long long tok = t0 + t;
         const bool isq = head < (unsigned)a.Hq;
-        const int hd = isq ? head : head - a.Hq;
-        const T* src = isq ? (const T*)a.q + tok * a.q_st + hd * a.q_sh : (const T*)a.k + tok * a.k_st + hd * a.k_sh;
-        T* dst = (isq ? (T*)a.qo + (tok * a.Hq + hd) * a.D : (T*)a.ko + (tok * a.Hk + hd) * a.D);
+        const int hd = isq ? head : head - a.Hq, d0 = (int)(rem - head * a.head_items) * 8;
+        const long long row = t0 + t;
+        const T* src = isq ? (const T*)a.q + row * a.q_st + hd * a.q_sh : (const T*)a.k + row * a.k_st + hd * a.k_sh;
+        T* dst = isq ? (T*)a.qo + (row * a.Hq + hd) * a.D : (T*)a.ko + (row * a.Hk + hd) * a.D;
         const float2* c = cs + t * a.pairs;
+        Raw8<T> v, w;
+        float f[8], g[8];
         if (FORM == 0) {
-            const int d0 = e * 8;
-            Raw8<T> v;
-            float f[8];
             v.load(src + d0);
             v.get(f);
 #pragma unroll
@@ -417,12 +442,10 @@ __global__ __launch_bounds__(256) void k_rotary(Rope a, RopeTable tab, int pos_t
             v.set(f);
             v.store(dst + d0);
         } else if (FORM == 1) {
-            const int d0 = e * 8;
+            const int d1 = d0 + a.pairs;
             if (d0 < a.pairs) {
-                Raw8<T> v, w;
-                float f[8], g[8];
                 v.load(src + d0);
-                w.load(src + d0 + a.pairs);
+                w.load(src + d1);
                 v.get(f);
                 w.get(g);
 #pragma unroll
@@ -433,23 +456,42 @@ __global__ __launch_bounds__(256) void k_rotary(Rope a, RopeTable tab, int pos_t
                     g[j] = x * z.y + y * z.x;
                 }
                 v.set(f);
-                w.set(g);
                 v.store(dst + d0);
-                w.store(dst + d0 + a.pairs);
+                w.set(g);
+                w.store(dst + d1);
             } else {
-                Raw8<T> v;
-                v.load(src + d0 + a.pairs);
-                v.store(dst + d0 + a.pairs);
+                v.load(src + d1);
+                v.store(dst + d1);
             }
         } else {
-            if ((int)e < a.pairs) {
-                const float x = ld1(src + e), y = ld1(src + e + a.pairs);
-                const float2 z = c[e];
-                st1(dst + e, x * z.x - y * z.y);
-                st1(dst + e + a.pairs, x * z.y + y * z.x);
-            } else {
-                dst[e + a.pairs] = src[e + a.pairs];
+            v.load(src + d0);
+            if (d0 < 2 * a.pairs) {
+                if (d0 + 8 <= a.pairs) {
+                    w = load_any(src + d0 + a.pairs);
+                } else if (d0 >= a.pairs && d0 + 8 <= 2 * a.pairs) {
+                    w = load_any(src + d0 - a.pairs);
+                } else {            // the chunks across the middle and the end
+                    T e[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int i = d0 + j;
+                        e[j] = src[i < a.pairs ? i + a.pairs : i < 2 * a.pairs ? i - a.pairs : i];
+                    }
+                    __builtin_memcpy(&w, e, sizeof(e));
+                }
+                v.get(f);
+                w.get(g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = d0 + j;
+                    const bool second = i >= a.pairs;
+                    const float2 z = c[i < 2 * a.pairs ? (second ? i - a.pairs : i) : 0];
+                    const float r = second ? g[j] * z.y + f[j] * z.x : f[j] * z.x - g[j] * z.y;
+                    if (i < 2 * a.pairs) f[j] = r;
+                }
+                v.set(f);
             }
+            v.store(dst + d0);
         }
     }
 }
@@ -478,7 +520,7 @@ int sam3_seq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int6
         return sam3_seq_fail(EINVAL_, "rms norm: tensors must be 16-byte aligned");
     if (ldx < C || bad_pitch(ldx, dtype) || (residual && (ldr < C || bad_pitch(ldr, dtype))))
         return sam3_seq_fail(EINVAL_, "rms norm: bad row pitch");
-    const NormFwd a{x, residual, weight, y, h_out, rstd_out, (unsigned char*)q8, scales, ldx, ldr, M, C, group, eps,
+    const NormFwd a{x, residual, weight, y, h_out, rstd_out, (unsigned char*)q8, scales, ldx, ldr, M, C, !group ? 0 : group == 32 ? 5 : group == 64 ? 6 : 7, eps,
                     fmt == SAM3_FP8_E4M3 ? 448.f : 57344.f};
     const int q = !q8 ? 0 : fmt == SAM3_FP8_E4M3 ? 1 : 2;
     return dtype == 0 ? launch_norm_fwd<bf16_t>(a, q, (hipStream_t)stream) : launch_norm_fwd<float>(a, q, (hipStream_t)stream);
@@ -526,11 +568,11 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
         (k && (bad_pitch(k_st, dtype) || bad_pitch(k_sh, dtype))))
         return sam3_seq_fail(EINVAL_, "rotary: tensors and strides must keep 16-byte accesses aligned");
     const int form = !halves ? 0 : pairs % 8 == 0 ? 1 : 2;
-    const int per_head = form == 0 ? D / 8 : form == 1 ? pairs / 8 + (D - 2 * pairs) / 8 : D - pairs;
+    const int per_head = form == 1 ? (D - pairs) / 8 : D / 8;
     Rope a{q, k, positions, q_out, k_out, q_st, q_sh, k_st, k_sh, pos_sa, pos_st, T, Hq, Hk, D, pairs, 0, 0, 0, 0, 0, 0, inverse ? -1.f : 1.f};
     a.head_items = per_head;
     a.row_items = (unsigned)per_head * (Hq + Hk);
-    a.TT = T >= 4096 ? 8 : T >= 1024 ? 4 : 1;
+    a.TT = T >= 16384 ? 8 : T >= 2048 ? (int)(T / 2048) : 1;      // tokens that share a table, as long as there are 2048 workgroups
     a.mul_head = magic(a.head_items);
     a.mul_row = magic(a.row_items);
     if ((uint64_t)a.TT * a.row_items * a.row_items >= 0x100000000ull) a.TT = 1;

@@ -29,6 +29,7 @@ __all__ = ["rms_norm", "rms_norm_q8", "rotary_axes", "packed_attention", "FP8_E4
 
 FP8_E4M3, FP8_E5M2 = _ffi.FP8_E4M3, _ffi.FP8_E5M2
 _FP8_TYPES = {FP8_E4M3: torch.float8_e4m3fn, FP8_E5M2: torch.float8_e5m2}
+_TYPE_CODES = {torch.bfloat16: _ffi.DT_BF16, torch.float32: _ffi.DT_F32}
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
@@ -42,41 +43,55 @@ def _need(ok, what: str) -> None:
         raise ValueError(what)
 
 
-def _activation(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> int:
-    """Type code of an activation; its place and type are ``like``'s."""
+def _activation(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
+    """Checks an activation; its place and type are ``like``'s."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if like is not None and (t.device != like.device or t.dtype != like.dtype):
         raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if t.dtype not in (torch.bfloat16, torch.float32):
+    if t.dtype not in _TYPE_CODES:
         raise LoRAKernelError(f"sam3_lora_amd: activations must be bfloat16 or float32, got {t.dtype} for {name}")
     if not t.is_cuda:
         raise LoRAKernelError(f"sam3_lora_amd: the sequence operators run only on an AMD GPU (got a {t.device} tensor for {name}); "
                               "there is no CPU fallback.")
-    return _ffi.DT_BF16 if t.dtype == torch.bfloat16 else _ffi.DT_F32
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
     """The tensors' device as the current one, where it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)      # torch.cuda.current_stream() without the objects around it
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with unit stride inside a row, and its address and other strides in multiples of 16 bytes (a copy where it has not)."""
-    per = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % per == 0 and s >= 0 for s in t.stride()[:-1]):
-        return t
+    """``t`` with unit stride inside a row, and its address and other strides in multiples of 16 bytes (a copy where it has not); its
+    last dimension is a multiple of 8."""
+    if t.data_ptr() & 15 == 0:
+        if t.is_contiguous():
+            return t
+        per = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(s % per == 0 and s >= 0 for s in t.stride()[:-1]):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of ``t``'s shape (the cheapest way to one)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 # ----------------------------------------------------------------------------------------------------------- RMS norm
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
-    t = t.detach().reshape(-1, width)
-    t = _aligned(t)
+    t = _aligned(t if t.dim() == 2 else t.reshape(-1, width))
     return t if t.shape[0] <= 1 or t.stride(0) >= width else t.contiguous()
 
 
@@ -88,24 +103,23 @@ def _norm_fwd(x, residual, weight, eps, want_y, want_rstd, q8=None):
     """(y, h, rstd, image, scales) of contiguous outputs; q8 = (group, fmt) or None."""
     width = x.shape[-1]
     x2 = _rows(x, width)
-    r2 = None if residual is None else _rows(residual, width)
-    w = _aligned(weight.detach())
     m = x2.shape[0]
-    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)      # noqa: E731
-    y = new() if want_y else None
-    h = new() if residual is not None else None
-    rstd = torch.empty(m, dtype=torch.float32, device=x.device) if want_rstd else None
+    r2, ldr, h = None, 0, None
+    if residual is not None:
+        r2 = _rows(residual, width)
+        ldr, h = _pitch(r2), _new(x)
+    w = _aligned(weight)
+    y = _new(x) if want_y else None
+    rstd = x.new_empty(m, dtype=torch.float32) if want_rstd else None
     image = scales = None
     group, fmt = q8 or (0, FP8_E4M3)
     if q8 is not None:
-        image = torch.empty(x.shape, dtype=_FP8_TYPES[fmt], device=x.device)
-        scales = torch.empty(x.shape[:-1] + (width // group if group else 1,), dtype=torch.float32, device=x.device)
-    ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+        image = x.new_empty(x.shape, dtype=_FP8_TYPES[fmt])
+        scales = x.new_empty(x.shape[:-1] + (width // group if group else 1,), dtype=torch.float32)
     with _on(x.device):
         _check(_ffi.load().sam3_seq_rms_norm_fwd(
-            x2.data_ptr(), _pitch(x2), ptr(r2), 0 if r2 is None else _pitch(r2), w.data_ptr(), ptr(y), ptr(h), ptr(rstd), ptr(image),
-            ptr(scales), group, fmt, m, width, eps, _ffi.DT_BF16 if x.dtype == torch.bfloat16 else _ffi.DT_F32, _stream(x.device)),
-            "sam3_seq_rms_norm_fwd")
+            x2.data_ptr(), _pitch(x2), _ptr(r2), ldr, w.data_ptr(), _ptr(y), _ptr(h), _ptr(rstd), _ptr(image), _ptr(scales), group, fmt, m,
+            width, eps, _TYPE_CODES[x.dtype], _stream(x.device)), "sam3_seq_rms_norm_fwd")
     return y, h, rstd, image, scales
 
 
@@ -128,10 +142,10 @@ class _RMSNorm(torch.autograd.Function):
         if gy is None:      # only the stream was used
             return gh if ctx.needs_input_grad[0] else None, gh if ctx.needs_input_grad[1] else None, None, None
         width = h.shape[-1]
-        h2, w = _rows(h, width), _aligned(weight.detach())
+        h2, w = _rows(h, width), _aligned(weight)
         gy2 = _aligned(gy.contiguous())
         gh2 = None if gh is None or not need_x else _aligned(gh.contiguous())
-        gx = torch.empty(h.shape, dtype=h.dtype, device=h.device) if need_x else None
+        gx = _new(h) if need_x else None
         gw = torch.empty_like(weight, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
         m = h2.shape[0]
         if m == 0:
@@ -139,12 +153,11 @@ class _RMSNorm(torch.autograd.Function):
         lib = _ffi.load()
         ws = None
         if gw is not None:
-            ws = torch.empty(lib.sam3_seq_rms_norm_bwd_workspace_bytes(m, width), dtype=torch.uint8, device=h.device)
-        ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+            ws = h.new_empty(lib.sam3_seq_rms_norm_bwd_workspace_bytes(m, width), dtype=torch.uint8)
         with _on(h.device):
             _check(lib.sam3_seq_rms_norm_bwd(
-                gy2.data_ptr(), ptr(gh2), h2.data_ptr(), _pitch(h2), w.data_ptr(), rstd.data_ptr(), ptr(gx), ptr(gw), m, width,
-                _ffi.DT_BF16 if h.dtype == torch.bfloat16 else _ffi.DT_F32, ptr(ws), 0 if ws is None else ws.numel(), _stream(h.device)),
+                gy2.data_ptr(), _ptr(gh2), h2.data_ptr(), _pitch(h2), w.data_ptr(), rstd.data_ptr(), _ptr(gx), _ptr(gw), m, width,
+                _TYPE_CODES[h.dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream(h.device)),
                 "sam3_seq_rms_norm_bwd")
         return gx if ctx.needs_input_grad[0] else None, gx if ctx.needs_input_grad[1] else None, gw, None
 
@@ -212,24 +225,25 @@ def _rotation_table(sections: Tuple[int, ...], theta: float, spectrum: str):
 
 def _tokens(t: torch.Tensor) -> torch.Tensor:
     """[..., heads, D] -> [tokens, heads, D], a view where it can be, with strides that the kernel takes."""
-    return _aligned(t.detach().reshape(-1, t.shape[-2], t.shape[-1]))
+    return _aligned(t if t.dim() == 3 else t.reshape(-1, t.shape[-2], t.shape[-1]))
 
 
 def _rotate(q, k, positions, table, halves, inverse):
     turns, axis, pairs = table
     q3 = _tokens(q)
-    k3 = None if k is None else _tokens(k)
-    pos = positions.reshape(positions.shape[0], -1)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
     t, hq, d = q3.shape
+    qs = q3.stride()
+    k3, hk, ks, ko = None, 0, (0, 0), None
+    if k is not None:
+        k3 = _tokens(k)
+        hk, ks, ko = k3.shape[1], k3.stride(), _new(k)
+    pos = positions if positions.dim() == 2 else positions.reshape(positions.shape[0], -1)
+    qo = _new(q)
     with _on(q.device):
         _check(_ffi.load().sam3_seq_rotary(
-            q3.data_ptr(), q3.stride(0), q3.stride(1), None if k is None else k3.data_ptr(), 0 if k is None else k3.stride(0),
-            0 if k is None else k3.stride(1), qo.data_ptr(), None if k is None else ko.data_ptr(), pos.data_ptr(), pos.stride(0),
-            pos.stride(1), _POSITION_TYPES[pos.dtype], pos.shape[0], turns, axis, pairs, int(halves), int(inverse), t, hq,
-            0 if k is None else k3.shape[1], d, _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32, _stream(q.device)),
-            "sam3_seq_rotary")
+            q3.data_ptr(), qs[0], qs[1], _ptr(k3), ks[0], ks[1], qo.data_ptr(), _ptr(ko), pos.data_ptr(), pos.stride(0), pos.stride(1),
+            _POSITION_TYPES[pos.dtype], pos.shape[0], turns, axis, pairs, halves, inverse, t, hq, hk, d, _TYPE_CODES[q.dtype],
+            _stream(q.device)), "sam3_seq_rotary")
     return qo, ko
 
 
@@ -299,21 +313,21 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
 def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse, want_stats=False):
     tq, hq, d = q.shape
     tk, hk = k.shape[:2]
-    q, k, v = _aligned(q.detach()), _aligned(k.detach()), _aligned(v.detach())
-    out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(tq, hq, dtype=torch.float32, device=q.device) if want_lse else None
-    stats = torch.empty(tq, hq, 2, dtype=torch.float32, device=q.device) if want_stats else None
-    dt = _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    out = _new(q)
+    lse = q.new_empty((tq, hq), dtype=torch.float32) if want_lse else None
+    stats = q.new_empty((tq, hq, 2), dtype=torch.float32) if want_stats else None
+    dt = _TYPE_CODES[q.dtype]
     lib = _ffi.load()
-    b = cu_q.numel() - 1
+    b = cu_q.shape[0] - 1
     nbytes = lib.sam3_seq_attn_fwd_workspace_bytes(tq, b, hq, hk, d, max_q, max_k, dt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
     with _on(q.device):
         _check(lib.sam3_seq_attn_fwd(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-            cu_q.data_ptr(), cu_k.data_ptr(), None if len_k is None else len_k.data_ptr(), out.data_ptr(),
-            None if lse is None else lse.data_ptr(), None if stats is None else stats.data_ptr(), tq, tk, b, hq, hk, d, max_q, max_k,
-            int(causal), scale, dt, None if ws is None else ws.data_ptr(), nbytes, _stream(q.device)), "sam3_seq_attn_fwd")
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(),
+            _ptr(len_k), out.data_ptr(), _ptr(lse), _ptr(stats), tq, tk, b, hq, hk, d, max_q, max_k, causal, scale, dt, _ptr(ws), nbytes,
+            _stream(q.device)), "sam3_seq_attn_fwd")
     return out, lse, stats
 
 
@@ -339,18 +353,18 @@ class _PackedAttention(torch.autograd.Function):
         max_q, max_k, causal, scale = ctx.how
         tq, hq, d = q.shape
         tk, hk = k.shape[:2]
-        q, k, v, go = (_aligned(t.detach()) for t in (q, k, v, go))
-        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        q, k, v, go = _aligned(q), _aligned(k), _aligned(v), _aligned(go)
+        gq, gk, gv = _new(q), _new(k), _new(v)
+        qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), go.stride()
         lib = _ffi.load()
         nbytes = lib.sam3_seq_attn_bwd_workspace_bytes(tq, hq)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
         with _on(q.device):
             _check(lib.sam3_seq_attn_bwd(
-                q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                go.data_ptr(), go.stride(0), go.stride(1), out.data_ptr(), stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
-                gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq, tk, cu_q.numel() - 1, hq, hk, d, max_q, max_k, int(causal), scale,
-                _ffi.DT_BF16 if q.dtype == torch.bfloat16 else _ffi.DT_F32, ws.data_ptr(), nbytes, _stream(q.device)),
-                "sam3_seq_attn_bwd")
+                q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], go.data_ptr(), gs[0], gs[1],
+                out.data_ptr(), stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq, tk,
+                cu_q.shape[0] - 1, hq, hk, d, max_q, max_k, causal, scale, _TYPE_CODES[q.dtype], ws.data_ptr(), nbytes,
+                _stream(q.device)), "sam3_seq_attn_bwd")
         need = ctx.needs_input_grad
         return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None) + (None,) * 7
 
