@@ -31,7 +31,8 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 struct Attn {
     const void *q, *k, *v, *go, *o;
     void *out, *gq, *gk, *gv;
-    float *lse, *delta;         // [Tq, Hq]
+    float *lse;                 // [Tq, Hq]
+    float *rowstat;             // [3, Hk, Tq, G] of the backward: exponent base (16 bits: with the sum's logarithm), D, 1 / sum (32 bits only)
     float2* stats;              // [Tq, Hq]: exponent base (powers of two) and 1 / sum of each row; 0 for a row that sees no key
     const int *cu_q, *cu_k, *len_k;
     long long q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
@@ -89,16 +90,20 @@ __device__ __forceinline__ void frag_of(Frag<float>& f, const float* p) {
     for (int j = 0; j < 8; ++j) f.v[j] = p[j];
 }
 
-// A tile of rows in LDS: rows of DP elements in chunks of 16 bytes, the chunks of a row permuted by f(row) so that neighbouring rows'
-// same chunk lies in different banks.
+// A tile of rows in LDS: rows of DP elements in chunks of 16 bytes, the chunks of a row permuted by an exclusive or with f(row).  LDS has
+// 64 banks of 4 bytes, a line of 16 chunks.  Reading rows, 16 lanes read the same chunk of 16 neighbouring rows: f takes them to 16
+// different places of a line.  Reading columns, lanes read the same four chunks of 4 neighbouring rows: f's upper bits come from the
+// row's lower ones, so that these fill a line too.  (With f = row % 8 two thirds of the LDS's busy time were bank conflicts.)
 template <typename T, int DP>
 struct Tile {
     static constexpr int EPC = 16 / sizeof(T);          // elements per chunk
     static constexpr int CPR = DP / EPC;                // chunks per row
     static constexpr int ROWB = DP * sizeof(T);
+    static constexpr int PERIOD = 16;                   // f(row) = f(row + 16)
     static __device__ __forceinline__ int f(int row) {
-        constexpr int rows_per_line = CPR >= 8 ? 1 : 8 / CPR;
-        return (row / rows_per_line) & (CPR < 8 ? CPR - 1 : 7);
+        if (CPR >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+        if (CPR == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        return (row >> 2) & 3;
     }
     static __device__ __forceinline__ int chunk_at(int row, int c) { return row * ROWB + ((c ^ f(row)) << 4); }
     // k-step s (16 elements) of row `row`: elements 16 s + 8 h .. + 7
@@ -268,34 +273,64 @@ __device__ __forceinline__ Place place(unsigned id, int pairs, int tiles) {
     return Place{xcd % lanes + lanes * (slot / per), tiles - 1 - tile};        // tile < 0: none
 }
 
-// 16 bytes per lane straight into LDS: lane l's go to lds + 16 l.  The instruction is written out because the compiler would wait for
-// every such load before any later read of LDS, and the loads of the next tile have to stay in flight; whoever reads waits at the
-// barrier in front (vmcnt(0)).
-__device__ __forceinline__ void load_to_lds(const void* p, char* lds) {
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory", "m0");
+// 16 bytes per lane straight into LDS, lane l's to lds + 16 l, from an address of the wave and 32 bits of the lane.  The instruction is
+// written out because the compiler would wait for every such load before any later read of LDS, and the loads of the next tile have to
+// stay in flight; whoever reads waits at the barrier in front (wait_loads).
+// Its destination is M0; the address goes through a scalar move inside the block: a scalar register that a vector instruction wrote (the
+// compiler's readfirstlane) may only be read by a memory instruction five wait states later, by a scalar one at once.
+__device__ __forceinline__ unsigned lds_at(const void* lds) {
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)lds);
 }
-// A tile of whole rows into LDS by 256 threads without passing through registers.  The chunks' permutation is on the address that a
-// lane reads; chunks behind the head's end are left alone (they were cleared once).
-template <typename T, int DP, int ROWS>
+__device__ __forceinline__ const void* of_wave(const void* p) {
+    const unsigned long long u = (unsigned long long)p;
+    const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)u), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
+    return (const void*)((unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
+    unsigned long long tmp;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(tmp) : "s"(lds), "v"(off), "s"(of_wave(base)) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(const void* p, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+// 4 bytes per lane
+__device__ __forceinline__ void word_to_lds(const void* base, unsigned off, unsigned lds) {
+    unsigned long long tmp;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dword %2, %0"
+                 : "=&s"(tmp) : "s"(lds), "v"(off), "s"(of_wave(base)) : "memory", "m0");
+}
+// Waits until at most N loads are under way.  The builtin (the compiler then knows that its own earlier loads have arrived: it would
+// otherwise wait for one of them inside the loop, and with it for the loads into LDS that it does not know of), and a fence for it.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+// A tile of whole rows into LDS by NT threads without passing through registers, in rounds of RPI rows.  The chunks' permutation is on
+// the address that a lane reads; chunks behind the head's end are left alone (they were cleared once).
+template <typename T, int DP, int ROWS, int NT = 256>
 struct Dma {
     typedef Tile<T, DP> L;
-    static constexpr int RPI = 256 / L::CPR;        // rows of one round of the workgroup
-    static constexpr int N = ROWS / RPI;
-    static_assert(ROWS % RPI == 0 && (RPI % 8 == 0 || N == 1), "the permutation must not depend on the round");
-    long long off;      // bytes from the tile's first row
-    bool on;
+    static constexpr int RPI = NT / L::CPR, N = ROWS / RPI, P = RPI >= L::PERIOD ? 1 : L::PERIOD / RPI;
+    static_assert(ROWS % RPI == 0, "whole rounds");
+    unsigned off[P];        // bytes from the tile's first row, for the rounds i = p, p + P, ... (a tile spans less than 2^31: check_tensor)
+    bool on[P];
     __device__ __forceinline__ Dma(long long st, int D) {
-        const int row = threadIdx.x / L::CPR, c = (threadIdx.x % L::CPR) ^ L::f(row);
-        off = ((long long)row * st + c * L::EPC) * (long long)sizeof(T);
-        on = c * L::EPC < D;
-    }
-    __device__ __forceinline__ void load(const T* tile, long long st, char* lds) const {
-        if (on) {
+        const int row = (threadIdx.x % NT) / L::CPR, slot = threadIdx.x % L::CPR;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                load_to_lds(reinterpret_cast<const char*>(tile + i * RPI * st) + off, lds + i * 4096 + (threadIdx.x >> 6) * 1024);
+        for (int p = 0; p < P; ++p) {
+            const int e = (slot ^ L::f(p * RPI + row)) * L::EPC;
+            off[p] = (unsigned)((row * st + e) * (long long)sizeof(T));
+            on[p] = e < D;
         }
+    }
+    // lds: where the wave's first 1024 bytes go (the tile's address + 1024 times the wave)
+    __device__ __forceinline__ void load(const T* tile, long long st, unsigned lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (on[i % P])
+                load_to_lds(tile + i * RPI * st, off[i % P], lds + i * NT * 16);
     }
 };
 
@@ -363,12 +398,12 @@ struct FwdState {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void k_attn_fwd(Attn a, int tiles, unsigned first_rest) {
+__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_fwd(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     constexpr int BN = FwdCfg<T, DP>::BN, TB = BN * L::ROWB;
     constexpr int KS = DP / 16, DT = DP / 32;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB];        // two tiles of keys and values
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T* out = (T*)a.out;
     if (blockIdx.x >= first_rest) {         // rows of no sequence
         const Rest z = rest(a.cu_q, a.B, a.Tq);
@@ -389,6 +424,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_fwd(Attn a, int tiles, unsigned
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
     const float c2 = a.scale * LOG2E;
     const Dma<T, DP, BN> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    const unsigned at_lds = lds_at(lds) + wave * 1024;
     if (a.D < DP) {
         for (int i = threadIdx.x; i < 4 * TB / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -413,14 +449,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_fwd(Attn a, int tiles, unsigned
         const int nfull = jall / BN;        // steps whose keys are all there and all seen: no mask, and loaded while the one before computes
         if (nfull > 0) {
             __syncthreads();
-            dk.load(k, a.k_st, lds);
-            dv.load(v, a.v_st, lds + TB);
+            dk.load(k, a.k_st, at_lds);
+            dv.load(v, a.v_st, at_lds + TB);
             for (int t = 0; t < nfull; ++t) {
                 char* now = lds + (t & 1) * 2 * TB;
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                wait_loads<0>();
                 __syncthreads();            // tile t is there, and nobody reads the other buffer any more
                 if (t + 1 < nfull) {
-                    char* next = lds + ((t + 1) & 1) * 2 * TB;
+                    const unsigned next = at_lds + ((t + 1) & 1) * 2 * TB;
                     dk.load(k + (long long)(t + 1) * BN * a.k_st, a.k_st, next);
                     dv.load(v + (long long)(t + 1) * BN * a.v_st, a.v_st, next + TB);
                 }
@@ -460,28 +496,6 @@ struct FewCfg {
     static constexpr int TB = 32 * DP * (int)sizeof(T), LDS = 4 * TB;
 };
 
-template <typename T, int DP>
-struct WaveDma {
-    typedef Tile<T, DP> L;
-    static constexpr int RPI = 64 / L::CPR, N = 32 / RPI, P = RPI >= 8 ? 1 : 8 / RPI;
-    long long off[P];       // bytes from the tile's first row, for the rounds i = p, p + P, ... (the permutation repeats every 8 rows)
-    bool on[P];
-    __device__ __forceinline__ WaveDma(long long st, int D) {
-        const int row = (threadIdx.x & 63) / L::CPR, slot = (threadIdx.x & 63) % L::CPR;
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const int e = (slot ^ L::f(p * RPI + row)) * L::EPC;
-            off[p] = (row * st + e) * (long long)sizeof(T);
-            on[p] = e < D;
-        }
-    }
-    __device__ __forceinline__ void load(const T* tile, long long st, char* lds) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (on[i % P]) load_to_lds(reinterpret_cast<const char*>(tile + i * RPI * st) + off[i % P], lds + i * 1024);
-    }
-};
-
 struct Few {
     int tiles, splits, chunk;       // row tiles of a pair, chunks of the longest sequence, keys of a chunk
     float* part;                    // [splits, Tq * Hq, D] unnormalised results, and
@@ -515,7 +529,8 @@ __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_a
     const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G};
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
     const float c2 = a.scale * LOG2E;
-    const WaveDma<T, DP> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    const Dma<T, DP, 32, 64> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    const unsigned at_lds = lds_at(mine);
     for (long long rr = (long long)pl.tile * 32; rr < R; rr += (long long)f.tiles * 32) {
         const int r0 = (int)rr, row = r0 + (lane & 31);
         const bool live = row < R;
@@ -541,19 +556,21 @@ __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_a
             int blk = 0, buf = 0;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (blk < full) {
-                dk.load(k + (long long)(begin + blk * 32) * a.k_st, a.k_st, mine);
-                dv.load(v + (long long)(begin + blk * 32) * a.v_st, a.v_st, mine + TB);
+                dk.load(k + (long long)(begin + blk * 32) * a.k_st, a.k_st, at_lds);
+                dv.load(v + (long long)(begin + blk * 32) * a.v_st, a.v_st, at_lds + TB);
+                wait_loads<0>();        // (for the rows' own loads too, which the loop would otherwise wait for)
             }
             for (; blk < full; ++blk, buf ^= 1) {
-                char *now = mine + buf * 2 * TB, *next = mine + (buf ^ 1) * 2 * TB;
+                char* now = mine + buf * 2 * TB;
+                const unsigned next = at_lds + (buf ^ 1) * 2 * TB;
                 // what was read of the other buffer has arrived; then its new loads, and the wait for all but those
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 if (blk + 1 < full) {
                     dk.load(k + (long long)(begin + (blk + 1) * 32) * a.k_st, a.k_st, next);
                     dv.load(v + (long long)(begin + (blk + 1) * 32) * a.v_st, a.v_st, next + TB);
-                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * WaveDma<T, DP>::N) : "memory");
+                    wait_loads<2 * Dma<T, DP, 32, 64>::N>();
                 } else {
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    wait_loads<0>();
                 }
                 st.template step<false>(now, now + TB, lane, c2, 32);
             }
@@ -684,12 +701,12 @@ struct GqState {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void k_attn_gq(Attn a, int tiles, unsigned first_rest) {
+__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     constexpr int BN = GqCfg<T, DP>::BN, TB = BN * L::ROWB;
     constexpr int KS = DP / 16, DT = DP / 32;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T* gq = (T*)a.gq;
     if (blockIdx.x >= first_rest) {
         const Rest z = rest(a.cu_q, a.B, a.Tq);
@@ -707,6 +724,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_gq(Attn a, int tiles, unsigned 
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
     const float c2 = a.scale * LOG2E;
     const Dma<T, DP, BN> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    const unsigned at_lds = lds_at(lds) + wave * 1024;
     if (a.D < DP) {
         for (int i = threadIdx.x; i < 4 * TB / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -743,22 +761,28 @@ __global__ __launch_bounds__(256, 2) void k_attn_gq(Attn a, int tiles, unsigned 
             }
         }
         st.delta = delta + __shfl_xor(delta, 32, 64);
-        if (live && h == 0) a.delta[at] = st.delta;
         const float2 stat = live ? a.stats[at] : make_float2(0.f, 0.f);
         st.base = stat.x;
+        if (live && h == 0) {
+            const long long all = a.Tq * a.Hq;
+            float* to = a.rowstat + ((long long)kv * a.Tq + sq.begin) * a.G + row;        // the rows of a pair lie in order
+            to[0] = sizeof(T) == 4 ? stat.x : stat.x - __builtin_amdgcn_logf(stat.y);
+            to[all] = st.delta;
+            if (sizeof(T) == 4) to[2 * all] = stat.y;
+        }
 #pragma unroll
         for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
         const int nfull = jall / BN;
         if (nfull > 0) {
             __syncthreads();
-            dk.load(k, a.k_st, lds);
-            dv.load(v, a.v_st, lds + TB);
+            dk.load(k, a.k_st, at_lds);
+            dv.load(v, a.v_st, at_lds + TB);
             for (int t = 0; t < nfull; ++t) {
                 char* now = lds + (t & 1) * 2 * TB;
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                wait_loads<0>();
                 __syncthreads();
                 if (t + 1 < nfull) {
-                    char* next = lds + ((t + 1) & 1) * 2 * TB;
+                    const unsigned next = at_lds + ((t + 1) & 1) * 2 * TB;
                     dk.load(k + (long long)(t + 1) * BN * a.k_st, a.k_st, next);
                     dv.load(v + (long long)(t + 1) * BN * a.v_st, a.v_st, next + TB);
                 }
@@ -793,50 +817,90 @@ struct GkvCfg {
     static constexpr int WAVES = sizeof(T) * DP > 256 ? 1 : 2;         // per SIMD
 };
 
-// the rows of a step, for a lane's part of each round of loads: token and head of row r0 + i RPI + threadIdx / CPR
-template <typename T, int DP, int BR>
+// The rows of a step (BR of them) of q and go into LDS.  EVEN: the heads of a group divide a step, so a lane's rows stay where they are
+// from step to step and only the wave's address moves.  Otherwise each lane follows its rows: a step is adv_t tokens and adv_g heads, one
+// token more where the head leaves the group.
+template <typename T, int DP, int BR, bool EVEN>
 struct RowDma {
     typedef Tile<T, DP> L;
     static constexpr int RPI = 256 / L::CPR, N = (BR + RPI - 1) / RPI;
-    static_assert((RPI % 8 == 0 && BR % RPI == 0) || N == 1, "the permutation must not depend on the round");
-    int tok[N], g[N], c;
-    bool on;
-    __device__ __forceinline__ RowDma(int r0, int G, int D) {
-        const int row = threadIdx.x / L::CPR;
-        c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC;
-        on = c < D && row < BR;
+    static_assert(BR % RPI == 0 || N == 1, "whole rounds");
+    const T *q, *go;
+    unsigned oq[N], og[N];
+    bool on[N];
+    __device__ __forceinline__ RowDma(const T* q0, const T* go0, const Attn& a, int r0) : q(q0 + r0 / a.G * a.q_st), go(go0 + r0 / a.G * a.go_st) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            tok[i] = (r0 + i * RPI + row) / G;
-            g[i] = r0 + i * RPI + row - tok[i] * G;
+            const int row = i * RPI + threadIdx.x / L::CPR, c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC, t = row / a.G, g = row - t * a.G;
+            on[i] = c < a.D && row < BR;
+            oq[i] = (unsigned)((t * a.q_st + g * a.q_sh + c) * (long long)sizeof(T));
+            og[i] = (unsigned)((t * a.go_st + g * a.go_sh + c) * (long long)sizeof(T));
         }
     }
-    __device__ __forceinline__ void advance(int G, int dt, int dg) {       // BR = dt G + dg
+    __device__ __forceinline__ void advance(const Attn& a) {
+        q += BR / a.G * a.q_st;
+        go += BR / a.G * a.go_st;
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+v"(oq[i]), "+v"(og[i]));        // (registers, not scratch: a reload waits for the loads)
+    }
+    __device__ __forceinline__ void load(unsigned lq, unsigned lg) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (on[i]) {
+                load_to_lds(q, oq[i], lq + i * 4096);
+                load_to_lds(go, og[i], lg + i * 4096);
+            }
+    }
+};
+template <typename T, int DP, int BR>
+struct RowDma<T, DP, BR, false> {
+    typedef Tile<T, DP> L;
+    static constexpr int RPI = 256 / L::CPR, N = (BR + RPI - 1) / RPI;
+    const T *q[N], *go[N];
+    int g[N];
+    bool on[N];
+    __device__ __forceinline__ RowDma(const T* q0, const T* go0, const Attn& a, int r0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            tok[i] += dt;
-            g[i] += dg;
-            if (g[i] >= G) g[i] -= G, ++tok[i];
+            const int row = i * RPI + threadIdx.x / L::CPR, c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC;
+            const int tok = (r0 + row) / a.G;
+            on[i] = c < a.D && row < BR;
+            g[i] = r0 + row - tok * a.G;
+            q[i] = q0 + tok * a.q_st + g[i] * a.q_sh + c;
+            go[i] = go0 + tok * a.go_st + g[i] * a.go_sh + c;
         }
     }
-    __device__ __forceinline__ void load(const T* base, long long st, long long sh, char* lds) const {
-        if (on) {
+    __device__ __forceinline__ void advance(const Attn& a) {
+        const int adv_t = BR / a.G, adv_g = BR - adv_t * a.G;
 #pragma unroll
-            for (int i = 0; i < N; ++i) load_to_lds(base + tok[i] * st + g[i] * sh + c, lds + i * 4096 + (threadIdx.x >> 6) * 1024);
+        for (int i = 0; i < N; ++i) {
+            g[i] += adv_g;
+            const bool over = g[i] >= a.G;
+            q[i] += adv_t * a.q_st + adv_g * a.q_sh + (over ? a.q_st - a.G * a.q_sh : 0);
+            go[i] += adv_t * a.go_st + adv_g * a.go_sh + (over ? a.go_st - a.G * a.go_sh : 0);
+            g[i] -= over ? a.G : 0;
         }
+    }
+    __device__ __forceinline__ void load(unsigned lq, unsigned lg) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (on[i]) {
+                load_to_lds(q[i], lq + i * 4096);
+                load_to_lds(go[i], lg + i * 4096);
+            }
     }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool EVEN>
 __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     typedef GkvCfg<T, DP> C;
     constexpr int KS = DP / 16, DT = DP / 32, BK = 128, BR = C::BR, TB = BR * L::ROWB;
     constexpr bool F32 = sizeof(T) == 4;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB + (C::V_LDS ? BK * L::ROWB : 0)];
-    __shared__ __attribute__((aligned(16))) float stat[2][3][BR];      // exponent base (16 bits: with the sum's logarithm), D, 1 / sum
+    __shared__ __attribute__((aligned(1024))) float stat[2][F32 ? 3 : 2][BR];
     char* lvt = lds + 4 * TB;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T *gk = (T*)a.gk, *gv = (T*)a.gv;
     if (blockIdx.x >= first_rest) {
         const Rest z = rest(a.cu_k, a.B, a.Tk);
@@ -854,34 +918,17 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
     if ((long long)tile * BK >= sk.n) return;
     const int R = sq.n * a.G;
-    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G},
-        srows{sq.begin, a.Hq, 1, a.G, kv * a.G};
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G};
     const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
     const T *q0 = (const T*)a.q + sq.begin * a.q_st + (long long)kv * a.G * a.q_sh, *g0 = (const T*)a.go + sq.begin * a.go_st + (long long)kv * a.G * a.go_sh;
     const float c2 = a.scale * LOG2E;
-    const int adv_t = BR / a.G, adv_g = BR - adv_t * a.G;
+    const long long all = a.Tq * a.Hq;
+    const unsigned at_lds = lds_at(lds) + wave * 1024, at_stat = lds_at(stat) + wave * BR * 4;      // (wave i brings the i-th statistic)
+    const float* rowstat = a.rowstat + ((long long)kv * a.Tq + sq.begin) * a.G;
     if (a.D < DP) {
         for (int i = threadIdx.x; i < 4 * TB / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
-    // this thread's row of statistics of the step at r0
-    const auto load_stat = [&](int r0, float* to) {
-        to[0] = to[1] = to[2] = 0.f;
-        if ((int)threadIdx.x < BR && r0 + (int)threadIdx.x < R) {
-            const long long at = srows.at(r0 + threadIdx.x);
-            const float2 s = a.stats[at];
-            to[0] = F32 ? s.x : s.x - __builtin_amdgcn_logf(s.y);
-            to[1] = a.delta[at];
-            to[2] = s.y;
-        }
-    };
-    const auto put_stat = [&](const float* from, int buf) {
-        if ((int)threadIdx.x < BR) {
-            stat[buf][0][threadIdx.x] = from[0];
-            stat[buf][1][threadIdx.x] = from[1];
-            if (F32) stat[buf][2][threadIdx.x] = from[2];
-        }
-    };
     for (long long kk = (long long)tile * BK; kk < sk.n; kk += (long long)tiles * BK) {
         const int k0 = (int)kk;
         const int key = k0 + wave * 32 + (lane & 31);
@@ -916,44 +963,49 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
                     s = mma(L::row_frag(lq, sub * 32 + (lane & 31), i, h), kf[i], s);
                     if constexpr (C::V_LDS) dp = mma(L::row_frag(lg, sub * 32 + (lane & 31), i, h), L::row_frag(lvt, wave * 32 + (lane & 31), i, h), dp);
                     else dp = mma(L::row_frag(lg, sub * 32 + (lane & 31), i, h), vf[i], dp);
+                    // (left alone, the compiler reads every operand ahead and spills; a reload in this loop waits for the tiles' loads)
+                    if (C::V_LDS && i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
                 }
-                float p[16], ds[16];
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const int r4 = sub * 32 + 8 * q4 + 4 * h;
-                    const float4 ba = *reinterpret_cast<const float4*>(&st[0][r4]), de = *reinterpret_cast<const float4*>(&st[1][r4]);
-                    float4 in = make_float4(1.f, 1.f, 1.f, 1.f);
-                    if (F32) in = *reinterpret_cast<const float4*>(&st[2][r4]);
-                    const float bb[4] = {ba.x, ba.y, ba.z, ba.w}, dd[4] = {de.x, de.y, de.z, de.w}, ii[4] = {in.x, in.y, in.z, in.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int i = 4 * q4 + j;
-                        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -bb[j]));
-                        if (F32) p[i] *= ii[j];
-                        ds[i] = p[i] * (dp[i] - dd[j]);
-                        if (MASK && !(r0 + r4 + j >= r_key && r0 + r4 + j < R)) p[i] = ds[i] = 0.f;
-                    }
-                }
+                Frag<T> pf[2], df[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    Frag<T> pf, df;
-                    frag_of(pf, p + 8 * t);
-                    frag_of(df, ds + 8 * t);
+                    float ba[8], de[8], in[8], p[8], ds[8];
+#pragma unroll
+                    for (int q4 = 0; q4 < 2; ++q4) {
+                        const int r4 = sub * 32 + 16 * t + 8 * q4 + 4 * h;
+                        *reinterpret_cast<float4*>(ba + 4 * q4) = *reinterpret_cast<const float4*>(&st[0][r4]);
+                        *reinterpret_cast<float4*>(de + 4 * q4) = *reinterpret_cast<const float4*>(&st[1][r4]);
+                        if (F32) *reinterpret_cast<float4*>(in + 4 * q4) = *reinterpret_cast<const float4*>(&st[F32 ? 2 : 0][r4]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = 8 * t + e, r = r0 + sub * 32 + reg_row(i, h);
+                        p[e] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -ba[e]));
+                        if (F32) p[e] *= in[e];
+                        ds[e] = p[e] * (dp[i] - de[e]);
+                        if (MASK && !(r >= r_key && r < R)) p[e] = ds[e] = 0.f;
+                    }
+                    frag_of(pf[t], p);
+                    frag_of(df[t], ds);
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        av[d] = mma(L::col_frag(lg, sub * 32 + 16 * t, d, lane), pf, av[d]);
-                        ak[d] = mma(L::col_frag(lq, sub * 32 + 16 * t, d, lane), df, ak[d]);
+                        av[d] = mma(L::col_frag(lg, sub * 32 + 16 * t, d, lane), pf[t], av[d]);
+                        ak[d] = mma(L::col_frag(lq, sub * 32 + 16 * t, d, lane), df[t], ak[d]);
                     }
-                }
             }
         };
         const auto border = [&](int r0) {
-            float mine[3];
-            load_stat(r0, mine);
             __syncthreads();
+            if ((int)threadIdx.x < BR) {
+                const bool on = r0 + (int)threadIdx.x < R;
+#pragma unroll
+                for (int i = 0; i < (F32 ? 3 : 2); ++i) stat[0][i][threadIdx.x] = on ? rowstat[i * all + r0 + threadIdx.x] : 0.f;
+            }
             bool bad = stage<T, DP, BR, true>(lds, (const T*)a.q, R - r0, a.D, [&](int r) { return qrows.at(r0 + r); });
             bad |= stage<T, DP, BR, true>(lds + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
-            put_stat(mine, 0);
             bad = __syncthreads_or(bad);
             step(std::true_type{}, lds, lds + TB, stat[0], r0);
             if (bad)
@@ -964,26 +1016,23 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
         for (; r0 < R && r0 < r_all; r0 += BR) border(r0);
         const int nfull = r0 < R ? (R - r0) / BR : 0;
         if (nfull > 0) {
-            RowDma<T, DP, BR> dma(r0, a.G, a.D);
-            float mine[3];
-            load_stat(r0, mine);
+            RowDma<T, DP, BR, EVEN> dma(q0, g0, a, r0);
+            const float* sp = rowstat + wave * all;
+            const bool son = wave < (F32 ? 3 : 2) && lane < BR;
             __syncthreads();
-            dma.load(q0, a.q_st, a.q_sh, lds);
-            dma.load(g0, a.go_st, a.go_sh, lds + TB);
-            put_stat(mine, 0);
+            dma.load(at_lds, at_lds + TB);
+            if (son) word_to_lds(sp + r0, lane * 4, at_stat);
             for (int t = 0; t < nfull; ++t, r0 += BR) {
                 char* now = lds + (t & 1) * 2 * TB;
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                wait_loads<0>();
                 __syncthreads();
                 if (t + 1 < nfull) {
-                    char* next = lds + ((t + 1) & 1) * 2 * TB;
-                    load_stat(r0 + BR, mine);
-                    dma.advance(a.G, adv_t, adv_g);
-                    dma.load(q0, a.q_st, a.q_sh, next);
-                    dma.load(g0, a.go_st, a.go_sh, next + TB);
+                    const unsigned next = at_lds + ((t + 1) & 1) * 2 * TB;
+                    dma.advance(a);
+                    dma.load(next, next + TB);
+                    if (son) word_to_lds(sp + r0 + BR, lane * 4, at_stat + ((t + 1) & 1) * (unsigned)sizeof(stat[0]));
                 }
                 step(std::false_type{}, now, now + TB, stat[t & 1], r0);
-                if (t + 1 < nfull) put_stat(mine, (t + 1) & 1);
             }
         }
         if (r0 < R) border(r0);
@@ -1017,6 +1066,8 @@ int check_tensor(const char* name, const void* p, int64_t st, int64_t sh, int dt
     if (!p) return sam3_seq_fail(EINVAL_, "attention: %s is a null pointer", name);
     if (misaligned(p) || bad_pitch(st, dtype) || bad_pitch(sh, dtype))
         return sam3_seq_fail(EINVAL_, "attention: %s: pointer and strides must keep 16-byte accesses aligned", name);
+    // (offsets inside a tile of 64 rows are 32 bits)
+    if (st < 0 || sh < 0 || st >= (1 << 22) || sh >= (1 << 22)) return sam3_seq_fail(ENOTSUP_, "attention: %s: strides must be below 2^22 elements", name);
     return 0;
 }
 
@@ -1128,7 +1179,7 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     return launched("sam3_seq_attn_fwd");
 }
 
-size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq) { return Tq > 0 && Hq > 0 ? (size_t)Tq * Hq * sizeof(float) : 0; }
+size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq) { return Tq > 0 && Hq > 0 ? (size_t)Tq * Hq * 3 * sizeof(float) : 0; }
 
 int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                       int64_t v_st, int64_t v_sh, const void* go, int64_t go_st, int64_t go_sh, const void* out, const float* stats,
@@ -1151,7 +1202,7 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     }
     if (!cu_q || !cu_k) return sam3_seq_fail(EINVAL_, "attention: null pointer");
     Attn a{};
-    a.q = q; a.k = k; a.v = v; a.go = go; a.o = out; a.stats = (float2*)stats; a.delta = (float*)workspace;
+    a.q = q; a.k = k; a.v = v; a.go = go; a.o = out; a.stats = (float2*)stats; a.rowstat = (float*)workspace;
     a.gq = gq; a.gk = gk; a.gv = gv; a.cu_q = cu_q; a.cu_k = cu_k;
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh; a.go_st = go_st; a.go_sh = go_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
@@ -1163,7 +1214,18 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
         BY_HEAD(k_attn_gq, dim3((unsigned)q_rest + REST), (hipStream_t)stream, a, qt, (unsigned)q_rest);
         if (int rc = launched("sam3_seq_attn_bwd")) return rc;
     }
-    if (Tk > 0) BY_HEAD(k_attn_gkv, dim3((unsigned)k_rest + REST), (hipStream_t)stream, a, kt, (unsigned)k_rest);
+    if (Tk > 0) {
+        const dim3 grid((unsigned)k_rest + REST);
+        hipStream_t st = (hipStream_t)stream;
+#define GKV(TY, W)                                                                                                                        \
+    do {                                                                                                                                  \
+        if (GkvCfg<TY, W>::BR % a.G == 0) hipLaunchKernelGGL((k_attn_gkv<TY, W, true>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest); \
+        else hipLaunchKernelGGL((k_attn_gkv<TY, W, false>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest);                             \
+    } while (0)
+        if (dtype == 0) { if (D <= 32) GKV(bf16_t, 32); else if (D <= 64) GKV(bf16_t, 64); else GKV(bf16_t, 128); }
+        else { if (D <= 32) GKV(float, 32); else if (D <= 64) GKV(float, 64); else GKV(float, 128); }
+#undef GKV
+    }
     return launched("sam3_seq_attn_bwd");
 }
 

@@ -50,7 +50,7 @@ def test_header_exports_and_error_text():
     lib = _ffi.load()
     assert lib.sam3_seq_rms_norm_bwd_workspace_bytes(0, 64) == 0 == lib.sam3_seq_rms_norm_bwd_workspace_bytes(8, 63)
     assert lib.sam3_seq_rms_norm_bwd_workspace_bytes(3, 1024) == 1024 * 4
-    assert lib.sam3_seq_attn_bwd_workspace_bytes(5, 4) == 80
+    assert lib.sam3_seq_attn_bwd_workspace_bytes(5, 4) == 240
     p = ctypes.c_void_p(64)
 
     def norm(M=1, C=64, dtype=0, x=p, w=p, y=p, q8=None, scales=None, group=0, fmt=0, eps=1e-6, ldx=64):
