@@ -842,13 +842,13 @@ struct GkvCfg {
     static constexpr int WAVES = sizeof(T) * DP > 256 ? 1 : 2;         // per SIMD
 };
 
-// The rows of a step (BR of them) of q and go into LDS.  EVEN: the heads of a group divide a step, so a lane's rows stay where they are
+// The rows of a step (BR of them, STEP to the next) of q and go into LDS by NT threads.  EVEN: the heads of a group divide a step, so a lane's rows stay where they are
 // from step to step and only the wave's address moves.  Otherwise each lane follows its rows: a step is adv_t tokens and adv_g heads, one
 // token more where the head leaves the group.
-template <typename T, int DP, int BR, bool EVEN>
+template <typename T, int DP, int BR, bool EVEN, int NT = 256, int STEP = BR>
 struct RowDma {
     typedef Tile<T, DP> L;
-    static constexpr int RPI = 256 / L::CPR, N = (BR + RPI - 1) / RPI;
+    static constexpr int RPI = NT / L::CPR, N = (BR + RPI - 1) / RPI;
     static_assert(BR % RPI == 0 || N == 1, "whole rounds");
     const T *q, *go;
     unsigned oq[N], og[N];
@@ -856,15 +856,15 @@ struct RowDma {
     __device__ __forceinline__ RowDma(const T* q0, const T* go0, const Attn& a, int r0) : q(q0 + r0 / a.G * a.q_st), go(go0 + r0 / a.G * a.go_st) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = i * RPI + threadIdx.x / L::CPR, c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC, t = row / a.G, g = row - t * a.G;
+            const int row = i * RPI + (int)threadIdx.x % NT / L::CPR, c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC, t = row / a.G, g = row - t * a.G;
             on[i] = c < a.D && row < BR;
             oq[i] = (unsigned)((t * a.q_st + g * a.q_sh + c) * (long long)sizeof(T));
             og[i] = (unsigned)((t * a.go_st + g * a.go_sh + c) * (long long)sizeof(T));
         }
     }
     __device__ __forceinline__ void advance(const Attn& a) {
-        q += BR / a.G * a.q_st;
-        go += BR / a.G * a.go_st;
+        q += STEP / a.G * a.q_st;
+        go += STEP / a.G * a.go_st;
 #pragma unroll
         for (int i = 0; i < N; ++i) asm volatile("" : "+v"(oq[i]), "+v"(og[i]));        // (registers, not scratch: a reload waits for the loads)
     }
@@ -872,22 +872,22 @@ struct RowDma {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (on[i]) {
-                load_to_lds(q, oq[i], lq + i * 4096);
-                load_to_lds(go, og[i], lg + i * 4096);
+                load_to_lds(q, oq[i], lq + i * NT * 16);
+                load_to_lds(go, og[i], lg + i * NT * 16);
             }
     }
 };
-template <typename T, int DP, int BR>
-struct RowDma<T, DP, BR, false> {
+template <typename T, int DP, int BR, int NT, int STEP>
+struct RowDma<T, DP, BR, false, NT, STEP> {
     typedef Tile<T, DP> L;
-    static constexpr int RPI = 256 / L::CPR, N = (BR + RPI - 1) / RPI;
+    static constexpr int RPI = NT / L::CPR, N = (BR + RPI - 1) / RPI;
     const T *q[N], *go[N];
     int g[N];
     bool on[N];
     __device__ __forceinline__ RowDma(const T* q0, const T* go0, const Attn& a, int r0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = i * RPI + threadIdx.x / L::CPR, c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC;
+            const int row = i * RPI + (int)threadIdx.x % NT / L::CPR, c = ((threadIdx.x % L::CPR) ^ L::f(row)) * L::EPC;
             const int tok = (r0 + row) / a.G;
             on[i] = c < a.D && row < BR;
             g[i] = r0 + row - tok * a.G;
@@ -896,7 +896,7 @@ struct RowDma<T, DP, BR, false> {
         }
     }
     __device__ __forceinline__ void advance(const Attn& a) {
-        const int adv_t = BR / a.G, adv_g = BR - adv_t * a.G;
+        const int adv_t = STEP / a.G, adv_g = STEP - adv_t * a.G;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             g[i] += adv_g;
@@ -910,8 +910,74 @@ struct RowDma<T, DP, BR, false> {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (on[i]) {
-                load_to_lds(q[i], lq + i * 4096);
-                load_to_lds(go[i], lg + i * 4096);
+                load_to_lds(q[i], lq + i * NT * 16);
+                load_to_lds(go[i], lg + i * NT * 16);
+            }
+    }
+};
+
+// One step of 32 rows for 32 keys: what both kernels for gk and gv compute.  lq, lg: the rows' tiles; lvw: the wave's value rows where they
+// are in LDS; st: exponent base, D and (32 bits) 1 / sum of the rows, `pitch` apart.  Rows r0 .. are seen from row `from` to `end`.
+template <typename T, int DP, bool V_LDS>
+struct GkvState {
+    typedef Tile<T, DP> L;
+    static constexpr int KS = DP / 16, DT = DP / 32;
+    static constexpr bool F32 = sizeof(T) == 4;
+    Frag<T> kf[KS], vf[V_LDS ? 1 : KS];
+    f32x16 ak[DT], av[DT];
+    bool spoilt;        // a row that is not finite sees the key: so are its gradients
+
+    __device__ __forceinline__ void begin(const T* k, const T* v, bool live, int D, int h) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + h * 8;
+            kf[s] = frag_global(k + d, live && d < D);
+            if (!V_LDS) vf[s] = frag_global(v + d, live && d < D);
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) ak[i] = zero16(), av[i] = zero16();
+        spoilt = false;
+    }
+    template <bool MASK>
+    __device__ __forceinline__ void step(const char* lq, const char* lg, const char* lvw, const float* st, int pitch, int lane, float c2, int r0, int from, int end) {
+        const int h = lane >> 5;
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            s = mma(L::row_frag(lq, lane & 31, i, h), kf[i], s);
+            if constexpr (V_LDS) dp = mma(L::row_frag(lg, lane & 31, i, h), L::row_frag(lvw, lane & 31, i, h), dp);
+            else dp = mma(L::row_frag(lg, lane & 31, i, h), vf[i], dp);
+            // (left alone, the compiler reads every operand ahead and spills; a reload in the loop waits for the tiles' loads)
+            if (V_LDS && i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        Frag<T> pf[2], df[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float ba[8], de[8], in[8], p[8], ds[8];
+#pragma unroll
+            for (int q4 = 0; q4 < 2; ++q4) {
+                const int r4 = 16 * t + 8 * q4 + 4 * h;
+                *reinterpret_cast<float4*>(ba + 4 * q4) = *reinterpret_cast<const float4*>(st + r4);
+                *reinterpret_cast<float4*>(de + 4 * q4) = *reinterpret_cast<const float4*>(st + pitch + r4);
+                if (F32) *reinterpret_cast<float4*>(in + 4 * q4) = *reinterpret_cast<const float4*>(st + 2 * pitch + r4);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = 8 * t + e, r = r0 + reg_row(i, h);
+                p[e] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -ba[e]));
+                if (F32) p[e] *= in[e];
+                ds[e] = p[e] * (dp[i] - de[e]);
+                if (MASK && !(r >= from && r < end)) p[e] = ds[e] = 0.f;
+            }
+            frag_of(pf[t], p);
+            frag_of(df[t], ds);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                av[d] = mma(L::col_frag(lg, 16 * t, d, lane), pf[t], av[d]);
+                ak[d] = mma(L::col_frag(lq, 16 * t, d, lane), df[t], ak[d]);
             }
     }
 };
@@ -920,7 +986,7 @@ template <typename T, int DP, bool EVEN>
 __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     typedef GkvCfg<T, DP> C;
-    constexpr int KS = DP / 16, DT = DP / 32, BK = 128, BR = C::BR, TB = BR * L::ROWB;
+    constexpr int DT = DP / 32, BK = 128, BR = C::BR, TB = BR * L::ROWB;
     constexpr bool F32 = sizeof(T) == 4;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB + (C::V_LDS ? BK * L::ROWB : 0)];
     __shared__ __attribute__((aligned(1024))) float stat[2][F32 ? 3 : 2][BR];
@@ -958,69 +1024,22 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
         const int k0 = (int)kk;
         const int key = k0 + wave * 32 + (lane & 31);
         const bool live = key < sk.n;
-        Frag<T> kf[KS], vf[C::V_LDS ? 1 : KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = s * 16 + h * 8;
-            kf[s] = frag_global(k + (live ? key * a.k_st : 0) + d, live && d < a.D);
-            if (!C::V_LDS) vf[s] = frag_global(v + (live ? key * a.v_st : 0) + d, live && d < a.D);
-        }
+        GkvState<T, DP, C::V_LDS> st;
+        st.begin(k + (live ? key * a.k_st : 0), v + (live ? key * a.v_st : 0), live, a.D, h);
         __syncthreads();
         if (C::V_LDS) stage<T, DP, BK, false>(lvt, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
-        f32x16 ak[DT], av[DT];
-#pragma unroll
-        for (int i = 0; i < DT; ++i) ak[i] = zero16(), av[i] = zero16();
         // rows before first see no key of the tile; from r_all on they see all of them; from r_key on, this lane's
         const auto first_row = [&](int j) {
             const long long t = a.causal ? (long long)j - (sk.n - sq.n) : 0;
             return (t < 0 ? 0 : t > sq.n ? sq.n : (int)t) * a.G;
         };
         const int first = first_row(k0), r_all = first_row(min(k0 + BK, sk.n) - 1), r_key = live ? first_row(key) : R;
-        bool spoilt = false;                    // a row that is not finite sees the key: so are its gradients
 
-        const auto step = [&](auto mask, const char* lq, const char* lg, const float (*st)[BR], int r0) {
-            constexpr bool MASK = decltype(mask)::value;
+        const auto step = [&](auto mask, int buf, int r0) {
 #pragma unroll
-            for (int sub = 0; sub < BR / 32; ++sub) {
-                f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    s = mma(L::row_frag(lq, sub * 32 + (lane & 31), i, h), kf[i], s);
-                    if constexpr (C::V_LDS) dp = mma(L::row_frag(lg, sub * 32 + (lane & 31), i, h), L::row_frag(lvt, wave * 32 + (lane & 31), i, h), dp);
-                    else dp = mma(L::row_frag(lg, sub * 32 + (lane & 31), i, h), vf[i], dp);
-                    // (left alone, the compiler reads every operand ahead and spills; a reload in this loop waits for the tiles' loads)
-                    if (C::V_LDS && i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-                }
-                Frag<T> pf[2], df[2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    float ba[8], de[8], in[8], p[8], ds[8];
-#pragma unroll
-                    for (int q4 = 0; q4 < 2; ++q4) {
-                        const int r4 = sub * 32 + 16 * t + 8 * q4 + 4 * h;
-                        *reinterpret_cast<float4*>(ba + 4 * q4) = *reinterpret_cast<const float4*>(&st[0][r4]);
-                        *reinterpret_cast<float4*>(de + 4 * q4) = *reinterpret_cast<const float4*>(&st[1][r4]);
-                        if (F32) *reinterpret_cast<float4*>(in + 4 * q4) = *reinterpret_cast<const float4*>(&st[F32 ? 2 : 0][r4]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int i = 8 * t + e, r = r0 + sub * 32 + reg_row(i, h);
-                        p[e] = __builtin_amdgcn_exp2f(fmaf(s[i], c2, -ba[e]));
-                        if (F32) p[e] *= in[e];
-                        ds[e] = p[e] * (dp[i] - de[e]);
-                        if (MASK && !(r >= r_key && r < R)) p[e] = ds[e] = 0.f;
-                    }
-                    frag_of(pf[t], p);
-                    frag_of(df[t], ds);
-                }
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        av[d] = mma(L::col_frag(lg, sub * 32 + 16 * t, d, lane), pf[t], av[d]);
-                        ak[d] = mma(L::col_frag(lq, sub * 32 + 16 * t, d, lane), df[t], ak[d]);
-                    }
-            }
+            for (int sub = 0; sub < BR / 32; ++sub)
+                st.template step<decltype(mask)::value>(lds + buf * 2 * TB + sub * 32 * L::ROWB, lds + buf * 2 * TB + TB + sub * 32 * L::ROWB, lvt + wave * 32 * L::ROWB,
+                                                        &stat[buf][0][sub * 32], BR, lane, c2, r0 + sub * 32, r_key, R);
         };
         const auto border = [&](int r0) {
             __syncthreads();
@@ -1032,10 +1051,10 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             bool bad = stage<T, DP, BR, true>(lds, (const T*)a.q, R - r0, a.D, [&](int r) { return qrows.at(r0 + r); });
             bad |= stage<T, DP, BR, true>(lds + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
             bad = __syncthreads_or(bad);
-            step(std::true_type{}, lds, lds + TB, stat[0], r0);
+            step(std::true_type{}, 0, r0);
             if (bad)
                 for (int r = max(r0, r_key); r < min(r0 + BR, R); ++r)
-                    spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
+                    st.spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
         };
         int r0 = first;
         for (; r0 < R && r0 < r_all; r0 += BR) border(r0);
@@ -1048,7 +1067,6 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             dma.load(at_lds, at_lds + TB);
             if (son) word_to_lds(sp + r0, lane * 4, at_stat);
             for (int t = 0; t < nfull; ++t, r0 += BR) {
-                char* now = lds + (t & 1) * 2 * TB;
                 wait_loads<0>();
                 __syncthreads();
                 if (t + 1 < nfull) {
@@ -1057,7 +1075,7 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
                     dma.load(next, next + TB);
                     if (son) word_to_lds(sp + r0 + BR, lane * 4, at_stat + ((t + 1) & 1) * (unsigned)sizeof(stat[0]));
                 }
-                step(std::false_type{}, now, now + TB, stat[t & 1], r0);
+                step(std::false_type{}, t & 1, r0);
             }
         }
         if (r0 < R) border(r0);
@@ -1065,10 +1083,290 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             T *ok = gk + ((sk.begin + key) * a.Hk + kv) * a.D, *ov = gv + ((sk.begin + key) * a.Hk + kv) * a.D;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                store_cols(ok, ak[d], d, h, a.D, spoilt ? NAN : a.scale);
-                store_cols(ov, av[d], d, h, a.D, spoilt ? NAN : 1.f);
+                store_cols(ok, st.ak[d], d, h, a.D, st.spoilt ? NAN : a.scale);
+                store_cols(ov, st.av[d], d, h, a.D, st.spoilt ? NAN : 1.f);
             }
         }
+    }
+}
+
+// -------------------------------------------------------------- the backward where its tiles of 128 would leave the chip idle
+// Tiles of 32 rows (gq) or keys (gk, gv); a workgroup's NW waves take the blocks of 32 of the other side in turn, with tiles of their own
+// and no barrier, and their results meet in LDS in a fixed order.  NW = 1 where there is not more than one block or two.
+template <typename T, int DP, int NW>
+struct SplitCfg {
+    static constexpr int TB = 32 * DP * (int)sizeof(T), LDS = NW * 4 * TB;
+    static constexpr int WAVES = LDS / NW >= 32768 || LDS > 65536 ? 1 : 2;      // per SIMD
+};
+
+// NW results of 32 rows x DP (lane: row) summed over the waves: each thread gets four neighbouring columns of a row
+template <typename T, int DP, int NW, typename F>
+__device__ __forceinline__ void over_waves(float* pool, const f32x16* acc, int lane, int wave, int D, F out) {
+    const int h = lane >> 5;
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(pool + (wave * 32 + (lane & 31)) * DP + ((d * 32 + 8 * g + 4 * h) ^ ((lane & 7) << 2))) =
+                make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (DP / 4); i += NW * 64) {
+        const int r = i / (DP / 4), d = (i % (DP / 4)) * 4;
+        if (d >= D) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(pool + (w * 32 + r) * DP + (d ^ ((r & 7) << 2)));
+            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        }
+        out(r, d, o);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float4& o, float mul) {
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(p) = make_uint2(pack2(o.x * mul, o.y * mul), pack2(o.z * mul, o.w * mul));
+    else *reinterpret_cast<float4*>(p) = make_float4(o.x * mul, o.y * mul, o.z * mul, o.w * mul);
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_attn_gq_split(Attn a, int tiles, unsigned first_rest) {
+    constexpr int KS = DP / 16, DT = DP / 32, TB = SplitCfg<T, DP, NW>::TB;
+    __shared__ __attribute__((aligned(1024))) char lds[SplitCfg<T, DP, NW>::LDS];
+    __shared__ float part[NW][32], mul[32];
+    __shared__ int bad_row[32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    T* gq = (T*)a.gq;
+    if (blockIdx.x >= first_rest) {
+        const Rest z = rest(a.cu_q, a.B, a.Tq);
+        for (long long i = (long long)(blockIdx.x - first_rest) * (NW * 8) + (threadIdx.x >> 3); i < z.n * a.Hq; i += (long long)(gridDim.x - first_rest) * (NW * 8))
+            zero_row(gq + (z.row(i / a.Hq) * a.Hq + i % a.Hq) * a.D, a.D, threadIdx.x & 7, 8);
+        return;
+    }
+    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    if (pl.tile < 0) return;
+    const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
+    const int R = sq.n * a.G;
+    if ((long long)pl.tile * 32 >= R) return;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G};
+    const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const float c2 = a.scale * LOG2E;
+    char* mine = lds + wave * 4 * TB;
+    const unsigned at_lds = lds_at(mine);
+    const Dma<T, DP, 32, 64> dk(a.k_st, a.D), dv(a.v_st, a.D);
+    for (long long rr = (long long)pl.tile * 32; rr < R; rr += (long long)tiles * 32) {
+        const int r0 = (int)rr, row = r0 + (lane & 31);
+        const bool live = row < R;
+        const int tok = live ? row / a.G : 0;
+        const long long at = live ? (sq.begin + tok) * a.Hq + kv * a.G + (row - tok * a.G) : 0;
+        const int jmax = live ? seen_keys(tok, sq.n, sk.n, a.causal) : 0;
+        const int jend = seen_keys((min(r0 + 32, R) - 1) / a.G, sq.n, sk.n, a.causal), jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);
+        __syncthreads();
+        if (a.D < DP)
+            for (int i = lane; i < 4 * TB / 16; i += 64) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+        if (threadIdx.x < 32) bad_row[threadIdx.x] = 0;
+        __syncthreads();
+        GqState<T, DP, 32> st;
+        const float2 stat = live ? a.stats[at] : make_float2(0.f, 0.f);
+        st.base = stat.x;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + h * 8;
+            const bool on = live && d < a.D;
+            st.qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + d, on);
+            st.gf[s] = frag_global((const T*)a.go + (live ? grows.at(row) : 0) + d, on);
+        }
+        // a block with a mask, through registers; false: nothing in it that is not finite
+        const auto bring = [&](int k0) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const bool bad = stage<T, DP, 32, true, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+            stage<T, DP, 32, false, 64>(mine + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            return __any(bad);
+        };
+        float delta = 0.f;
+        if (jend <= EXACT_D) {
+            st.delta = st.sum = 0.f;
+            for (int k0 = wave * 32; k0 < jend; k0 += NW * 32) {
+                bring(k0);
+                st.template step<true, true>(mine, mine + TB, lane, c2, jmax - k0);
+            }
+            delta = st.sum + __shfl_xor(st.sum, 32, 64);
+            if (h == 0) part[wave][lane & 31] = delta;
+            __syncthreads();
+            delta = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) delta += part[w][lane & 31];
+            delta *= stat.y;
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = s * 16 + h * 8;
+                if (live && d < a.D) {
+                    Raw8<T> x, y;
+                    float fx[8], fy[8];
+                    x.load((const T*)a.o + at * a.D + d);
+                    y.load((const T*)a.go + grows.at(row) + d);
+                    x.get(fx);
+                    y.get(fy);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) delta += fx[j] * fy[j];
+                }
+            }
+            delta += __shfl_xor(delta, 32, 64);
+        }
+        st.delta = delta;
+        if (wave == 0 && live && h == 0) {
+            const long long all = a.Tq * a.Hq;
+            float* to = a.rowstat + ((long long)kv * a.Tq + sq.begin) * a.G + row;
+            to[0] = sizeof(T) == 4 ? stat.x : stat.x - __builtin_amdgcn_logf(stat.y);
+            to[all] = delta;
+            if (sizeof(T) == 4) to[2 * all] = stat.y;
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
+        const int full = jall / 32;
+        bool spoilt = false;
+        int blk = wave, buf = 0;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (blk < full) {
+            dk.load(k + (long long)blk * 32 * a.k_st, a.k_st, at_lds);
+            dv.load(v + (long long)blk * 32 * a.v_st, a.v_st, at_lds + TB);
+            wait_loads<0>();
+        }
+        for (; blk < full; blk += NW, buf ^= 1) {
+            char* now = mine + buf * 2 * TB;
+            const unsigned next = at_lds + (buf ^ 1) * 2 * TB;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (blk + NW < full) {
+                dk.load(k + (long long)(blk + NW) * 32 * a.k_st, a.k_st, next);
+                dv.load(v + (long long)(blk + NW) * 32 * a.v_st, a.v_st, next + TB);
+                wait_loads<2 * Dma<T, DP, 32, 64>::N>();
+            } else {
+                wait_loads<0>();
+            }
+            st.template step<false>(now, now + TB, lane, c2, 32);
+        }
+        for (; blk * 32 < jend; blk += NW) {
+            const bool bad = bring(blk * 32);
+            st.template step<true>(mine, mine + TB, lane, c2, jmax - blk * 32);
+            if (bad)
+                for (int j = 0; j < min(jmax - blk * 32, 32); ++j) spoilt |= spoils(k + (blk * 32 + j) * a.k_st, a.D);
+        }
+        if (spoilt) bad_row[lane & 31] = 1;
+        if (wave == 0 && h == 0) mul[lane & 31] = a.scale * stat.y;
+        over_waves<T, DP, NW>(reinterpret_cast<float*>(lds), st.acc, lane, wave, a.D, [&](int r, int d, const float4& o) {
+            if (r0 + r >= R) return;
+            const int t = (r0 + r) / a.G;
+            store4(gq + ((sq.begin + t) * a.Hq + kv * a.G + (r0 + r - t * a.G)) * a.D + d, o, bad_row[r] ? NAN : mul[r]);
+        });
+    }
+}
+
+template <typename T, int DP, int NW, bool EVEN>
+__global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_attn_gkv_split(Attn a, int tiles, unsigned first_rest) {
+    constexpr int TB = SplitCfg<T, DP, NW>::TB;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int NS = F32 ? 3 : 2;
+    __shared__ __attribute__((aligned(1024))) char lds[SplitCfg<T, DP, NW>::LDS];
+    __shared__ __attribute__((aligned(1024))) float stat[NW][2][NS][32];
+    __shared__ int bad_key[32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    T *gk = (T*)a.gk, *gv = (T*)a.gv;
+    if (blockIdx.x >= first_rest) {
+        const Rest z = rest(a.cu_k, a.B, a.Tk);
+        for (long long i = (long long)(blockIdx.x - first_rest) * (NW * 8) + (threadIdx.x >> 3); i < z.n * a.Hk; i += (long long)(gridDim.x - first_rest) * (NW * 8)) {
+            const long long r = z.row(i / a.Hk) * a.Hk + i % a.Hk;
+            zero_row(gk + r * a.D, a.D, threadIdx.x & 7, 8);
+            zero_row(gv + r * a.D, a.D, threadIdx.x & 7, 8);
+        }
+        return;
+    }
+    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    if (pl.tile < 0) return;
+    const int tile = tiles - 1 - pl.tile;
+    const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
+    const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
+    if ((long long)tile * 32 >= sk.n) return;
+    const int R = sq.n * a.G;
+    const Rows qrows{sq.begin, a.q_st, a.q_sh, a.G, kv * a.G}, grows{sq.begin, a.go_st, a.go_sh, a.G, kv * a.G};
+    const T *k = (const T*)a.k + sk.begin * a.k_st + kv * a.k_sh, *v = (const T*)a.v + sk.begin * a.v_st + kv * a.v_sh;
+    const T *q0 = (const T*)a.q + sq.begin * a.q_st + (long long)kv * a.G * a.q_sh, *g0 = (const T*)a.go + sq.begin * a.go_st + (long long)kv * a.G * a.go_sh;
+    const float c2 = a.scale * LOG2E;
+    const long long all = a.Tq * a.Hq;
+    char* mine = lds + wave * 4 * TB;
+    const unsigned at_lds = lds_at(mine), at_stat = lds_at(&stat[wave][0][0][0]);
+    const float* rowstat = a.rowstat + ((long long)kv * a.Tq + sq.begin) * a.G;
+    for (long long kk = (long long)tile * 32; kk < sk.n; kk += (long long)tiles * 32) {
+        const int k0 = (int)kk, key = k0 + (lane & 31);
+        const bool live = key < sk.n;
+        __syncthreads();
+        if (a.D < DP)
+            for (int i = lane; i < 4 * TB / 16; i += 64) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+        if (threadIdx.x < 32) bad_key[threadIdx.x] = 0;
+        __syncthreads();
+        GkvState<T, DP, false> st;
+        st.begin(k + (live ? key * a.k_st : 0), v + (live ? key * a.v_st : 0), live, a.D, h);
+        const auto first_row = [&](int j) {
+            const long long t = a.causal ? (long long)j - (sk.n - sq.n) : 0;
+            return (t < 0 ? 0 : t > sq.n ? sq.n : (int)t) * a.G;
+        };
+        const int first = first_row(k0), r_all = first_row(min(k0 + 32, sk.n) - 1), r_key = live ? first_row(key) : R;
+        // steps of 32 rows from `first`: those below `lo` and the last one, if it is short, need a mask
+        const int steps = R > first ? (R - first + 31) / 32 : 0, lo = min((r_all - first + 31) / 32, steps), hi = max(lo, R > first ? (R - first) / 32 : 0);
+        const auto border = [&](int s) {
+            const int r0 = first + s * 32;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (lane < 32) {
+                const bool on = r0 + lane < R;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) stat[wave][0][i][lane] = on ? rowstat[i * all + r0 + lane] : 0.f;
+            }
+            bool bad = stage<T, DP, 32, true, 64>(mine, (const T*)a.q, R - r0, a.D, [&](int r) { return qrows.at(r0 + r); });
+            bad |= stage<T, DP, 32, true, 64>(mine + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            st.template step<true>(mine, mine + TB, nullptr, &stat[wave][0][0][0], 32, lane, c2, r0, r_key, R);
+            if (__any(bad))
+                for (int r = max(r0, r_key); r < min(r0 + 32, R); ++r)
+                    st.spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
+        };
+        int s = wave;
+        for (; s < lo; s += NW) border(s);
+        if (s < hi) {
+            RowDma<T, DP, 32, EVEN, 64, NW * 32> dma(q0, g0, a, first + s * 32);
+            const auto load = [&](unsigned to, unsigned st_to, int r0) {
+                dma.load(to, to + TB);
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    if (lane < 32) word_to_lds(rowstat + i * all + r0, lane * 4, st_to + i * 128);
+            };
+            constexpr int LOADS = 2 * RowDma<T, DP, 32, EVEN, 64, NW * 32>::N + NS;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load(at_lds, at_stat, first + s * 32);
+            wait_loads<0>();
+            for (int buf = 0; s < hi; s += NW, buf ^= 1) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (s + NW < hi) {
+                    dma.advance(a);
+                    load(at_lds + (buf ^ 1) * 2 * TB, at_stat + (buf ^ 1) * NS * 128, first + (s + NW) * 32);
+                    wait_loads<LOADS>();
+                } else {
+                    wait_loads<0>();
+                }
+                char* now = mine + buf * 2 * TB;
+                st.template step<false>(now, now + TB, nullptr, &stat[wave][buf][0][0], 32, lane, c2, first + s * 32, r_key, R);
+            }
+        }
+        for (; s < steps; s += NW) border(s);
+        if (st.spoilt) bad_key[lane & 31] = 1;
+        float* pool = reinterpret_cast<float*>(lds);
+        over_waves<T, DP, NW>(pool, st.ak, lane, wave, a.D, [&](int r, int d, const float4& o) {
+            if (k0 + r < sk.n) store4(gk + ((sk.begin + k0 + r) * a.Hk + kv) * a.D + d, o, bad_key[r] ? NAN : a.scale);
+        });
+        over_waves<T, DP, NW>(pool, st.av, lane, wave, a.D, [&](int r, int d, const float4& o) {
+            if (k0 + r < sk.n) store4(gv + ((sk.begin + k0 + r) * a.Hk + kv) * a.D + d, o, bad_key[r] ? NAN : 1.f);
+        });
     }
 }
 
@@ -1116,7 +1414,9 @@ unsigned tiles(int64_t rows, int per) {
     return (unsigned)(t < 1 ? 1 : t);
 }
 
-// The forward for few rows: where the tiles of 128 rows would leave most of the chip idle, and there are keys to split.
+// The forward for few rows: rows of one token's heads or so (32 prompts' worth of short rows run 21 us in tiles of 128 and 11 in tiles of
+// 32), or where the tiles of 128 rows would leave most of the chip idle and there are keys to split: at 32 tiles over 8192 keys 195 us in
+// tiles of 128, 85 split and joined; at 128 tiles over 4096 keys 110 and 161, so not there.
 struct Plan {
     bool few;
     int tiles, splits, chunk;
@@ -1124,7 +1424,7 @@ struct Plan {
 Plan plan(int64_t Tq, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
     const int64_t rows = (max_q < Tq ? max_q : Tq) * (Hq / Hk), pairs = (int64_t)B * Hk;
     Plan p{};
-    p.few = rows <= 32 || (max_k >= 256 && pairs * tiles(rows, BM) <= 96);
+    p.few = rows <= 32 || (max_k >= 256 && max_k >= 4 * max_q && pairs * tiles(rows, BM) <= 64);
     if (!p.few) return p;
     p.tiles = (int)tiles(rows, 32);
     // Chunks of 256 to 1024 keys as long as that gives 1024 waves, four for each CU; longer ones for a lot of keys, where 8192 of them
@@ -1232,20 +1532,41 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh; a.go_st = go_st; a.go_sh = go_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest_q = max_q < Tq ? max_q : Tq, longest_k = max_k < Tk ? max_k : Tk;
-    const int qt = (int)tiles(longest_q * a.G, BM), kt = (int)tiles(longest_k, 128);
+    // Tiles of 32, shared by the waves of a workgroup, where tiles of 128 would be too few for the chip.  Measured on both sides (us, tiles of
+    // 128 / of 32; bf16): gq at 48 tiles 63 / 25, at 128 143 / 119, at 256 51 / 77; gk and gv at 64 241 / 72, at 128 438 / 155, at 256 859 / 524.
+    const int64_t pairs = (int64_t)B * Hk;
+    const bool q_split = pairs * tiles(longest_q * a.G, BM) <= 128 || longest_q * a.G <= 32,
+               k_split = pairs * tiles(longest_k, 128) <= 256 || longest_k <= 32;
+    const int qt = (int)tiles(longest_q * a.G, q_split ? 32 : BM), kt = (int)tiles(longest_k, k_split ? 32 : 128);
     const long long q_rest = places(B * Hk, qt), k_rest = places(B * Hk, kt);
     if (q_rest > 0x7ffffff0ll || k_rest > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+    const bool q_one = longest_k <= 64, k_one = longest_q * a.G <= 64;      // not more than two blocks for the waves to share
+    hipStream_t st = (hipStream_t)stream;
     if (Tq > 0) {
-        BY_HEAD(k_attn_gq, dim3((unsigned)q_rest + REST), (hipStream_t)stream, a, qt, (unsigned)q_rest);
+        const dim3 grid((unsigned)q_rest + REST);
+#define GQ(TY, W)                                                                                                                       \
+    do {                                                                                                                                \
+        constexpr int NW = sizeof(TY) * W > 256 ? 2 : 4;                                                                                \
+        if (!q_split) hipLaunchKernelGGL((k_attn_gq<TY, W>), grid, dim3(256), 0, st, a, qt, (unsigned)q_rest);                          \
+        else if (q_one) hipLaunchKernelGGL((k_attn_gq_split<TY, W, 1>), grid, dim3(64), 0, st, a, qt, (unsigned)q_rest);                \
+        else hipLaunchKernelGGL((k_attn_gq_split<TY, W, NW>), grid, dim3(NW * 64), 0, st, a, qt, (unsigned)q_rest);                     \
+    } while (0)
+        if (dtype == 0) { if (D <= 32) GQ(bf16_t, 32); else if (D <= 64) GQ(bf16_t, 64); else GQ(bf16_t, 128); }
+        else { if (D <= 32) GQ(float, 32); else if (D <= 64) GQ(float, 64); else GQ(float, 128); }
+#undef GQ
         if (int rc = launched("sam3_seq_attn_bwd")) return rc;
     }
     if (Tk > 0) {
         const dim3 grid((unsigned)k_rest + REST);
-        hipStream_t st = (hipStream_t)stream;
-#define GKV(TY, W)                                                                                                                        \
-    do {                                                                                                                                  \
-        if (GkvCfg<TY, W>::BR % a.G == 0) hipLaunchKernelGGL((k_attn_gkv<TY, W, true>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest); \
-        else hipLaunchKernelGGL((k_attn_gkv<TY, W, false>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest);                             \
+#define GKV(TY, W)                                                                                                                      \
+    do {                                                                                                                                \
+        constexpr int NW = sizeof(TY) * W > 256 ? 2 : 4;                                                                                \
+        if (!k_split) { if (GkvCfg<TY, W>::BR % a.G == 0) hipLaunchKernelGGL((k_attn_gkv<TY, W, true>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest); \
+                        else hipLaunchKernelGGL((k_attn_gkv<TY, W, false>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest); }          \
+        else if (k_one) { if (32 % a.G == 0) hipLaunchKernelGGL((k_attn_gkv_split<TY, W, 1, true>), grid, dim3(64), 0, st, a, kt, (unsigned)k_rest);      \
+                          else hipLaunchKernelGGL((k_attn_gkv_split<TY, W, 1, false>), grid, dim3(64), 0, st, a, kt, (unsigned)k_rest); } \
+        else { if (32 % a.G == 0) hipLaunchKernelGGL((k_attn_gkv_split<TY, W, NW, true>), grid, dim3(NW * 64), 0, st, a, kt, (unsigned)k_rest);           \
+               else hipLaunchKernelGGL((k_attn_gkv_split<TY, W, NW, false>), grid, dim3(NW * 64), 0, st, a, kt, (unsigned)k_rest); }      \
     } while (0)
         if (dtype == 0) { if (D <= 32) GKV(bf16_t, 32); else if (D <= 64) GKV(bf16_t, 64); else GKV(bf16_t, 128); }
         else { if (D <= 32) GKV(float, 32); else if (D <= 64) GKV(float, 64); else GKV(float, 128); }
