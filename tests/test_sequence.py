@@ -452,6 +452,28 @@ def test_packed_attention_and_gradients(case, dtype):
     check_attention(*case, dtype, seed=len(case[0]) + case[4])
 
 
+MANY = [  # as above, often enough for the tiles of 128 rows and keys (more than 256 of them over the pairs)
+    ([130, 70, 1, 0, 65], 2, 2, 64, True, 40), ([200, 3], 4, 2, 128, True, 50), ([33, 140], 3, 1, 32, True, 150), ([90], 7, 1, 64, True, 260),
+    ([150, 64], 6, 2, 96, False, 60), ([129], 10, 2, 128, False, 70), ([40, 31], 5, 1, 128, True, 140)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(str(v).replace(" ", "") for v in c))
+def test_packed_attention_many_sequences(case, dtype):
+    lens, hq, hk, d, causal, times = case
+    check_attention(lens * times, lens * times, hq, hk, d, causal, dtype, seed=d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_many_sequences_of_other_key_lengths(d, dtype):
+    lq, lk = [40, 100, 7, 0, 130] * 30, [140, 60, 7, 9, 200] * 30
+    for causal in (True, False):
+        check_attention(lq, lk, 4, 2, d, causal, dtype, seed=d, hints=causal)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DT, ids=ids)
 def test_packed_attention_hints_and_scale(dtype):
@@ -534,24 +556,29 @@ def test_packed_attention_rows_of_no_sequence_and_bad_bounds(dtype):
 @pytest.mark.parametrize("dtype", DT, ids=ids)
 @pytest.mark.parametrize("n,hq,hk,d", [(100, 2, 1, 64), (200, 4, 4, 128), (300, 3, 1, 32)])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
-def test_packed_attention_what_a_query_does_not_see_stays_out(value, n, hq, hk, d, dtype):
-    """A token that is not finite spoils the results that depend on it and no others, forward and backward."""
+@pytest.mark.parametrize("others", [0, 300])
+def test_packed_attention_what_a_query_does_not_see_stays_out(others, value, n, hq, hk, d, dtype):
+    """A token that is not finite spoils the results that depend on it and no others, forward and backward; with 300 more sequences the
+    kernels for many tiles run."""
     g = gen(n)
-    q, k, v, go = (rand(g, n, h, d, dtype=dtype).to("cuda", dtype) for h in (hq, hk, hk, hq))
-    cu = ends([n])
+    total = n + 16 * others
+    q, k, v, go = (rand(g, total, h, d, dtype=dtype).to("cuda", dtype) for h in (hq, hk, hk, hq))
+    cu = ends([n] + [16] * others)
     at, el = n // 2 + 3, 5
 
     def grads(q, k, v, go):
         leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
-        out = sequence.packed_attention(*leaves, cu)
-        return (out,) + torch.autograd.grad(out, leaves, go)
+        out = sequence.packed_attention(*leaves, cu, max_q=n, max_k=n)
+        got = (out,) + torch.autograd.grad(out, leaves, go)
+        assert all(torch.isfinite(t[n:]).all() for t in got)
+        return tuple(t[:n] for t in got)
     good = grads(q, k, v, go)
     bad_v = v.clone()
     bad_v[at, :, el] = value
     out, gq, gk, gv = grads(q, k, bad_v, go)
     assert torch.equal(out[:at], good[0][:at]) and not torch.isfinite(out[at:, :, el]).any()
-    others = [i for i in range(d) if i != el]
-    assert torch.equal(out[at:][..., others], good[0][at:][..., others])
+    rest = [i for i in range(d) if i != el]
+    assert torch.equal(out[at:][..., rest], good[0][at:][..., rest])
     if not math.isnan(value):
         assert (out[at:, :, el] == value).all()
     assert torch.equal(gq[:at], good[1][:at]) and not torch.isfinite(gq[at:]).all(-1).any()
