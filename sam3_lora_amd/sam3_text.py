@@ -9,8 +9,9 @@ Restates, for the training step of row a14, what ``sam3/model/tokenizer_ve.py:12
     ``c_proj`` / ``out_proj`` are adapter targets of the package API), and
   * a reference state dict must load with ``strict=True`` (``tests/golden/sam3_state_keys.json``).
 
-Everything here runs on stock PyTorch-ROCm (north star: only the LoRA adapter path is hand-written HIP); the adapted
-``nn.Linear``s inside it reach the HIP kernels through ``LoRALinear`` / ``LinearWithLoRA`` like any other.
+By default everything here runs on stock PyTorch-ROCm; the adapted ``nn.Linear``s inside it reach the HIP kernels through
+``LoRALinear`` / ``LinearWithLoRA`` like any other, and :func:`set_packed_text` moves the tower's attention to
+``sequence.packed_attention`` on the prompts' own tokens.
 
 Differences from the reference that are deliberate:
   * ``positional_embedding`` and ``text_projection`` get a seeded-init (N(0, 0.01) and N(0, width^-0.5)) instead of
@@ -32,10 +33,11 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 __all__ = ["SimpleTokenizer", "ResidualAttentionBlock", "Transformer", "TextTransformer", "VETextEncoder",
-           "LayerScale"]
+           "LayerScale", "set_packed_text"]
 
 SOT, EOT = "<start_of_text>", "<end_of_text>"
 N_MERGES = 49152 - 256 - 2          # merge rules kept from the vocabulary file (tokenizer_ve.py:142)
@@ -196,6 +198,22 @@ class ResidualAttentionBlock(nn.Module):
         x = q_x + self.ls_1(self.attn(h, k, v, need_weights=False, attn_mask=attn_mask)[0])
         return x + self.ls_2(self.mlp(self.ln_2(x)))
 
+    def forward_packed(self, x: torch.Tensor, cu: torch.Tensor, longest: int) -> torch.Tensor:
+        """:meth:`forward` with the causal mask on prompts that lie one behind the other: x [tokens, width], cu int32 [prompts + 1]."""
+        from .sequence import packed_attention
+        a = self.attn
+        qkv = F.linear(self.ln_1(x), a.in_proj_weight, a.in_proj_bias).view(x.shape[0], 3, a.num_heads, -1)
+        o = packed_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], cu, max_q=longest, max_k=longest)
+        x = x + self.ls_1(F.linear(o.flatten(1), a.out_proj.weight, a.out_proj.bias))
+        return x + self.ls_2(self.mlp(self.ln_2(x)))
+
+    def packs(self) -> bool:
+        """Whether :meth:`forward_packed` computes what :meth:`forward` does."""
+        a = self.attn
+        return (a._qkv_same_embed_dim and a.bias_k is None and not a.add_zero_attn and a.in_proj_bias is not None
+                and not (a.dropout > 0 and self.training) and a.head_dim % 8 == 0 and a.head_dim <= 128
+                and a.in_proj_weight.dtype in (torch.bfloat16, torch.float32) and not torch.is_autocast_enabled("cuda"))
+
 
 class Transformer(nn.Module):
     def __init__(self, width: int, layers: int, heads: int, mlp_ratio: float = 4.0,
@@ -213,6 +231,14 @@ class Transformer(nn.Module):
                 x = checkpoint(blk, x, None, None, attn_mask, use_reentrant=False)
             else:
                 x = blk(x, attn_mask=attn_mask)
+        return x
+
+    def forward_packed(self, x: torch.Tensor, cu: torch.Tensor, longest: int) -> torch.Tensor:
+        for blk in self.resblocks:
+            if self.grad_checkpointing and self.training and torch.is_grad_enabled():
+                x = checkpoint(blk.forward_packed, x, cu, longest, use_reentrant=False)
+            else:
+                x = blk.forward_packed(x, cu, longest)
         return x
 
 
@@ -270,9 +296,30 @@ class TextTransformer(nn.Module):
         return (pooled, tokens) if self.output_tokens else pooled
 
 
+    def forward_packed(self, text: torch.Tensor, lengths: Sequence[int]) -> torch.Tensor:
+        """The tokens of :meth:`forward` (``pool_type="none"``) for prompts of ``lengths`` ids each, without the work on the padding behind
+        them: the causal mask lets no token see what follows it.  text [B, L] on the GPU; returns [B, L, width] with zeros in the padding."""
+        B, L = text.shape
+        rows = [b * L + i for b, n in enumerate(lengths) for i in range(n)]
+        at = torch.tensor(rows, dtype=torch.long).to(text.device, non_blocking=True)
+        cu = torch.tensor([0] + list(lengths)).cumsum(0).to(torch.int32).to(text.device, non_blocking=True)
+        x = self.token_embedding(text.reshape(-1)[at]) + self.positional_embedding[at % L]
+        x = self.ln_final(self.transformer.forward_packed(x, cu, max(lengths)))
+        return x.new_zeros(B * L, x.shape[-1]).index_copy(0, at, x).view(B, L, -1)
+
+    def packs(self) -> bool:
+        return self.attn_mask is not None and self.pool_type == "none" and all(b.packs() for b in self.transformer.resblocks)
+
+
 class VETextEncoder(nn.Module):
     """``forward(list_of_str, device=) -> (padding_mask[B, L] (True = pad), memory[L, B, d_model], embeds[L, B, width])``
-    -- text_encoder_ve.py:255-328: tokenise to ``context_length`` = 32, run the tower, ``resizer`` to the DETR width."""
+    -- text_encoder_ve.py:255-328: tokenise to ``context_length`` = 32, run the tower, ``resizer`` to the DETR width.
+
+    ``packed`` (off by default, :func:`set_packed_text`): on a GPU the tower runs on the prompts' own tokens, one prompt behind the other
+    (``sequence.packed_attention``), instead of on ``context_length`` tokens each; memory and mask come out as before, except that the
+    memory's rows under the mask hold the resizer's bias."""
+
+    packed = False
 
     def __init__(self, d_model: int, tokenizer: Callable, width: int = 1024, heads: int = 16, layers: int = 24,
                  context_length: int = 32, vocab_size: int = 49408, use_ln_post: bool = True,
@@ -289,8 +336,28 @@ class VETextEncoder(nn.Module):
             mask, memory, tokenized = text
             return mask, memory, tokenized["inputs_embeds"].transpose(0, 1)
         assert input_boxes is None or len(input_boxes) == 0, "not supported"
-        ids = self.tokenizer(text, context_length=self.context_length).to(device)
+        ids = self.tokenizer(text, context_length=self.context_length)
+        lengths = self._lengths(ids) if self.packed else None
+        ids = ids.to(device)
         embeds = self.encoder.token_embedding(ids)
-        _, tokens = self.encoder(ids)
+        if lengths is not None and ids.is_cuda and sum(lengths) > 0 and self.encoder.packs():
+            tokens = self.encoder.forward_packed(ids, lengths)
+        else:
+            _, tokens = self.encoder(ids)
         memory = self.resizer(tokens.transpose(0, 1))
         return ids == 0, memory, embeds.transpose(0, 1)
+
+    @staticmethod
+    def _lengths(ids: torch.Tensor) -> List[int]:
+        """Tokens of each prompt: up to its last id that is not padding (the end-of-text id is never 0; an id in the middle may be)."""
+        used = ids != 0
+        last = ids.shape[1] - used.flip(1).int().argmax(1)
+        return torch.where(used.any(1), last, torch.zeros_like(last)).tolist()
+
+
+def set_packed_text(model: nn.Module, on: bool = True) -> int:
+    """Switches the packed text tower of every :class:`VETextEncoder` in ``model``; returns how many there are."""
+    found = [m for m in model.modules() if isinstance(m, VETextEncoder)]
+    for m in found:
+        m.packed = bool(on)
+    return len(found)

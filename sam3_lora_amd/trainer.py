@@ -33,7 +33,8 @@ Settings that exist only on this engine live under an optional ``engine:`` secti
 behaviour) and as command-line switches: ``bf16_frozen`` (frozen tensors in bf16, A/B fp32 masters),
 ``act_checkpoint`` (keep | auto | on | off), ``match_once`` (skip the model-internal matching that the loop repeats),
 ``loader_workers`` / ``loader_prefetch`` (samples built by a thread pool and batches copied to the GPU ahead of the step;
-0 = the reference's ``num_workers=0``), ``grad_accumulation_steps``, ``direct_grad``, ``fp8_frozen``.
+0 = the reference's ``num_workers=0``), ``grad_accumulation_steps``, ``direct_grad``, ``fp8_frozen``, ``packed_text`` (the text
+tower on the prompts' own tokens).
 """
 from __future__ import annotations
 
@@ -275,6 +276,9 @@ class SAM3TrainerNative:
                 raise ValueError("engine.fp8_frozen requires engine.bf16_frozen (fp8 operands are cut from bf16 tensors)")
             from .fp8 import enable_fp8_frozen
             enable_fp8_frozen(True)
+        if engine.get("packed_text", False):    # the text tower without its padding (sam3_text.set_packed_text)
+            from .sam3_text import set_packed_text
+            set_packed_text(self.model)
         if act_checkpoint != "keep":   # "auto" | "on" | "off" for this library's ViT trunk (vit.set_activation_checkpointing)
             from .vit import set_activation_checkpointing
             mode = {"on": True, "off": False}.get(act_checkpoint, "auto")

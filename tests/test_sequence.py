@@ -811,3 +811,86 @@ def test_a_block_of_the_operators_together():
     want = (OUT,) + torch.autograd.grad(OUT, (X, R, W, a, b), gy.double())
     for name, t, u in zip(("out", "x", "r", "w", "A", "B"), got, want):
         assert (t.cpu().double() - u).abs().max() <= 1e-4 * u.abs().max(), name
+
+
+# --------------------------------------------------------------------------------------------------- packed text tower
+PROMPTS = ["crack", "a dog", "person", "cat"]
+
+
+def tower(device, dtype, seed=0):
+    from sam3_lora_amd.sam3_text import VETextEncoder
+    lens = {p: n for p, n in zip(PROMPTS, (3, 9, 32, 1))}
+
+    def tokenizer(texts, context_length):
+        ids = torch.zeros(len(texts), context_length, dtype=torch.long)
+        for row, t in enumerate(texts):
+            n = lens[t]
+            ids[row, :n] = torch.randint(1, 300, (n,), generator=gen(len(t)))
+            if n > 4:
+                ids[row, 2] = 0         # an id like the padding's in the middle of a prompt
+        return ids
+    torch.manual_seed(seed)
+    enc = VETextEncoder(d_model=64, tokenizer=tokenizer, width=128, heads=4, layers=3, context_length=32, vocab_size=300, use_act_checkpoint=True)
+    return enc.to(device, dtype)
+
+
+def test_packed_text_switch_and_lengths_on_the_cpu():
+    from sam3_lora_amd.sam3_text import VETextEncoder, set_packed_text
+    ids = torch.tensor([[5, 6, 0, 7, 0, 0], [0, 0, 0, 0, 0, 0], [1, 2, 3, 4, 5, 6]])
+    assert VETextEncoder._lengths(ids) == [4, 0, 6]
+    enc = tower("cpu", torch.float32).eval()
+    with torch.no_grad():
+        want = enc(PROMPTS, device="cpu")
+        assert set_packed_text(torch.nn.ModuleList([enc])) == 1 and enc.packed
+        got = enc(PROMPTS, device="cpu")          # no GPU: the padded form
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("train", [False, True])
+def test_packed_text_tower_equals_the_padded_one(train, dtype):
+    """Three pre-norm blocks of 128: both forms round the same expressions at the same places in bf16 (2^-8 of values that the residual keeps
+    near their start; a token passes 3 x 6 roundings) and differ in the order of fp32 sums otherwise (3 x 128 terms and more)."""
+    from sam3_lora_amd.sam3_text import set_packed_text
+    enc = tower("cuda", dtype)
+    enc.train(train)
+    g = torch.randn(32, len(PROMPTS), 64, generator=gen(3)).to("cuda", dtype)
+    results = []
+    for on in (False, True):
+        set_packed_text(enc, on)
+        enc.zero_grad()
+        mask, memory, embeds = enc(PROMPTS, device="cuda")
+        keep = ~mask.t()[..., None]
+        if train:
+            (memory * g * keep).float().sum().backward()
+        results.append((mask, (memory * keep).detach(), embeds.detach(), {n: p.grad.clone() for n, p in enc.named_parameters() if p.grad is not None}))
+    (m0, a, e0, g0), (m1, b, e1, g1) = results
+    assert torch.equal(m0, m1) and torch.equal(e0, e1) and set(g0) == set(g1)
+    tol = 18 * unit(dtype) if dtype == torch.bfloat16 else 2000 * F
+    assert (a - b).float().abs().max() <= tol * a.float().abs().max()
+    for n in g0:
+        assert (g0[n] - g1[n]).float().norm() <= tol * max(g0[n].float().norm(), 1e-6), n
+
+
+@pytest.mark.gpu
+def test_packed_text_in_the_whole_model():
+    """The tiny SAM3 image model in fp32: the loss does not change when its text tower runs packed (what the mask hides is not used)."""
+    from sam3_lora_amd.sam3_data import SyntheticSegmentDataset, collate_fn_api
+    from sam3_lora_amd.sam3_image import TINY_CONFIG, build_sam3_image_model
+    from sam3_lora_amd.sam3_text import set_packed_text
+    from sam3_lora_amd.trainer import build_criterion, match_all_steps, move_to_device
+    cfg = dict(TINY_CONFIG, text=dict(TINY_CONFIG["text"], vocab_size=49408, context_length=32))
+    ds = SyntheticSegmentDataset(2, resolution=112, source=128)
+    batch = move_to_device(collate_fn_api([ds[0], ds[1]], dict_key="input", with_seg_masks=True)["input"], "cuda")
+    model = build_sam3_image_model(device="cpu", eval_mode=False, config=cfg, match_in_forward=False, act_checkpoint=False, seed=6).to("cuda").train()
+    _, wrapper = build_criterion("local")
+    losses = []
+    for on in (False, True):
+        assert set_packed_text(model, on) == 1
+        torch.manual_seed(0)
+        out = model(batch)
+        targets = [model.back_convert(t) for t in batch.find_targets]
+        match_all_steps(wrapper, out.output, targets)
+        losses.append(float(wrapper(out, targets)["core_loss"].detach()))
+    assert abs(losses[0] - losses[1]) <= 1e-4 * abs(losses[0]), losses
