@@ -24,7 +24,7 @@ const char* sam3_seq_last_error(void);
  * weight has the activations' type.  Outputs, each NULL or contiguous [M, C]:  y;  h_out (h, rounded once);  rstd_out [M] fp32
  * (what the backward takes);  q8 [M, C] bytes with scales fp32 [M, C / group] (group 32, 64 or 128; 0: [M, 1]):
  *   scale = max(max|y|, 2^-24) / fmt_max over the group's unrounded y,   q8 = fp8(y / scale)   (fmt: sam3_fp8_amd.h)
- * A row with a NaN or an infinity has NaN in all its outputs but h_out, its scales among them.
+ * A row with a NaN has NaN in all its outputs but h_out.
  */
 int sam3_seq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* y, void* h_out,
                           float* rstd_out, void* q8, float* scales, int group, int fmt, int64_t M, int C, float eps, int dtype,
@@ -55,7 +55,8 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
 
 /*
  * Attention over packed sequences with grouped heads.
- *   q [Tq, Hq, D], k, v [Tk, Hk, D], strides (token, head) in elements, unit inside a head; Hq % Hk == 0, D % 8 == 0, D <= 128.
+ *   q [Tq, Hq, D], k, v [Tk, Hk, D], strides (token, head) in elements below 2^22, unit inside a head, 16-byte alignment throughout;
+ *   Hq % Hk == 0, D % 8 == 0, D <= 128.
  *   Sequence b of B owns the query rows cu_q[b] .. cu_q[b+1] - 1 and the key rows cu_k[b] .. cu_k[b] + n - 1 with
  *   n = len_k[b], or cu_k[b+1] - cu_k[b] where len_k is NULL (int32, device; values outside the tensors are clamped to them).
  *   causal: query i of n_q sees the keys j <= i + n - n_q (the last query sees all); otherwise every key.

@@ -38,17 +38,15 @@ def _check(rc: int, what: str) -> None:
         raise LoRAKernelError(f"{what} failed (code {rc}): {(_ffi.load().sam3_seq_last_error() or b'').decode()}")
 
 
-def _need(ok, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
 def _activation(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
-    """Checks an activation; its place and type are ``like``'s."""
+    """Checks an activation; its place and type are ``like``'s.  (The messages are made where they are needed only: a small call is
+    over in about 15 us.)"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if like is not None and (t.device != like.device or t.dtype != like.dtype):
-        raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if like is not None:
+        if t.dtype is not like.dtype or t.device != like.device:
+            raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+        return
     if t.dtype not in _TYPE_CODES:
         raise LoRAKernelError(f"sam3_lora_amd: activations must be bfloat16 or float32, got {t.dtype} for {name}")
     if not t.is_cuda:
@@ -165,14 +163,16 @@ class _RMSNorm(torch.autograd.Function):
 def _norm_args(x, weight, residual, eps):
     _activation("x", x)
     _activation("weight", weight, x)
-    _need(x.dim() >= 1 and weight.dim() == 1 and x.shape[-1] == weight.shape[0],
-          f"weight must have x's last dimension: got x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    _need(x.shape[-1] > 0 and x.shape[-1] % 8 == 0 and x.shape[-1] <= 16384,
-          f"the normalised dimension must be a multiple of 8 up to 16384, got {x.shape[-1]}")
+    if x.dim() == 0 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"weight must have x's last dimension: got x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    if not 0 < x.shape[-1] <= 16384 or x.shape[-1] % 8:
+        raise ValueError(f"the normalised dimension must be a multiple of 8 up to 16384, got {x.shape[-1]}")
     if residual is not None:
         _activation("residual", residual, x)
-        _need(residual.shape == x.shape, f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
-    _need(0.0 <= eps < 3e38, f"eps must be finite and not negative, got {eps}")
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if not 0.0 <= eps < 3e38:
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
@@ -199,10 +199,11 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
     require a gradient are refused where gradients are recorded.
     """
     _norm_args(x, weight, residual, eps)
-    _need(fmt in _FP8_TYPES, f"fmt must be FP8_E4M3 or FP8_E5M2, got {fmt}")
-    _need(group == 0 or (group in (32, 64, 128) and x.shape[-1] % group == 0),
-          f"group must be 0, or 32, 64 or 128 and divide {x.shape[-1]}, got {group}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if fmt not in _FP8_TYPES:
+        raise ValueError(f"fmt must be FP8_E4M3 or FP8_E5M2, got {fmt}")
+    if group != 0 and (group not in (32, 64, 128) or x.shape[-1] % group):
+        raise ValueError(f"group must be 0, or 32, 64 or 128 and divide {x.shape[-1]}, got {group}")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         raise ValueError("rms_norm_q8 has no gradient: call it under torch.no_grad(), or rms_norm for training")
     _, h, _, image, scales = _norm_fwd(x, residual, weight, eps, False, False, (group, fmt))
     return (image, scales) if residual is None else (image, scales, h)
@@ -210,8 +211,14 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
 
 # --------------------------------------------------------------------------------------------------- rotary positions
 @lru_cache(maxsize=256)
-def _rotation_table(sections: Tuple[int, ...], theta: float, spectrum: str):
-    """(turns per position step, axis) of each pair as the C arrays that a call reads."""
+def _rotation_table(sections: Tuple[int, ...], theta: float, spectrum: str, d: int):
+    """(turns per position step, axis) of each pair as the C arrays that a call reads, and their number."""
+    if not (len(sections) > 0 and all(n >= 0 for n in sections) and 0 < 2 * sum(sections) <= d):
+        raise ValueError(f"sections {sections} do not fit a head of {d}")
+    if spectrum not in ("shared", "per_axis"):
+        raise ValueError(f"spectrum must be 'shared' or 'per_axis', got {spectrum!r}")
+    if not 0.0 < theta < float("inf"):
+        raise ValueError(f"theta must be positive and finite, got {theta}")
     pairs = sum(sections)
     two_pi = 6.283185307179586476925286766559
     turns, axis = [], []
@@ -282,26 +289,26 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     Angles are reduced in 64 bits, so far positions keep their precision.  Differentiable in q and k.
     """
     _activation("q", q)
-    _need(q.dim() >= 2 and q.shape[-1] > 0 and q.shape[-1] % 8 == 0 and q.shape[-1] <= 256,
-          f"q must be [..., heads, D] with D a multiple of 8 up to 256, got {tuple(q.shape)}")
+    if q.dim() < 2 or not 0 < q.shape[-1] <= 256 or q.shape[-1] % 8:
+        raise ValueError(f"q must be [..., heads, D] with D a multiple of 8 up to 256, got {tuple(q.shape)}")
     if k is not None:
         _activation("k", k, q)
-        _need(k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == q.shape[-1],
-              f"k must have q's tokens and head size: got q {tuple(q.shape)}, k {tuple(k.shape)}")
-    _need(q.shape[-2] > 0 and (k is None or k.shape[-2] > 0), "q and k must have heads")
-    sections = tuple(int(n) for n in sections)
-    _need(len(sections) > 0 and all(n >= 0 for n in sections) and 0 < 2 * sum(sections) <= q.shape[-1],
-          f"sections {sections} do not fit a head of {q.shape[-1]}")
-    _need(pairing in ("adjacent", "halves"), f"pairing must be 'adjacent' or 'halves', got {pairing!r}")
-    _need(spectrum in ("shared", "per_axis"), f"spectrum must be 'shared' or 'per_axis', got {spectrum!r}")
-    theta = float(theta)
-    _need(0.0 < theta < float("inf"), f"theta must be positive and finite, got {theta}")
+        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise ValueError(f"k must have q's tokens and head size: got q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if q.shape[-2] == 0 or (k is not None and k.shape[-2] == 0):
+        raise ValueError("q and k must have heads")
+    if type(sections) is not tuple:
+        sections = tuple(int(n) for n in sections)
+    table = _rotation_table(sections, float(theta), spectrum, q.shape[-1])
+    if pairing not in ("adjacent", "halves"):
+        raise ValueError(f"pairing must be 'adjacent' or 'halves', got {pairing!r}")
     if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_TYPES:
         raise TypeError("positions must be an int32, int64 or float32 tensor")
-    _need(positions.device == q.device and positions.shape == (len(sections),) + q.shape[:-2],
-          f"positions must be {(len(sections),) + tuple(q.shape[:-2])} on {q.device}, got {tuple(positions.shape)} on {positions.device}")
-    _need(not positions.requires_grad, "positions have no gradient")
-    table = _rotation_table(sections, theta, spectrum)
+    if positions.device != q.device or positions.dim() == 0 or positions.shape[0] != len(sections) or positions.shape[1:] != q.shape[:-2]:
+        raise ValueError(f"positions must be {(len(sections),) + tuple(q.shape[:-2])} on {q.device}, got {tuple(positions.shape)} on "
+                         f"{positions.device}")
+    if positions.requires_grad:
+        raise ValueError("positions have no gradient")
     halves = pairing == "halves"
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryAxes.apply(q, k, positions, table, halves)
@@ -328,17 +335,22 @@ def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse,
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(),
             _ptr(len_k), out.data_ptr(), _ptr(lse), _ptr(stats), tq, tk, b, hq, hk, d, max_q, max_k, causal, scale, dt, _ptr(ws), nbytes,
             _stream(q.device)), "sam3_seq_attn_fwd")
-    return out, lse, stats
+    return out, lse, stats, (q, k, v), qs + ks + vs
 
 
 class _PackedAttention(torch.autograd.Function):
-    """``(out, lse)``, lse None where it is not wanted."""
+    """``(out, lse)``, lse None where it is not wanted.  What does not change until the backward is worked out here: that runs in
+    another thread, where Python is slower."""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, causal, scale, want_lse):
-        out, lse, stats = _attn_fwd(q, k, v, cu_q, cu_k, None, max_q, max_k, causal, scale, want_lse, True)
+        out, lse, stats, (q, k, v), strides = _attn_fwd(q, k, v, cu_q, cu_k, None, max_q, max_k, causal, scale, want_lse, True)
         ctx.save_for_backward(q, k, v, out, stats, cu_q, cu_k)
-        ctx.how = max_q, max_k, causal, scale
+        tq, hq, d = q.shape
+        tk, hk = k.shape[:2]
+        ctx.strides = strides
+        ctx.nbytes = _ffi.load().sam3_seq_attn_bwd_workspace_bytes(tq, hq)
+        ctx.shape = tq, tk, cu_q.shape[0] - 1, hq, hk, d, max_q, max_k, causal, scale, _TYPE_CODES[q.dtype]
         ctx.set_materialize_grads(False)
         if lse is not None:
             ctx.mark_non_differentiable(lse)
@@ -350,21 +362,16 @@ class _PackedAttention(torch.autograd.Function):
         if go is None:
             return (None,) * 10
         q, k, v, out, stats, cu_q, cu_k = ctx.saved_tensors
-        max_q, max_k, causal, scale = ctx.how
-        tq, hq, d = q.shape
-        tk, hk = k.shape[:2]
-        q, k, v, go = _aligned(q), _aligned(k), _aligned(v), _aligned(go)
+        go = _aligned(go)
         gq, gk, gv = _new(q), _new(k), _new(v)
-        qs, ks, vs, gs = q.stride(), k.stride(), v.stride(), go.stride()
-        lib = _ffi.load()
-        nbytes = lib.sam3_seq_attn_bwd_workspace_bytes(tq, hq)
-        ws = q.new_empty(nbytes, dtype=torch.uint8)
+        qt, qh, _, kt, kh, _, vt, vh, _ = ctx.strides
+        gs = go.stride()
+        ws = q.new_empty(ctx.nbytes, dtype=torch.uint8)
         with _on(q.device):
-            _check(lib.sam3_seq_attn_bwd(
-                q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], go.data_ptr(), gs[0], gs[1],
-                out.data_ptr(), stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), tq, tk,
-                cu_q.shape[0] - 1, hq, hk, d, max_q, max_k, causal, scale, _TYPE_CODES[q.dtype], ws.data_ptr(), nbytes,
-                _stream(q.device)), "sam3_seq_attn_bwd")
+            _check(_ffi.load().sam3_seq_attn_bwd(
+                q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, go.data_ptr(), gs[0], gs[1], out.data_ptr(),
+                stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *ctx.shape, ws.data_ptr(),
+                ctx.nbytes, _stream(q.device)), "sam3_seq_attn_bwd")
         need = ctx.needs_input_grad
         return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None) + (None,) * 7
 
@@ -372,8 +379,8 @@ class _PackedAttention(torch.autograd.Function):
 def _index(name: str, t: torch.Tensor, n: int, device) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
         raise TypeError(f"{name} must be an int32 tensor")
-    _need(t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.device == device,
-          f"{name} must be a contiguous [{n}] on {device}, got {tuple(t.shape)} on {t.device}")
+    if t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{n}] on {device}, got {tuple(t.shape)} on {t.device}")
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: Optional[torch.Tensor] = None, *,
@@ -381,8 +388,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
                      scale: Optional[float] = None, return_lse: bool = False):
     """Softmax attention over sequences of different lengths that lie one behind the other; returns out [Tq, Hq, D].
 
-    q: [Tq, Hq, D], k, v: [Tk, Hk, D], one type (bf16 or fp32), any strides (views of a fused projection or of a cache); Hq a multiple
-    of Hk: head h of q reads head ``h // (Hq / Hk)`` of k and v.  D a multiple of 8, at most 128.
+    q: [Tq, Hq, D], k, v: [Tk, Hk, D], one type (bf16 or fp32), strided as they come (views of a fused projection or of a cache; rows less
+    than 2^22 elements apart); Hq a multiple of Hk: head h of q reads head ``h // (Hq / Hk)`` of k and v.  D a multiple of 8, at most 128.
     cu_q, cu_k: int32 [B + 1] on the GPU; sequence b is rows ``cu_q[b]:cu_q[b + 1]`` of q and ``cu_k[b]:cu_k[b + 1]`` of k and v
     (cu_k None: the same rows).  Sequences may be empty.  Rows in front of the first and behind the last sequence give zeros.
     causal: the last query of a sequence sees all its keys, the one before it all but the last, and so on; False: all see all.  A query
@@ -397,30 +404,36 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     _activation("q", q)
     _activation("k", k, q)
     _activation("v", v, q)
-    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.shape[2] == k.shape[2],
-          f"q must be [Tq, Hq, D] and k, v [Tk, Hk, D]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+        raise ValueError(f"q must be [Tq, Hq, D] and k, v [Tk, Hk, D]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     (tq, hq, d), (tk, hk) = q.shape, k.shape[:2]
-    _need(hq > 0 and hk > 0 and hq % hk == 0, f"{hq} query heads do not share {hk} key heads")
-    _need(d > 0 and d % 8 == 0 and d <= 128, f"the head size must be a multiple of 8 up to 128, got {d}")
+    if hq == 0 or hk == 0 or hq % hk:
+        raise ValueError(f"{hq} query heads do not share {hk} key heads")
+    if d == 0 or d % 8 or d > 128:
+        raise ValueError(f"the head size must be a multiple of 8 up to 128, got {d}")
     if not isinstance(cu_q, torch.Tensor) or cu_q.dim() != 1 or cu_q.numel() < 1:
         raise TypeError("cu_q must be an int32 tensor [B + 1]")
     n = cu_q.numel()
     _index("cu_q", cu_q, n, q.device)
     if cu_k is None:
-        _need(tk == tq, f"without cu_k, k and v must have q's {tq} rows, got {tk}")
+        if tk != tq:
+            raise ValueError(f"without cu_k, k and v must have q's {tq} rows, got {tk}")
         cu_k = cu_q
     else:
         _index("cu_k", cu_k, n, q.device)
     if len_k is not None:
         _index("len_k", len_k, n - 1, q.device)
     for name, m in (("max_q", max_q), ("max_k", max_k)):
-        _need(m is None or (isinstance(m, int) and 0 <= m < 2 ** 31), f"{name} must be a length, got {m}")
+        if m is not None and not (isinstance(m, int) and 0 <= m < 2 ** 31):
+            raise ValueError(f"{name} must be a length, got {m}")
     max_q, max_k = tq if max_q is None else min(max_q, tq), tk if max_k is None else min(max_k, tk)
     scale = d ** -0.5 if scale is None else float(scale)
-    _need(0.0 < scale < 3e38, f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        _need(len_k is None, "len_k has no gradient: call packed_attention under torch.no_grad()")
+        if len_k is not None:
+            raise ValueError("len_k has no gradient: call packed_attention under torch.no_grad()")
         out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, bool(causal), scale, return_lse)
     else:
-        out, lse, _ = _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, bool(causal), scale, return_lse)
+        out, lse, _, _, _ = _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, bool(causal), scale, return_lse)
     return (out, lse) if return_lse else out

@@ -442,7 +442,8 @@ ATTN = [  # query lengths, key lengths, heads, kv heads, D, causal
     ([0, 0], [0, 0], 2, 1, 64, True), ([4], [300], 4, 2, 64, True), ([40, 3], [10, 3], 2, 1, 64, True), ([10, 5], [0, 7], 2, 1, 64, True),
     ([100], [35], 2, 2, 128, True), ([1, 1, 1], [1, 257, 64], 8, 2, 128, True), ([3, 2], [1000, 130], 4, 1, 64, True),
     ([70], [70], 2, 2, 64, False), ([1], [200], 2, 1, 64, False), ([150, 20], [33, 97], 4, 2, 32, False), ([64], [128], 2, 1, 128, False),
-    ([12, 0, 4], [0, 5, 9], 2, 1, 24, False), ([260], [260], 2, 1, 64, True), ([300], [300], 1, 1, 128, False)]
+    ([12, 0, 4], [0, 5, 9], 2, 1, 24, False), ([260], [260], 2, 1, 64, True), ([300], [300], 1, 1, 128, False),
+    ([9, 30], [9, 30], 40, 1, 64, True), ([5, 3], [70, 3], 64, 1, 32, True)]
 
 
 @pytest.mark.gpu
@@ -645,6 +646,19 @@ def test_packed_attention_cache_rows_beyond_32_bits():
         got, want = (torch.autograd.grad(sequence.packed_attention(*t, cu_q, cu_k), t, q) for t in (far, near))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     del big
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    for kind in ("norm", "rope", "attention"):
+        _, make = train_call(kind)
+        args = make(1)
+        leaf = args[0].detach().requires_grad_(True)
+        out = {"norm": lambda: sequence.rms_norm(leaf, args[1]), "rope": lambda: sequence.rotary_axes(leaf, None, args[2], (16, 8, 8)),
+               "attention": lambda: sequence.packed_attention(leaf, args[1], args[2], args[4], args[5])}[kind]()
+        g = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="once_differentiable|differentiate"):
+            torch.autograd.grad(g.float().sum(), leaf)
 
 
 def two_streams(call, make):
