@@ -10,6 +10,12 @@
 // the other index in registers: statistics of a row are a lane's own scalars, and the result turns into the second operand of the
 // next product without leaving the lane -- the sum over k runs in the order the registers hold it, and the other operand, read
 // from LDS by transposing reads, follows that order.
+//
+// Prompts are bound by the matrix cores and by what the chip may draw (it runs them at 1.75 to 2.0 GHz of 2.4): with 32 / 8 heads of 128
+// and 8192 tokens that all see each other the forward runs at 925 TF, gq at 1090 (three products) and gk, gv at 970 (four), where a
+// library product of 8192^3 runs at 1295; heads of 64 (16 of them, 4 x 5184 tokens) at 810, 910 and 910, the exponentials next to fewer
+// products.  The backward recomputes the scores in both of its kernels, seven products for the five of the formulas: one pass with sums
+// in memory would need atomics, whose order changes the result, or a second pass over 32-bit partial sums.
 #include "seq_common.inc"
 
 #include <type_traits>
@@ -1067,17 +1073,25 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             __syncthreads();
             dma.load(at_lds, at_lds + TB);
             if (son) word_to_lds(sp + r0, lane * 4, at_stat);
-            for (int t = 0; t < nfull; ++t, r0 += BR) {
+            const auto full = [&](auto buf, int t) {
+                constexpr int NOW = decltype(buf)::value, NEXT = 1 - NOW;
                 wait_loads<0>();
                 __syncthreads();
                 if (t + 1 < nfull) {
-                    const unsigned next = at_lds + ((t + 1) & 1) * 2 * TB;
                     dma.advance(a);
-                    dma.load(next, next + TB);
-                    if (son) word_to_lds(sp + r0 + BR, lane * 4, at_stat + ((t + 1) & 1) * (unsigned)sizeof(stat[0]));
+                    dma.load(at_lds + NEXT * 2 * TB, at_lds + NEXT * 2 * TB + TB);
+                    if (son) word_to_lds(sp + r0 + BR, lane * 4, at_stat + NEXT * (unsigned)sizeof(stat[0]));
                 }
-                step(std::false_type{}, t & 1, r0);
+                step(std::false_type{}, NOW, r0);
+                r0 += BR;
+            };
+            // Two steps at a time: the buffers' places are part of the instructions (heads of 128: 2335 -> 2270 us; the forward and gq gain nothing)
+            int t = 0;
+            for (; t + 1 < nfull; t += 2) {
+                full(std::integral_constant<int, 0>{}, t);
+                full(std::integral_constant<int, 1>{}, t + 1);
             }
+            if (t < nfull) full(std::integral_constant<int, 0>{}, t);
         }
         if (r0 < R) border(r0);
         if (live) {
