@@ -55,10 +55,11 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
 
 /*
  * Attention over packed sequences with grouped heads.
- *   q [Tq, Hq, D], k, v [Tk, Hk, D], strides (token, head) in elements below 2^22, unit inside a head, 16-byte alignment throughout;
- *   Hq % Hk == 0, D % 8 == 0, D <= 128.
+ *   q [Tq, Hq, D], k, v [Tk, Hk, D], strides (token, head) in elements, unit inside a head, 16-byte alignment throughout; below 2^22, but
+ *   those between the heads of k and v, and of q where Hq == Hk, which may be any.  Hq % Hk == 0, D % 8 == 0, D <= 128.
  *   Sequence b of B owns the query rows cu_q[b] .. cu_q[b+1] - 1 and the key rows cu_k[b] .. cu_k[b] + n - 1 with
- *   n = len_k[b], or cu_k[b+1] - cu_k[b] where len_k is NULL (int32, device; values outside the tensors are clamped to them).
+ *   n = len_k[b], or cu_k[b+1] - cu_k[b] where len_k is NULL (int32, device; cu_q and cu_k
+ *   do not decrease; values outside the tensors are clamped to them).
  *   causal: query i of n_q sees the keys j <= i + n - n_q (the last query sees all); otherwise every key.
  *   out [Tq, Hq, D] contiguous;  lse [Tq, Hq] fp32 (natural logarithm; NULL: not wanted).  A row that sees no key gives zeros and
  *   lse = -inf, and so do rows of no sequence.  stats [Tq, Hq, 2] fp32 is what the backward takes (NULL: not wanted).

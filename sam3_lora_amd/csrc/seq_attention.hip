@@ -1400,12 +1400,15 @@ int check(int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, i
     if (!(scale > 0.f) || scale > 3.0e38f) return sam3_seq_fail(EINVAL_, "attention: scale must be positive and finite");
     return 0;
 }
-int check_tensor(const char* name, const void* p, int64_t st, int64_t sh, int dtype) {
+// Offsets inside a tile of 64 rows are 32 bits: between tokens, and where a tile's rows are a group's heads (grouped) between these.  Key
+// heads are chosen by workgroups, in 64 bits: a cache may have its heads outside.
+int check_tensor(const char* name, const void* p, int64_t st, int64_t sh, bool grouped, int dtype) {
     if (!p) return sam3_seq_fail(EINVAL_, "attention: %s is a null pointer", name);
     if (misaligned(p) || bad_pitch(st, dtype) || bad_pitch(sh, dtype))
         return sam3_seq_fail(EINVAL_, "attention: %s: pointer and strides must keep 16-byte accesses aligned", name);
-    // (offsets inside a tile of 64 rows are 32 bits)
-    if (st < 0 || sh < 0 || st >= (1 << 22) || sh >= (1 << 22)) return sam3_seq_fail(ENOTSUP_, "attention: %s: strides must be below 2^22 elements", name);
+    if (st < 0 || sh < 0) return sam3_seq_fail(EINVAL_, "attention: %s: negative strides", name);
+    if (st >= (1 << 22) || (grouped && sh >= (1 << 22)))
+        return sam3_seq_fail(ENOTSUP_, "attention: %s: rows must be less than 2^22 elements apart", name);
     return 0;
 }
 
@@ -1475,10 +1478,10 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     sam3_seq_clear_error();
     if (int rc = check(Tq, Tk, B, Hq, Hk, D, max_q, max_k, scale, dtype)) return rc;
     if (Tq == 0) return 0;
-    if (int rc = check_tensor("q", q, q_st, q_sh, dtype)) return rc;
+    if (int rc = check_tensor("q", q, q_st, q_sh, Hq > Hk, dtype)) return rc;
     if (Tk > 0) {
-        if (int rc = check_tensor("k", k, k_st, k_sh, dtype)) return rc;
-        if (int rc = check_tensor("v", v, v_st, v_sh, dtype)) return rc;
+        if (int rc = check_tensor("k", k, k_st, k_sh, false, dtype)) return rc;
+        if (int rc = check_tensor("v", v, v_st, v_sh, false, dtype)) return rc;
     }
     if (!cu_q || !cu_k || !out || misaligned(out)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
     if (B == 0) max_q = max_k = 0;
@@ -1529,15 +1532,15 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     sam3_seq_clear_error();
     if (int rc = check(Tq, Tk, B, Hq, Hk, D, max_q, max_k, scale, dtype)) return rc;
     if (Tq > 0) {
-        if (int rc = check_tensor("q", q, q_st, q_sh, dtype)) return rc;
-        if (int rc = check_tensor("go", go, go_st, go_sh, dtype)) return rc;
+        if (int rc = check_tensor("q", q, q_st, q_sh, Hq > Hk, dtype)) return rc;
+        if (int rc = check_tensor("go", go, go_st, go_sh, Hq > Hk, dtype)) return rc;
         if (!out || !stats || !gq || misaligned(out) || misaligned(gq)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
         if (!workspace || workspace_bytes < sam3_seq_attn_bwd_workspace_bytes(Tq, Hq))
             return sam3_seq_fail(ENOMEM_, "attention: workspace too small: %zu < %zu", workspace_bytes, sam3_seq_attn_bwd_workspace_bytes(Tq, Hq));
     }
     if (Tk > 0) {
-        if (int rc = check_tensor("k", k, k_st, k_sh, dtype)) return rc;
-        if (int rc = check_tensor("v", v, v_st, v_sh, dtype)) return rc;
+        if (int rc = check_tensor("k", k, k_st, k_sh, false, dtype)) return rc;
+        if (int rc = check_tensor("v", v, v_st, v_sh, false, dtype)) return rc;
         if (!gk || !gv || misaligned(gk) || misaligned(gv)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
     }
     if (!cu_q || !cu_k) return sam3_seq_fail(EINVAL_, "attention: null pointer");

@@ -78,6 +78,21 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _strides(t: torch.Tensor) -> Tuple[int, int]:
+    """Strides of [tokens, heads, D] between tokens and between heads; 0 in place of a dimension of one's, which may be anything."""
+    n, heads, _ = t.shape
+    st, sh, _ = t.stride()
+    return st if n > 1 else 0, sh if heads > 1 else 0
+
+
+def _near(t: torch.Tensor, groups: bool) -> torch.Tensor:
+    """:func:`_aligned` for q and the gradient of out: a copy too where rows that share a tile are 2^22 elements apart or more (each head's
+    tokens side by side over very many of them; the copy is small beside the attention of so many)."""
+    t = _aligned(t)
+    st, sh = _strides(t)
+    return t if st < 1 << 22 and (sh < 1 << 22 or not groups) else t.contiguous()
+
+
 def _new(t: torch.Tensor) -> torch.Tensor:
     """An uninitialised contiguous tensor of ``t``'s shape (the cheapest way to one)."""
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
@@ -213,7 +228,7 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
 @lru_cache(maxsize=256)
 def _rotation_table(sections: Tuple[int, ...], theta: float, spectrum: str, d: int):
     """(turns per position step, axis) of each pair as the C arrays that a call reads, and their number."""
-    if not (len(sections) > 0 and all(n >= 0 for n in sections) and 0 < 2 * sum(sections) <= d):
+    if not (0 < len(sections) <= 256 and all(n >= 0 for n in sections) and 0 < 2 * sum(sections) <= d):
         raise ValueError(f"sections {sections} do not fit a head of {d}")
     if spectrum not in ("shared", "per_axis"):
         raise ValueError(f"spectrum must be 'shared' or 'per_axis', got {spectrum!r}")
@@ -239,11 +254,11 @@ def _rotate(q, k, positions, table, halves, inverse):
     turns, axis, pairs = table
     q3 = _tokens(q)
     t, hq, d = q3.shape
-    qs = q3.stride()
+    qs = _strides(q3)
     k3, hk, ks, ko = None, 0, (0, 0), None
     if k is not None:
         k3 = _tokens(k)
-        hk, ks, ko = k3.shape[1], k3.stride(), _new(k)
+        hk, ks, ko = k3.shape[1], _strides(k3), _new(k)
     pos = positions if positions.dim() == 2 else positions.reshape(positions.shape[0], -1)
     qo = _new(q)
     with _on(q.device):
@@ -320,7 +335,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
 def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse, want_stats=False):
     tq, hq, d = q.shape
     tk, hk = k.shape[:2]
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    q, k, v = _near(q, hq > hk), _aligned(k), _aligned(v)
     out = _new(q)
     lse = q.new_empty((tq, hq), dtype=torch.float32) if want_lse else None
     stats = q.new_empty((tq, hq, 2), dtype=torch.float32) if want_stats else None
@@ -329,7 +344,7 @@ def _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, causal, scale, want_lse,
     b = cu_q.shape[0] - 1
     nbytes = lib.sam3_seq_attn_fwd_workspace_bytes(tq, b, hq, hk, d, max_q, max_k, dt)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    qs, ks, vs = _strides(q), _strides(k), _strides(v)
     with _on(q.device):
         _check(lib.sam3_seq_attn_fwd(
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(),
@@ -362,10 +377,10 @@ class _PackedAttention(torch.autograd.Function):
         if go is None:
             return (None,) * 10
         q, k, v, out, stats, cu_q, cu_k = ctx.saved_tensors
-        go = _aligned(go)
+        go = _near(go, q.shape[1] > k.shape[1])
         gq, gk, gv = _new(q), _new(k), _new(v)
-        qt, qh, _, kt, kh, _, vt, vh, _ = ctx.strides
-        gs = go.stride()
+        qt, qh, kt, kh, vt, vh = ctx.strides
+        gs = _strides(go)
         ws = q.new_empty(ctx.nbytes, dtype=torch.uint8)
         with _on(q.device):
             _check(_ffi.load().sam3_seq_attn_bwd(
@@ -388,10 +403,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
                      scale: Optional[float] = None, return_lse: bool = False):
     """Softmax attention over sequences of different lengths that lie one behind the other; returns out [Tq, Hq, D].
 
-    q: [Tq, Hq, D], k, v: [Tk, Hk, D], one type (bf16 or fp32), strided as they come (views of a fused projection or of a cache; rows less
-    than 2^22 elements apart); Hq a multiple of Hk: head h of q reads head ``h // (Hq / Hk)`` of k and v.  D a multiple of 8, at most 128.
+    q: [Tq, Hq, D], k, v: [Tk, Hk, D], one type (bf16 or fp32), strided as they come (views of a fused projection, or of a cache with
+    its heads inside or outside; tokens of k and v less than 2^22 elements apart); Hq a multiple of Hk: head h of q reads head
+    ``h // (Hq / Hk)`` of k and v.  D a multiple of 8, at most 128.
     cu_q, cu_k: int32 [B + 1] on the GPU; sequence b is rows ``cu_q[b]:cu_q[b + 1]`` of q and ``cu_k[b]:cu_k[b + 1]`` of k and v
-    (cu_k None: the same rows).  Sequences may be empty.  Rows in front of the first and behind the last sequence give zeros.
+    (cu_k None: the same rows).  They do not decrease; sequences may be empty.  Rows in front of the first and behind the last sequence
+    give zeros.
     causal: the last query of a sequence sees all its keys, the one before it all but the last, and so on; False: all see all.  A query
     that sees no key gives zeros.  One new token per request over its cache is ``cu_q = arange(B + 1)``.
     len_k: int32 [B], for caches with room behind each request: only the first ``len_k[b]`` of the rows from ``cu_k[b]`` count (without

@@ -81,6 +81,24 @@ def test_header_exports_and_error_text():
     assert lib.sam3_seq_attn_bwd(*([p, 64, 64] * 4), p, p, p, p, p, p, p, 8, 8, 1, 4, 2, 64, 8, 8, 1, 0.1, 0, None, 0, None) == -12
 
 
+def test_strides_that_the_attention_kernels_cannot_follow_are_refused():
+    import ctypes
+    lib, p, far = _ffi.load(), ctypes.c_void_p(64), 1 << 22
+
+    def call(qs=(64, 64), ks=(64, 64), vs=(64, 64), gs=(64, 64), hk=2, back=True):
+        if back:
+            return lib.sam3_seq_attn_bwd(p, *qs, p, *ks, p, *vs, p, *gs, p, p, p, p, p, p, p, 8, 8, 1, 4, hk, 64, 8, 8, 1, 0.1, 0, p, 1 << 20, None)
+        return lib.sam3_seq_attn_fwd(p, *qs, p, *ks, p, *vs, p, p, None, p, None, None, 8, 8, 1, 4, hk, 64, 8, 8, 1, 0.1, 0, None, 0, None)
+    for back in (False, True):
+        for bad in (dict(qs=(far, 64)), dict(qs=(64, far)), dict(ks=(far, 64)), dict(vs=(far, 64)), dict(qs=(far, 64), hk=4)) + ((dict(gs=(far, 64)), dict(gs=(64, far))) if back else ()):
+            assert call(back=back, **bad) == -95 and "2^22" in lib.sam3_seq_last_error().decode(), bad
+        for bad in (dict(qs=(-64, 64)), dict(ks=(64, -64)), dict(vs=(64, 60))):
+            assert call(back=back, **bad) == -22, bad
+    with pytest.raises(ValueError, match="do not fit"):
+        sequence._rotation_table((0,) * 256 + (8,), 10000.0, "shared", 64)
+    assert list(sequence._rotation_table((0,) * 255 + (8,), 10000.0, "shared", 64)[1]) == [255] * 8
+
+
 def test_calls_are_refused_before_they_reach_the_gpu():
     x, w = torch.zeros(4, 64), torch.ones(64)
     with pytest.raises(LoRAKernelError, match="AMD GPU"):
@@ -624,6 +642,52 @@ def test_packed_attention_views_of_a_fused_projection_and_shared_inputs():
     spread = parts[1].detach()[:, :1].expand(150, 2, 64)        # one key head for both groups, as a broadcast view
     assert torch.equal(sequence.packed_attention(parts[0].detach(), spread, spread, cu),
                        sequence.packed_attention(parts[0].detach(), spread.contiguous(), spread.contiguous(), cu))
+
+
+@pytest.mark.gpu
+def test_one_token_of_a_wider_buffer_has_any_stride():
+    """A view of one token is contiguous whatever its stride between tokens, an odd one too."""
+    for dtype in DT:
+        buf = torch.randn(3, 4 * 64 + 5, generator=gen(21)).to("cuda", dtype)
+        row = buf[1, :256].clone().as_strided((1, 4, 64), (261, 64, 1))
+        assert row.is_contiguous() and row.stride(0) == 261
+        plain = row.clone()
+        pos, cu = torch.full((1, 1), 7, device="cuda"), ends([1])
+        for a, b in zip(sequence.rotary_axes(row, row, pos, (32,)), sequence.rotary_axes(plain, plain, pos, (32,))):
+            assert torch.equal(a, b)
+        leaf, want = row.detach().requires_grad_(True), plain.requires_grad_(True)
+        go = buf[2, :256].clone().as_strided((1, 4, 64), (261, 64, 1))
+        out, ref = sequence.packed_attention(leaf, leaf, leaf, cu), sequence.packed_attention(want, want, want, cu)
+        assert torch.equal(out, ref)
+        assert torch.equal(torch.autograd.grad(out, leaf, go)[0], torch.autograd.grad(ref, want, go.clone())[0])
+        assert torch.equal(sequence.rms_norm(row.as_strided((1, 256), (261, 1)), buf[0, :256].clone()), sequence.rms_norm(plain.detach().view(1, 256), buf[0, :256].clone()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("nq", [1, 5, 200])
+def test_packed_attention_heads_of_a_long_buffer_outside(nq, dtype):
+    """[heads, tokens, D] buffers seen as [tokens, heads, D]: heads 2^22 elements and more apart, for the cache, q and out's gradient."""
+    g = gen(22)
+    room, d = (1 << 22) // 64 + 8, 64
+    lk = [300, 70]
+    cu_q, cu_k = ends([nq, 3]), ends(lk)
+
+    def outside(n, heads):
+        return torch.zeros(heads, room, d, device="cuda", dtype=dtype).transpose(0, 1)[:n].copy_(rand(g, n, heads, d, dtype=dtype))
+    q, k, v, go = outside(nq + 3, 4), outside(sum(lk), 2), outside(sum(lk), 2), outside(nq + 3, 4)
+    assert min(t.stride(1) for t in (q, k, v, go)) > 1 << 22
+    far = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    near = [t.detach().contiguous().requires_grad_(True) for t in (q, k, v)]
+    out, ref = sequence.packed_attention(*far, cu_q, cu_k), sequence.packed_attention(*near, cu_q, cu_k)
+    assert torch.equal(out, ref)
+    for a, b in zip(torch.autograd.grad(out, far, go), torch.autograd.grad(ref, near, go.contiguous())):
+        assert torch.equal(a, b)
+    alone = [t[:, :2] for t in (q, k, v)]           # one query head to each key head: q is read where it lies
+    assert torch.equal(sequence.packed_attention(*alone, cu_q, cu_k), sequence.packed_attention(*(t.contiguous() for t in alone), cu_q, cu_k))
+    with torch.no_grad(), pytest.raises(LoRAKernelError, match="2\\^22"):
+        apart = torch.zeros((1 << 22) + 2 * d, device="cuda", dtype=dtype).as_strided((2, 2, d), (1 << 22, d, 1))
+        sequence.packed_attention(q, apart, apart, cu_q, ends([1, 1]))
 
 
 @pytest.mark.gpu
