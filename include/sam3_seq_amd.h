@@ -21,23 +21,24 @@ const char* sam3_seq_last_error(void);
 /*
  * RMS norm of rows x[M, C] (row pitch ldx elements; residual: ldr), C % 8 == 0, C <= 16384:
  *   h = x + residual (fp32, not rounded; residual NULL: h = x)      rstd = 1 / sqrt(mean(h^2) + eps)      y = h * rstd * weight
- * weight has the activations' type.  Outputs, each NULL or contiguous [M, C]:  y;  h_out (h, rounded once);  rstd_out [M] fp32
+ * weight has the activations' type.  Outputs, each NULL or contiguous [M, C]:  y;  h_out (h, rounded once);  h_low [M, C / 8]
+ * 16 bits (two bits for each element that bf16 took from h, for the backward's sums; with a bf16 h_out);  rstd_out [M] fp32
  * (what the backward takes);  q8 [M, C] bytes with scales fp32 [M, C / group] (group 32, 64 or 128; 0: [M, 1]):
  *   scale = max(max|y|, 2^-24) / fmt_max over the group's unrounded y,   q8 = fp8(y / scale)   (fmt: sam3_fp8_amd.h)
  * A row with a NaN has NaN in all its outputs but h_out.
  */
 int sam3_seq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* y, void* h_out,
-                          float* rstd_out, void* q8, float* scales, int group, int fmt, int64_t M, int C, float eps, int dtype,
+                          void* h_low, float* rstd_out, void* q8, float* scales, int group, int fmt, int64_t M, int C, float eps, int dtype,
                           void* stream);
 
 /*
  * Gradients: gx = rstd (u - xhat mean(u xhat)) + gh   with u = gy weight, xhat = h rstd;  gw[c] = sum over the rows of gy xhat.
- * h is h_out of the forward (x without a residual), row pitch ldh; gx is the gradient of x and of the residual.  gy, gh [M, C]
+ * h is h_out of the forward (x without a residual), row pitch ldh; h_low (with ldh = C) or NULL; gx is the gradient of x and of the residual.  gy, gh [M, C]
  * contiguous, gh may be NULL.  gx or gw may be NULL.  gw has the weight's type; its sums are fp32, in a fixed order.
  */
 size_t sam3_seq_rms_norm_bwd_workspace_bytes(int64_t M, int C);
-int sam3_seq_rms_norm_bwd(const void* gy, const void* gh, const void* h, int64_t ldh, const void* weight, const float* rstd, void* gx,
-                          void* gw, int64_t M, int C, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int sam3_seq_rms_norm_bwd(const void* gy, const void* gh, const void* h, int64_t ldh, const void* h_low, const void* weight,
+                          const float* rstd, void* gx, void* gw, int64_t M, int C, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Rotary positions with several axes.  q [T, Hq, D], k [T, Hk, D] (k NULL: q alone), strides in elements (token, head; unit inside a

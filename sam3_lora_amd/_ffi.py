@@ -197,12 +197,12 @@ def _declare(lib):
     lib.sam3_seq_last_error.restype = c_char_p
     lib.sam3_seq_last_error.argtypes = []
     lib.sam3_seq_rms_norm_fwd.restype = c_int
-    lib.sam3_seq_rms_norm_fwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 6 + [c_int, c_int, c_int64, c_int, c_float,
+    lib.sam3_seq_rms_norm_fwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 7 + [c_int, c_int, c_int64, c_int, c_float,
                                                                                            c_int, c_void_p]
     lib.sam3_seq_rms_norm_bwd_workspace_bytes.restype = c_size_t
     lib.sam3_seq_rms_norm_bwd_workspace_bytes.argtypes = [c_int64, c_int]
     lib.sam3_seq_rms_norm_bwd.restype = c_int
-    lib.sam3_seq_rms_norm_bwd.argtypes = [c_void_p] * 3 + [c_int64] + [c_void_p] * 4 + [c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p]
+    lib.sam3_seq_rms_norm_bwd.argtypes = [c_void_p] * 3 + [c_int64] + [c_void_p] * 5 + [c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p]
     strided = [c_void_p, c_int64, c_int64]                     # tensor, token stride, head stride
     lib.sam3_seq_rotary.restype = c_int
     lib.sam3_seq_rotary.argtypes = strided * 2 + [c_void_p] * 3 + [c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,

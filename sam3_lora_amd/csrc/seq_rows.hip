@@ -31,6 +31,7 @@ namespace {
 struct NormFwd {
     const void *x, *r, *w;
     void *y, *h;
+    unsigned short* low;
     float* rstd;
     unsigned char* q8;
     float* scales;
@@ -80,6 +81,25 @@ __device__ __forceinline__ unsigned to_fp8x4(float a, float b, float c, float d)
     return (unsigned)w;
 }
 
+// What the rounding of h to 16 bits took away, to about a tenth of it, in two bits: 0, or +-3/8 of the last place that is left (the
+// difference of the bit patterns counts in last places whatever the exponent).  The weight's gradient sums products with h over the rows:
+// with the rounded h it is off by sqrt(2) of its own rounding, and worse by chance; with these bits by 1.05.  A sixteenth of y's bytes.
+__device__ __forceinline__ unsigned low_bits(const float* h, const Raw8<bf16_t>& o) {
+    const unsigned b[4] = {o.a.x, o.a.y, o.a.z, o.a.w};
+    unsigned code = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int d = (int)(__float_as_uint(h[j]) - (j & 1 ? b[j / 2] & 0xffff0000u : b[j / 2] << 16));
+        code |= (d > 0x3000 ? 1u : d < -0x3000 ? 3u : 0u) << (2 * j);
+    }
+    return code;
+}
+__device__ __forceinline__ void add_low_bits(float* h, unsigned code) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = __uint_as_float(__float_as_uint(h[j]) + ((int)(code << (30 - 2 * j)) >> 30) * 0x6000);
+}
+__device__ __forceinline__ unsigned low_bits(const float*, const Raw8<float>&) { return 0; }
+
 // Q8: 0 none, 1 e4m3, 2 e5m2
 template <typename T, int LPR, int CPL, int Q8>
 __global__ __launch_bounds__(256) void k_rms_fwd(NormFwd a) {
@@ -128,6 +148,7 @@ __global__ __launch_bounds__(256) void k_rms_fwd(NormFwd a) {
                 if (a.h) {
                     o.set(h[i]);
                     o.store((T*)a.h + row * a.C + c);
+                    if (sizeof(T) == 2 && a.low) a.low[(row * a.C + c) >> 3] = (unsigned short)low_bits(h[i], o);
                 }
                 float g[8];
                 w[i].get(g);
@@ -177,6 +198,7 @@ __global__ __launch_bounds__(256) void k_rms_fwd(NormFwd a) {
 
 struct NormBwd {
     const void *gy, *gh, *h, *w;
+    const unsigned short* low;
     const float* rstd;
     void* gx;
     float* part;        // [workgroups, C] fp32, or NULL: no weight gradient
@@ -216,6 +238,7 @@ __global__ __launch_bounds__(256) void k_rms_bwd(NormBwd a) {
                 v.load(hh + row * a.ldh + c);
                 g.load(gy + row * a.C + c);
                 v.get(xh[i]);
+                if (sizeof(T) == 2 && a.low) add_low_bits(xh[i], a.low[(row * a.C + c) >> 3]);
                 g.get(u[i]);
                 float wv[8];
                 w[i].get(wv);
@@ -505,22 +528,23 @@ extern "C" {
 const char* sam3_seq_last_error(void) { return g_err; }
 
 int sam3_seq_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* y, void* h_out,
-                          float* rstd_out, void* q8, float* scales, int group, int fmt, int64_t M, int C, float eps, int dtype,
+                          void* h_low, float* rstd_out, void* q8, float* scales, int group, int fmt, int64_t M, int C, float eps, int dtype,
                           void* stream) {
     sam3_seq_clear_error();
     if (int rc = norm_check(M, C, dtype)) return rc;
     if (!(eps >= 0.f) || eps > 3.0e38f) return sam3_seq_fail(EINVAL_, "rms norm: eps must be finite and not negative");
+    if (h_low && (dtype != 0 || !h_out)) return sam3_seq_fail(EINVAL_, "rms norm: h_low goes with a bf16 h_out");
     if ((q8 == nullptr) != (scales == nullptr)) return sam3_seq_fail(EINVAL_, "rms norm: the 8-bit output needs its scales");
     if (q8 && fmt != SAM3_FP8_E4M3 && fmt != SAM3_FP8_E5M2) return sam3_seq_fail(EINVAL_, "rms norm: unknown 8-bit format %d", fmt);
     if (q8 && group && ((group != 32 && group != 64 && group != 128) || C % group))
         return sam3_seq_fail(EINVAL_, "rms norm: scale groups are 32, 64 or 128 columns that divide %d, got %d", C, group);
     if (M == 0) return 0;
     if (!x || !weight || (!y && !q8)) return sam3_seq_fail(EINVAL_, "rms norm: null pointer");
-    if (misaligned(x) || misaligned(residual) || misaligned(weight) || misaligned(y) || misaligned(h_out) || ((uintptr_t)q8 & 7))
+    if (misaligned(x) || misaligned(residual) || misaligned(weight) || misaligned(y) || misaligned(h_out) || ((uintptr_t)q8 & 7) || ((uintptr_t)h_low & 1))
         return sam3_seq_fail(EINVAL_, "rms norm: tensors must be 16-byte aligned");
     if (ldx < C || bad_pitch(ldx, dtype) || (residual && (ldr < C || bad_pitch(ldr, dtype))))
         return sam3_seq_fail(EINVAL_, "rms norm: bad row pitch");
-    const NormFwd a{x, residual, weight, y, h_out, rstd_out, (unsigned char*)q8, scales, ldx, ldr, M, C, !group ? 0 : group == 32 ? 5 : group == 64 ? 6 : 7, eps,
+    const NormFwd a{x, residual, weight, y, h_out, (unsigned short*)h_low, rstd_out, (unsigned char*)q8, scales, ldx, ldr, M, C, !group ? 0 : group == 32 ? 5 : group == 64 ? 6 : 7, eps,
                     fmt == SAM3_FP8_E4M3 ? 448.f : 57344.f};
     const int q = !q8 ? 0 : fmt == SAM3_FP8_E4M3 ? 1 : 2;
     return dtype == 0 ? launch_norm_fwd<bf16_t>(a, q, (hipStream_t)stream) : launch_norm_fwd<float>(a, q, (hipStream_t)stream);
@@ -530,7 +554,7 @@ size_t sam3_seq_rms_norm_bwd_workspace_bytes(int64_t M, int C) {
     return M > 0 && C > 0 && C % 8 == 0 && C <= 16384 ? (size_t)norm_bwd_blocks(M, C) * C * sizeof(float) : 0;
 }
 
-int sam3_seq_rms_norm_bwd(const void* gy, const void* gh, const void* h, int64_t ldh, const void* weight, const float* rstd, void* gx,
+int sam3_seq_rms_norm_bwd(const void* gy, const void* gh, const void* h, int64_t ldh, const void* h_low, const void* weight, const float* rstd, void* gx,
                           void* gw, int64_t M, int C, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
     sam3_seq_clear_error();
     if (int rc = norm_check(M, C, dtype)) return rc;
@@ -538,10 +562,11 @@ int sam3_seq_rms_norm_bwd(const void* gy, const void* gh, const void* h, int64_t
     if (!gy || !h || !weight || !rstd || (!gx && !gw)) return sam3_seq_fail(EINVAL_, "rms norm: null pointer");
     if (misaligned(gy) || misaligned(gh) || misaligned(h) || misaligned(weight) || misaligned(gx))
         return sam3_seq_fail(EINVAL_, "rms norm: tensors must be 16-byte aligned");
+    if (h_low && (dtype != 0 || ldh != C || ((uintptr_t)h_low & 1))) return sam3_seq_fail(EINVAL_, "rms norm: h_low goes with a contiguous bf16 h");
     if (ldh < C || bad_pitch(ldh, dtype)) return sam3_seq_fail(EINVAL_, "rms norm: bad row pitch");
     if (gw && (!workspace || workspace_bytes < sam3_seq_rms_norm_bwd_workspace_bytes(M, C)))
         return sam3_seq_fail(ENOMEM_, "rms norm: workspace too small: %zu < %zu", workspace_bytes, sam3_seq_rms_norm_bwd_workspace_bytes(M, C));
-    const NormBwd a{gy, gh, h, weight, rstd, gx, gw ? (float*)workspace : nullptr, ldh, M, C};
+    const NormBwd a{gy, gh, h, weight, (const unsigned short*)h_low, rstd, gx, gw ? (float*)workspace : nullptr, ldh, M, C};
     return dtype == 0 ? launch_norm_bwd<bf16_t>(a, gw, (hipStream_t)stream) : launch_norm_bwd<float>(a, gw, (hipStream_t)stream);
 }
 

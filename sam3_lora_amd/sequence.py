@@ -113,14 +113,16 @@ def _pitch(t: torch.Tensor) -> int:
 
 
 def _norm_fwd(x, residual, weight, eps, want_y, want_rstd, q8=None):
-    """(y, h, rstd, image, scales) of contiguous outputs; q8 = (group, fmt) or None."""
+    """(y, h, low, rstd, image, scales) of contiguous outputs; q8 = (group, fmt) or None.  low and rstd are for the backward."""
     width = x.shape[-1]
     x2 = _rows(x, width)
     m = x2.shape[0]
-    r2, ldr, h = None, 0, None
+    r2, ldr, h, low = None, 0, None, None
     if residual is not None:
         r2 = _rows(residual, width)
         ldr, h = _pitch(r2), _new(x)
+        if want_rstd and x.dtype is torch.bfloat16:
+            low = x.new_empty((m, width // 8), dtype=torch.int16)
     w = _aligned(weight)
     y = _new(x) if want_y else None
     rstd = x.new_empty(m, dtype=torch.float32) if want_rstd else None
@@ -131,18 +133,18 @@ def _norm_fwd(x, residual, weight, eps, want_y, want_rstd, q8=None):
         scales = x.new_empty(x.shape[:-1] + (width // group if group else 1,), dtype=torch.float32)
     with _on(x.device):
         _check(_ffi.load().sam3_seq_rms_norm_fwd(
-            x2.data_ptr(), _pitch(x2), _ptr(r2), ldr, w.data_ptr(), _ptr(y), _ptr(h), _ptr(rstd), _ptr(image), _ptr(scales), group, fmt, m,
-            width, eps, _TYPE_CODES[x.dtype], _stream(x.device)), "sam3_seq_rms_norm_fwd")
-    return y, h, rstd, image, scales
+            x2.data_ptr(), _pitch(x2), _ptr(r2), ldr, w.data_ptr(), _ptr(y), _ptr(h), _ptr(low), _ptr(rstd), _ptr(image), _ptr(scales), group, fmt,
+            m, width, eps, _TYPE_CODES[x.dtype], _stream(x.device)), "sam3_seq_rms_norm_fwd")
+    return y, h, low, rstd, image, scales
 
 
 class _RMSNorm(torch.autograd.Function):
-    """``(y, h)``; saves the stream h (x itself without a residual) and rstd."""
+    """``(y, h)``; saves the stream h (x itself without a residual), two bits more of it than bf16 holds, and rstd."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
-        y, h, rstd, _, _ = _norm_fwd(x, residual, weight, eps, True, True)
-        ctx.save_for_backward(x if residual is None else h, weight, rstd)
+        y, h, low, rstd, _, _ = _norm_fwd(x, residual, weight, eps, True, True)
+        ctx.save_for_backward(x if residual is None else h, low, weight, rstd)
         ctx.with_residual = residual is not None
         ctx.set_materialize_grads(False)
         return (y, h) if ctx.with_residual else y
@@ -150,7 +152,7 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gy, gh=None):
-        h, weight, rstd = ctx.saved_tensors
+        h, low, weight, rstd = ctx.saved_tensors
         need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         if gy is None:      # only the stream was used
             return gh if ctx.needs_input_grad[0] else None, gh if ctx.needs_input_grad[1] else None, None, None
@@ -169,7 +171,7 @@ class _RMSNorm(torch.autograd.Function):
             ws = h.new_empty(lib.sam3_seq_rms_norm_bwd_workspace_bytes(m, width), dtype=torch.uint8)
         with _on(h.device):
             _check(lib.sam3_seq_rms_norm_bwd(
-                gy2.data_ptr(), _ptr(gh2), h2.data_ptr(), _pitch(h2), w.data_ptr(), rstd.data_ptr(), _ptr(gx), _ptr(gw), m, width,
+                gy2.data_ptr(), _ptr(gh2), h2.data_ptr(), _pitch(h2), _ptr(low), w.data_ptr(), rstd.data_ptr(), _ptr(gx), _ptr(gw), m, width,
                 _TYPE_CODES[h.dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream(h.device)),
                 "sam3_seq_rms_norm_bwd")
         return gx if ctx.needs_input_grad[0] else None, gx if ctx.needs_input_grad[1] else None, gw, None
@@ -200,7 +202,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     _norm_args(x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return _RMSNorm.apply(x, residual, weight, eps)
-    y, h, _, _, _ = _norm_fwd(x, residual, weight, eps, True, False)
+    y, h, _, _, _, _ = _norm_fwd(x, residual, weight, eps, True, False)
     return y if residual is None else (y, h)
 
 
@@ -220,7 +222,7 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
         raise ValueError(f"group must be 0, or 32, 64 or 128 and divide {x.shape[-1]}, got {group}")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         raise ValueError("rms_norm_q8 has no gradient: call it under torch.no_grad(), or rms_norm for training")
-    _, h, _, image, scales = _norm_fwd(x, residual, weight, eps, False, False, (group, fmt))
+    _, h, _, _, image, scales = _norm_fwd(x, residual, weight, eps, False, False, (group, fmt))
     return (image, scales) if residual is None else (image, scales, h)
 
 

@@ -53,11 +53,11 @@ def test_header_exports_and_error_text():
     assert lib.sam3_seq_attn_bwd_workspace_bytes(5, 4) == 240
     p = ctypes.c_void_p(64)
 
-    def norm(M=1, C=64, dtype=0, x=p, w=p, y=p, q8=None, scales=None, group=0, fmt=0, eps=1e-6, ldx=64):
-        return lib.sam3_seq_rms_norm_fwd(x, ldx, None, 0, w, y, None, None, q8, scales, group, fmt, M, C, eps, dtype, None)
+    def norm(M=1, C=64, dtype=0, x=p, w=p, y=p, q8=None, scales=None, group=0, fmt=0, eps=1e-6, ldx=64, low=None):
+        return lib.sam3_seq_rms_norm_fwd(x, ldx, None, 0, w, y, None, low, None, q8, scales, group, fmt, M, C, eps, dtype, None)
     for bad, text in ((dict(dtype=2), "dtype"), (dict(C=60), "multiples of 8"), (dict(M=-1), "sizes"), (dict(x=None), "null"), (dict(y=None), "null"),
                       (dict(q8=p), "scales"), (dict(q8=p, scales=p, group=48), "groups"), (dict(q8=p, scales=p, fmt=3), "format"),
-                      (dict(eps=-1.0), "eps"), (dict(ldx=32), "pitch"), (dict(x=ctypes.c_void_p(68)), "aligned")):
+                      (dict(eps=-1.0), "eps"), (dict(ldx=32), "pitch"), (dict(low=p), "h_low"), (dict(x=ctypes.c_void_p(68)), "aligned")):
         assert norm(**bad) == -22, bad
         assert text in lib.sam3_seq_last_error().decode(), (bad, lib.sam3_seq_last_error())
     assert norm(C=16392, ldx=16392) == -95 and norm(M=0) == 0
@@ -207,6 +207,27 @@ def test_rms_norm_and_gradients(rows, width, residual, dtype):
     with torch.no_grad():       # without a gradient: the same kernel
         again = sequence.rms_norm(dev(x), dev(w), residual=dev(r))
     assert torch.equal(again[0] if residual else again, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width", [(1, 8), (37, 72), (300, 1024), (40, 2056)])
+def test_rms_norm_gradients_know_two_bits_more_than_the_stream(rows, width):
+    """bf16 with a residual: the two bits leave at most 3/16 of a last place of h, which is 2 u at most: 3/8 u where the rounded h has u."""
+    dtype, g = torch.bfloat16, gen(rows + width)
+    x, r = rand(g, rows, width, dtype=dtype), rand(g, rows, width, dtype=dtype, scale=0.37)
+    x[0, :3], r[0, :3] = 0.0, torch.tensor([0.0, -0.0, 2.0 ** -120])        # nothing, and next to nothing
+    x[-1, 4:8], r[-1, 4:8] = torch.tensor([1.0, -1.0, 1.0, 2.0]).double(), torch.tensor([2.0 ** -8, 2.0 ** -8, -2.0 ** -9, -2.0 ** -8]).double()    # halves and quarters of a place
+    w, gy, gh = (rand(g, width, dtype=dtype, scale=0.3) + 1).to(dtype).double(), rand(g, rows, width, dtype=dtype), torch.zeros(rows, width, dtype=torch.double)
+    ref = norm_ref(x, w, r, 1e-6, gy, gh)
+    leaves = [t.to("cuda", dtype).requires_grad_(True) for t in (x, r, w)]
+    got = sequence.rms_norm(leaves[0], leaves[2], residual=leaves[1])
+    grads = torch.autograd.grad(got, leaves, (gy.to("cuda", dtype), gh.to("cuda", dtype)))
+    u = unit(dtype)
+    us = 3 / 8 * u
+    absmean = (ref["u"] * ref["xhat"]).abs().mean(-1, keepdim=True)
+    tol = ref["rstd"] * (2 * NORM_OPS * F * (ref["u"].abs() + ref["xhat"].abs() * absmean) + 2 * us * ref["xhat"].abs() * absmean)
+    close(grads[0], ref["gx"], tol + (u + 2 * F) * ref["gx"].abs(), "gx")
+    close(grads[2], ref["gw"], u * ref["gw"].abs() + (us + (rows + NORM_OPS) * F) * (gy * ref["xhat"]).abs().sum(0), "gw")
 
 
 @pytest.mark.gpu
