@@ -96,6 +96,16 @@ __device__ __forceinline__ void frag_of(Frag<float>& f, const float* p) {
     for (int j = 0; j < 8; ++j) f.v[j] = p[j];
 }
 
+// What that rounding to 16 bits took away, as one more operand.  Weights and dS rounded once cost a result sqrt(2) of its own rounding, and more
+// by chance where a few of them decide it; the products with the rest are taken where a call is small or waits for memory anyway (FINE).
+__device__ __forceinline__ void rest_of(Frag<bf16_t>& f, const Frag<bf16_t>& hi, const float* p) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = p[j] - (float)hi.v[j];
+    frag_of(f, r);
+}
+__device__ __forceinline__ void rest_of(Frag<float>&, const Frag<float>&, const float*) {}
+
 // A tile of rows in LDS: rows of DP elements in chunks of 16 bytes, the chunks of a row permuted by an exclusive or with f(row).  LDS has
 // 64 banks of 4 bytes, a line of 16 chunks.  Reading rows, 16 lanes read the same chunk of 16 neighbouring rows: f takes them to 16
 // different places of a line.  Reading columns, lanes read the same four chunks of 4 neighbouring rows: f's upper bits come from the
@@ -356,7 +366,7 @@ struct FwdState {
     f32x16 acc[DT];
     float base, l;      // exponent base in powers of two, this half-wave's part of the sum
 
-    template <bool MASK>
+    template <bool MASK, bool FINE = false>
     __device__ __forceinline__ void step(const char* lk, const char* lv, int lane, float c2, int left) {
         const int h = lane >> 5;
         f32x16 s[SUBS];
@@ -394,10 +404,15 @@ struct FwdState {
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                Frag<T> pf;
+                Frag<T> pf, pr;
                 frag_of(pf, p + 8 * t);
+                if (FINE) rest_of(pr, pf, p + 8 * t);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lv, sub * 32 + 16 * t, d, lane), pf, acc[d]);
+                for (int d = 0; d < DT; ++d) {
+                    const Frag<T> vf = L::col_frag(lv, sub * 32 + 16 * t, d, lane);
+                    acc[d] = mma(vf, pf, acc[d]);
+                    if (FINE && sizeof(T) == 2) acc[d] = mma(vf, pr, acc[d]);
+                }
             }
         }
     }
@@ -510,7 +525,7 @@ struct Few {
     unsigned first_rest;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_attn_few(Attn a, Few f) {
     typedef Tile<T, DP> L;
     constexpr int KS = DP / 16, DT = DP / 32, TB = FewCfg<T, DP>::TB;
@@ -579,7 +594,7 @@ __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_a
                 } else {
                     wait_loads<0>();
                 }
-                st.template step<false>(now, now + TB, lane, c2, 32);
+                st.template step<false, FINE>(now, now + TB, lane, c2, 32);
             }
             for (int i = full; begin + i * 32 < end; ++i) {
                 const int k0 = begin + i * 32;
@@ -587,7 +602,7 @@ __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_a
                 stage<T, DP, 32, false, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
                 const bool bad = __any(stage<T, DP, 32, true, 64>(mine + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; }));
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                st.template step<true>(mine, mine + TB, lane, c2, min(jmax, end) - k0);
+                st.template step<true, FINE>(mine, mine + TB, lane, c2, min(jmax, end) - k0);
                 if (bad) add_nonfinite<T, DT>(st.acc, v + (long long)k0 * a.v_st, a.v_st, min(min(jmax, end) - k0, 32), a.D, h);
             }
         }
@@ -683,7 +698,7 @@ struct GqState {
     f32x16 acc[DT];
     float base, delta, sum;
 
-    template <bool MASK, bool SUM = false>
+    template <bool MASK, bool SUM = false, bool FINE = false>
     __device__ __forceinline__ void step(const char* lk, const char* lv, int lane, float c2, int left) {
         const int h = lane >> 5;
 #pragma unroll
@@ -707,10 +722,15 @@ struct GqState {
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                Frag<T> f;
+                Frag<T> f, r;
                 frag_of(f, ds + 8 * t);
+                if (FINE) rest_of(r, f, ds + 8 * t);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) acc[d] = mma(L::col_frag(lk, sub * 32 + 16 * t, d, lane), f, acc[d]);
+                for (int d = 0; d < DT; ++d) {
+                    const Frag<T> kf = L::col_frag(lk, sub * 32 + 16 * t, d, lane);
+                    acc[d] = mma(kf, f, acc[d]);
+                    if (FINE && sizeof(T) == 2) acc[d] = mma(kf, r, acc[d]);
+                }
             }
         }
     }
@@ -945,7 +965,7 @@ struct GkvState {
         for (int i = 0; i < DT; ++i) ak[i] = zero16(), av[i] = zero16();
         spoilt = false;
     }
-    template <bool MASK>
+    template <bool MASK, bool FINE = false>
     __device__ __forceinline__ void step(const char* lq, const char* lg, const char* lvw, const float* st, int pitch, int lane, float c2, int r0, int from, int end) {
         const int h = lane >> 5;
         f32x16 s = zero16(), dp = zero16();
@@ -957,7 +977,7 @@ struct GkvState {
             // (left alone, the compiler reads every operand ahead and spills; a reload in the loop waits for the tiles' loads)
             if (V_LDS && i % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
-        Frag<T> pf[2], df[2];
+        Frag<T> pf[2], df[2], pr[2], dr[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             float ba[8], de[8], in[8], p[8], ds[8];
@@ -978,13 +998,16 @@ struct GkvState {
             }
             frag_of(pf[t], p);
             frag_of(df[t], ds);
+            if (FINE) rest_of(pr[t], pf[t], p), rest_of(dr[t], df[t], ds);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                av[d] = mma(L::col_frag(lg, 16 * t, d, lane), pf[t], av[d]);
-                ak[d] = mma(L::col_frag(lq, 16 * t, d, lane), df[t], ak[d]);
+                const Frag<T> gf = L::col_frag(lg, 16 * t, d, lane), qf = L::col_frag(lq, 16 * t, d, lane);
+                av[d] = mma(gf, pf[t], av[d]);
+                ak[d] = mma(qf, df[t], ak[d]);
+                if (FINE && sizeof(T) == 2) av[d] = mma(gf, pr[t], av[d]), ak[d] = mma(qf, dr[t], ak[d]);
             }
     }
 };
@@ -1261,11 +1284,11 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             } else {
                 wait_loads<0>();
             }
-            st.template step<false>(now, now + TB, lane, c2, 32);
+            st.template step<false, false, NW == 1>(now, now + TB, lane, c2, 32);
         }
         for (; blk * 32 < jend; blk += NW) {
             const bool bad = bring(blk * 32);
-            st.template step<true>(mine, mine + TB, lane, c2, jmax - blk * 32);
+            st.template step<true, false, NW == 1>(mine, mine + TB, lane, c2, jmax - blk * 32);
             if (bad)
                 for (int j = 0; j < min(jmax - blk * 32, 32); ++j) spoilt |= spoils(k + (blk * 32 + j) * a.k_st, a.D);
         }
@@ -1341,7 +1364,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             bool bad = stage<T, DP, 32, true, 64>(mine, (const T*)a.q, R - r0, a.D, [&](int r) { return qrows.at(r0 + r); });
             bad |= stage<T, DP, 32, true, 64>(mine + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            st.template step<true>(mine, mine + TB, nullptr, &stat[wave][0][0][0], 32, lane, c2, r0, r_key, R);
+            st.template step<true, NW == 1>(mine, mine + TB, nullptr, &stat[wave][0][0][0], 32, lane, c2, r0, r_key, R);
             if (__any(bad))
                 for (int r = max(r0, r_key); r < min(r0 + 32, R); ++r)
                     st.spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
@@ -1370,7 +1393,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
                     wait_loads<0>();
                 }
                 char* now = mine + buf * 2 * TB;
-                st.template step<false>(now, now + TB, nullptr, &stat[wave][buf][0][0], 32, lane, c2, first + s * 32, r_key, R);
+                st.template step<false, NW == 1>(now, now + TB, nullptr, &stat[wave][buf][0][0], 32, lane, c2, first + s * 32, r_key, R);
             }
         }
         for (; s < steps; s += NW) border(s);
@@ -1500,7 +1523,11 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
         f.pstat = reinterpret_cast<float2*>(f.part + (p.splits > 1 ? (size_t)p.splits * Tq * Hq * D : 0));
         const dim3 grid(f.first_rest + REST);
         hipStream_t st = (hipStream_t)stream;
-#define FEW(TY, W) hipLaunchKernelGGL((k_attn_few<TY, W>), grid, dim3(64), 0, st, a, f)
+#define FEW(TY, W)                                                                                                    \
+    do {                                                                                                              \
+        if (sizeof(TY) == 2 && p.tiles == 1) hipLaunchKernelGGL((k_attn_few<TY, W, sizeof(TY) == 2>), grid, dim3(64), 0, st, a, f); \
+        else hipLaunchKernelGGL((k_attn_few<TY, W, false>), grid, dim3(64), 0, st, a, f);                             \
+    } while (0)
         if (dtype == 0) { if (D <= 32) FEW(bf16_t, 32); else if (D <= 64) FEW(bf16_t, 64); else FEW(bf16_t, 128); }
         else { if (D <= 32) FEW(float, 32); else if (D <= 64) FEW(float, 64); else FEW(float, 128); }
 #undef FEW
