@@ -96,8 +96,12 @@ __device__ __forceinline__ void frag_of(Frag<float>& f, const float* p) {
     for (int j = 0; j < 8; ++j) f.v[j] = p[j];
 }
 
-// What that rounding to 16 bits took away, as one more operand.  Weights and dS rounded once cost a result sqrt(2) of its own rounding, and more
-// by chance where a few of them decide it; the products with the rest are taken where a call is small or waits for memory anyway (FINE).
+// What that rounding to 16 bits took away, as one more operand.  Weights and dS rounded once leave a result sqrt(2) of its own rounding's error,
+// more where a few of them decide it, and in gq, whose keys are weighted most where they lie along q, up to 1.57 for heads of 32 (4 x 2000
+// to 32 x 500 tokens; 1.5 for 64, 1.47 for 128).  The products with the rest are taken (FINE; the error is 1.0 to 1.1 then) where they are
+// cheap or needed most: one tile of rows in the forward (decode of 24 requests 417 -> 423 us; with more tiles, 64 new tokens over 32768 keys,
+// 134 -> 148), gq in tiles of 32 (120 -> 128 at 4 x 128 tokens over 4096 keys) and for heads up to 32 (4 x 4096 tokens 177 -> 224; for heads
+// of 64 it would be 715 -> 906), gk and gv of one wave (text prompts 12.4 -> 12.5; with four waves it would be 480 -> 600 at 4096 tokens).
 __device__ __forceinline__ void rest_of(Frag<bf16_t>& f, const Frag<bf16_t>& hi, const float* p) {
     float r[8];
 #pragma unroll
@@ -688,6 +692,7 @@ constexpr int EXACT_D = 128;
 template <typename T, int DP>
 struct GqCfg {
     static constexpr int BN = sizeof(T) * DP > 256 ? 32 : 64;
+    static constexpr bool FINE = DP <= 32;      // (rest_of())
 };
 
 template <typename T, int DP, int BN>
@@ -838,7 +843,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq
                     dk.load(k + (long long)(t + 1) * BN * a.k_st, a.k_st, next);
                     dv.load(v + (long long)(t + 1) * BN * a.v_st, a.v_st, next + TB);
                 }
-                st.template step<false>(now, now + TB, lane, c2, BN);
+                st.template step<false, false, GqCfg<T, DP>::FINE>(now, now + TB, lane, c2, BN);
             }
         }
         for (int k0 = nfull * BN; k0 < jend; k0 += BN) {
@@ -846,7 +851,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq
             bool bad = stage<T, DP, BN, true>(lds, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
             stage<T, DP, BN, false>(lds + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
             bad = __syncthreads_or(bad);
-            if (k0 < jwave) st.template step<true>(lds, lds + TB, lane, c2, jmax - k0);
+            if (k0 < jwave) st.template step<true, false, GqCfg<T, DP>::FINE>(lds, lds + TB, lane, c2, jmax - k0);
             if (bad)
                 for (int j = 0; j < min(jmax - k0, BN); ++j) spoilt |= spoils(k + (k0 + j) * a.k_st, a.D);
         }
@@ -1284,11 +1289,11 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             } else {
                 wait_loads<0>();
             }
-            st.template step<false, false, NW == 1>(now, now + TB, lane, c2, 32);
+            st.template step<false, false, true>(now, now + TB, lane, c2, 32);
         }
         for (; blk * 32 < jend; blk += NW) {
             const bool bad = bring(blk * 32);
-            st.template step<true, false, NW == 1>(mine, mine + TB, lane, c2, jmax - blk * 32);
+            st.template step<true, false, true>(mine, mine + TB, lane, c2, jmax - blk * 32);
             if (bad)
                 for (int j = 0; j < min(jmax - blk * 32, 32); ++j) spoilt |= spoils(k + (blk * 32 + j) * a.k_st, a.D);
         }

@@ -418,7 +418,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     scale: of the scores, 1 / sqrt(D) if None.  return_lse: also the logarithm of each row's sum, fp32 [Tq, Hq], without a gradient.
 
     Keys and values that a query does not see do not enter its result, whatever they hold.  Sums and statistics are fp32; for bf16 the
-    probabilities are rounded to bf16 for the product with v.  Gradients come out the same in every run.
+    probabilities are rounded to bf16 for the product with v, but for calls of few rows, where they keep 16 bits.  Gradients come out the
+    same in every run.
     """
     _activation("q", q)
     _activation("k", k, q)

@@ -400,8 +400,9 @@ def test_rotary_axes_edges():
 
 
 # ---------------------------------------------------------------------------------------------------------- attention
-def attn_ref(q, k, v, lq, lk, causal, scale, u, go=None, len_k=None):
-    """Results and error bounds in 64 bits: the bounds follow the roundings named at each line."""
+def attn_ref(q, k, v, lq, lk, causal, scale, u, go=None, len_k=None, uw=None):
+    """Results and error bounds in 64 bits: the bounds follow the roundings named at each line.  uw: of a weight, or of dS (u)."""
+    uw = u if uw is None else uw
     hq, hk, d = q.shape[1], k.shape[1], q.shape[2]
     r = {n: torch.zeros_like(t) for n, t in (("o", q), ("to", q), ("gq", q), ("tgq", q), ("gk", k), ("tgk", k), ("gv", v), ("tgv", v))}
     r["lse"] = torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
@@ -421,7 +422,7 @@ def attn_ref(q, k, v, lq, lk, causal, scale, u, go=None, len_k=None):
             es = ((d + 6) * F * (Q.abs() @ K.abs().T) * scale + 6 * F * s.abs().masked_fill(~seen, 0.0) + 4 * F).masked_fill(~seen, 0.0)
             worst = es.amax(1, keepdim=True) if nn else es.new_zeros(m, 1)
             ep = es + worst + (nn + 16) * F            # relative, of a weight; the sum of nn terms and its rescalings
-            to = ((ep + u) * p) @ V.abs() + (nn + 16) * F * (p @ V.abs()) + u * o.abs()      # u: the weight's rounding, the result's
+            to = ((ep + uw) * p) @ V.abs() + (nn + 16) * F * (p @ V.abs()) + u * o.abs()      # the weight's rounding, the result's
             r["o"][a:a + m, h], r["to"][a:a + m, h] = o, to
             if nn:
                 r["lse"][a:a + m, h] = torch.logsumexp(s, 1)
@@ -435,14 +436,14 @@ def attn_ref(q, k, v, lq, lk, causal, scale, u, go=None, len_k=None):
                 # the forward's rounded result in delta, its sum of d products, and those of dp
                 ed = (G.abs() * to).sum(1, keepdim=True) + (d + 2) * F * (G.abs() * o.abs()).sum(1, keepdim=True)
                 ep2 = 2 * ep + 4 * F                   # weights recomputed from the stored fp32 lse
-                eds = p * ((d + 2) * F * (G.abs() @ V.abs().T) + ed) + (ep2 + 4 * F) * ds.abs() + u * ds.abs()
+                eds = p * ((d + 2) * F * (G.abs() @ V.abs().T) + ed) + (ep2 + 4 * F) * ds.abs() + uw * ds.abs()
                 r["gq"][a:a + m, h] = ds @ K * scale
                 r["tgq"][a:a + m, h] = (eds @ K.abs() + (nn + 2) * F * (ds.abs() @ K.abs())) * scale + (u + 2 * F) * r["gq"][a:a + m, h].abs()
                 rows = m * (hq // hk)
                 r["gk"][b:b + nn, kh] += ds.T @ Q * scale
                 r["tgk"][b:b + nn, kh] += (eds.T @ Q.abs() + (rows + 2) * F * (ds.abs().T @ Q.abs())) * scale
                 r["gv"][b:b + nn, kh] += p.T @ G
-                r["tgv"][b:b + nn, kh] += ((ep2 + u) * p).T @ G.abs() + (rows + 2) * F * (p.T @ G.abs())
+                r["tgv"][b:b + nn, kh] += ((ep2 + uw) * p).T @ G.abs() + (rows + 2) * F * (p.T @ G.abs())
         a, b = a + m, b + n
     r["tgk"] += (u + 2 * F) * r["gk"].abs()
     r["tgv"] += (u + 2 * F) * r["gv"].abs()
@@ -539,6 +540,23 @@ def test_packed_attention_hints_and_scale(dtype):
 def test_packed_attention_few_rows_over_many_keys(lq, lk, hq, hk, d, causal, dtype):
     check_attention(lq, lk, hq, hk, d, causal, dtype, seed=d)
     check_attention(lq, lk, hq, hk, d, causal, dtype, seed=d + 1, train=False, hints=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,hq,hk,d", [([1, 1, 1], [300, 1, 2000], 8, 2, 64), ([20, 3, 31], [20, 3, 31], 4, 4, 64), ([2, 7], [60, 9], 4, 2, 128),
+                                           ([30], [30], 1, 1, 32), ([1], [5000], 1, 1, 128)])
+def test_packed_attention_of_few_rows_keeps_16_bits_of_the_weights(lq, lk, hq, hk, d):
+    """bf16, one tile of rows or one block of the other side: weights and dS go into the products as two roundings to bf16, u^2 off."""
+    dtype, g = torch.bfloat16, gen(23)
+    q, go = rand(g, sum(lq), hq, d, dtype=dtype, scale=1.5), rand(g, sum(lq), hq, d, dtype=dtype)
+    k, v = rand(g, sum(lk), hk, d, dtype=dtype), rand(g, sum(lk), hk, d, dtype=dtype)
+    u = unit(dtype)
+    ref = attn_ref(q, k, v, lq, lk, True, d ** -0.5, u, go, uw=u * u)
+    leaves = [t.to("cuda", dtype).requires_grad_(True) for t in (q, k, v)]
+    out = sequence.packed_attention(*leaves, ends(lq), ends(lk), max_q=max(lq), max_k=max(lk))
+    close(out, ref["o"], ref["to"], "out")
+    for n, t in zip(("gq", "gk", "gv"), torch.autograd.grad(out, leaves, go.to("cuda", dtype))):
+        close(t, ref[n], ref["t" + n], n)
 
 
 @pytest.mark.gpu
