@@ -515,7 +515,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 
 // With few rows (one new token of each request: the heads of one group) the keys are what has to be read, once, and nothing else
 // counts.  A wave is a workgroup here: it takes 32 rows and a chunk of keys in blocks of 32, with two tiles of its own that the next
 // block's loads fill while it computes (no barrier: a wave waits for its own loads), and the chunks' results meet in k_attn_join.
-// Bound by HBM: 24 requests of 16384 keys, 8 key heads of 128 (1.6 GB) in 335 us = 4.8 TB/s, where a copy runs at 5.1.  Workgroups of 2
+// Bound by HBM: 24 requests of 1 .. 32768 keys, 8 key heads of 128 (2.03 GB) in 420 us = 4.8 TB/s, where a copy runs at 5.1.  Workgroups of 2
 // or 4 waves that join in LDS were 15 to 50 % slower on short caches (32768 keys of one request: 46 and 60 us against 40).
 template <typename T, int DP>
 struct FewCfg {
