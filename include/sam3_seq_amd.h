@@ -64,9 +64,13 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
  *   causal: query i of n_q sees the keys j <= i + n - n_q (the last query sees all); otherwise every key.
  *   out [Tq, Hq, D] contiguous;  lse [Tq, Hq] fp32 (natural logarithm; NULL: not wanted).  A row that sees no key gives zeros and
  *   lse = -inf, and so do rows of no sequence.  stats [Tq, Hq, 2] fp32 is what the backward takes (NULL: not wanted).
- * max_q, max_k: the longest lengths if known (they size the grid; longer sequences are still computed), or Tq and Tk.
+ * max_q, max_k: the longest lengths if known (they choose the kernels and size the grid; longer sequences are still computed), or Tq and Tk.
+ * sam3_seq_attn_workgroups: the workgroups of the forward's main launch (kernel 0) and of the backward's two (1: gq, 2: gk and gv) -- never
+ * more than a small multiple of the tiles that Tq or Tk rows in B sequences can have -- or -95 where they exceed what can be launched
+ * (2^32 threads: B * Hk in the tens of millions), as the calls do.
  * Key and value rows that a query does not see never enter its result, whatever they hold.
  */
+int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int64_t max_q, int64_t max_k);
 size_t sam3_seq_attn_fwd_workspace_bytes(int64_t Tq, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype);
 int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                       int64_t v_st, int64_t v_sh, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, void* out,

@@ -42,7 +42,7 @@ FP8_EXPORTS = ("sam3_fp8_last_error", "sam3_fp8_quantize")                 # inc
 SEG_EXPORTS = ("sam3_seg_last_error", "sam3_gn_nhwc_supported", "sam3_gn_nhwc_workspace_bytes", "sam3_gn_nhwc_fwd",
                "sam3_gn_nhwc_bwd", "sam3_rpb_bias_fwd")                                             # include/sam3_seg_amd.h
 SEQ_EXPORTS = ("sam3_seq_last_error", "sam3_seq_rms_norm_fwd", "sam3_seq_rms_norm_bwd_workspace_bytes", "sam3_seq_rms_norm_bwd",
-               "sam3_seq_rotary", "sam3_seq_attn_fwd_workspace_bytes", "sam3_seq_attn_fwd", "sam3_seq_attn_bwd_workspace_bytes",
+               "sam3_seq_rotary", "sam3_seq_attn_workgroups", "sam3_seq_attn_fwd_workspace_bytes", "sam3_seq_attn_fwd", "sam3_seq_attn_bwd_workspace_bytes",
                "sam3_seq_attn_bwd")                                                                 # include/sam3_seq_amd.h
 FP8_E4M3, FP8_E5M2 = 0, 1
 FP8_AMAX_SLOTS = 64            # SAM3_FP8_AMAX_SLOTS
@@ -207,6 +207,8 @@ def _declare(lib):
     lib.sam3_seq_rotary.restype = c_int
     lib.sam3_seq_rotary.argtypes = strided * 2 + [c_void_p] * 3 + [c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                                                    c_int64, c_int, c_int, c_int, c_int, c_void_p]
+    lib.sam3_seq_attn_workgroups.restype = c_int64
+    lib.sam3_seq_attn_workgroups.argtypes = [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int64]
     lib.sam3_seq_attn_fwd_workspace_bytes.restype = c_size_t
     lib.sam3_seq_attn_fwd_workspace_bytes.argtypes = [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]
     shape = [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int, c_float, c_int]      # Tq, Tk, B, Hq, Hk, D, max_q, max_k, ...

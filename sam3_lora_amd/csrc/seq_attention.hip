@@ -292,6 +292,29 @@ __device__ __forceinline__ Place place(unsigned id, int pairs, int tiles) {
     const int tile = (slot % per) * s + xcd / lanes;
     return Place{xcd % lanes + lanes * (slot / per), tiles - 1 - tile};        // tile < 0: none
 }
+// The longest sequence's tiles for every pair are far too many where the others are much shorter, or where nobody said how long they are.
+// Then the tiles are listed instead: sequence b, whose rows begin at row cu[b] * g of all, has the places from cu[b] * g / PER + b on, at
+// least as many as it has tiles, and a workgroup finds its sequence among them, 64 at a time.  The heads of a place are neighbours.
+__device__ __forceinline__ long long first_place(const int* cu, int b, int g, int per, long long total) {
+    const long long c = cu[b];
+    return (c < 0 ? 0 : c > total ? total : c) * g / per + b;
+}
+template <int PER>
+__device__ __forceinline__ Place listed(unsigned id, const int* cu, int B, int Hk, int g, long long total) {
+    const int lane = threadIdx.x & 63, kv = (int)(id % (unsigned)Hk);
+    const long long slot = id / (unsigned)Hk;
+    int lo = 0, n = B;              // the sequence is one of lo .. lo + n - 1
+    while (n > 1) {
+        const int apart = (n + 63) / 64, at = lane * apart;
+        const int below = __popcll(__ballot(at < n && first_place(cu, lo + min(at, n - 1), g, PER, total) <= slot));
+        const int skip = (below > 1 ? below - 1 : 0) * apart;
+        lo += skip;
+        n = min(apart, n - skip);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const long long tile = slot - first_place(cu, lo, g, PER, total);
+    return Place{lo * Hk + kv, (int)(tile < 0 ? -1 : tile)};
+}
 
 // 16 bytes per lane straight into LDS, lane l's to lds + 16 l, from an address of the wave and 32 bits of the lane.  The instruction is
 // written out because the compiler would wait for every such load before any later read of LDS, and the loads of the next tile have to
@@ -423,7 +446,7 @@ struct FwdState {
 };
 
 // (three waves share a SIMD's registers up to heads of 128 bytes: 4 x 5184, heads of 64: 707 -> 674 us)
-template <typename T, int DP>
+template <typename T, int DP, bool LISTED>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 128 ? 3 : 2)) void k_attn_fwd(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     constexpr int BN = FwdCfg<T, DP>::BN, TB = BN * L::ROWB;
@@ -440,7 +463,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 
         }
         return;
     }
-    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    const Place pl = LISTED ? listed<BM>(blockIdx.x, a.cu_q, a.B, a.Hk, a.G, a.Tq) : place(blockIdx.x, a.B * a.Hk, tiles);
     if (pl.tile < 0) return;
     const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, a.len_k, b, a.Tk);
@@ -741,7 +764,7 @@ struct GqState {
     }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool LISTED>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     constexpr int BN = GqCfg<T, DP>::BN, TB = BN * L::ROWB;
@@ -755,7 +778,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq
             zero_row(gq + (z.row(i / a.Hq) * a.Hq + i % a.Hq) * a.D, a.D, threadIdx.x & 7, 8);
         return;
     }
-    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    const Place pl = LISTED ? listed<BM>(blockIdx.x, a.cu_q, a.B, a.Hk, a.G, a.Tq) : place(blockIdx.x, a.B * a.Hk, tiles);
     if (pl.tile < 0) return;
     const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
@@ -1017,7 +1040,7 @@ struct GkvState {
     }
 };
 
-template <typename T, int DP, bool EVEN>
+template <typename T, int DP, bool EVEN, bool LISTED>
 __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     typedef GkvCfg<T, DP> C;
@@ -1037,9 +1060,9 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
         }
         return;
     }
-    const Place pl = place(blockIdx.x, a.B * a.Hk, tiles);
+    const Place pl = LISTED ? listed<BK>(blockIdx.x, a.cu_k, a.B, a.Hk, 1, a.Tk) : place(blockIdx.x, a.B * a.Hk, tiles);
     if (pl.tile < 0) return;
-    const int tile = tiles - 1 - pl.tile;       // the first keys have the most rows
+    const int tile = LISTED ? pl.tile : tiles - 1 - pl.tile;       // the first keys have the most rows
     const int b = pl.pair / a.Hk, kv = pl.pair - b * a.Hk;
     const Span sq = span(a.cu_q, nullptr, b, a.Tq), sk = span(a.cu_k, nullptr, b, a.Tk);
     if ((long long)tile * BK >= sk.n) return;
@@ -1442,22 +1465,42 @@ int check_tensor(const char* name, const void* p, int64_t st, int64_t sh, bool g
 
 constexpr unsigned REST = 32;       // workgroups that clear the rows of no sequence (mostly there are none)
 
-#define BY_HEAD(KERNEL, GRID, ST, ...)                                                                         \
+#define BY_HEAD(KERNEL, FLAG, GRID, ST, ...)                                                                         \
     do {                                                                                                        \
         if (dtype == 0) {                                                                                       \
-            if (D <= 32) hipLaunchKernelGGL((KERNEL<bf16_t, 32>), GRID, dim3(256), 0, ST, __VA_ARGS__);                 \
-            else if (D <= 64) hipLaunchKernelGGL((KERNEL<bf16_t, 64>), GRID, dim3(256), 0, ST, __VA_ARGS__);            \
-            else hipLaunchKernelGGL((KERNEL<bf16_t, 128>), GRID, dim3(256), 0, ST, __VA_ARGS__);                        \
+            if (D <= 32) hipLaunchKernelGGL((KERNEL<bf16_t, 32, FLAG>), GRID, dim3(256), 0, ST, __VA_ARGS__);                 \
+            else if (D <= 64) hipLaunchKernelGGL((KERNEL<bf16_t, 64, FLAG>), GRID, dim3(256), 0, ST, __VA_ARGS__);            \
+            else hipLaunchKernelGGL((KERNEL<bf16_t, 128, FLAG>), GRID, dim3(256), 0, ST, __VA_ARGS__);                        \
         } else {                                                                                                \
-            if (D <= 32) hipLaunchKernelGGL((KERNEL<float, 32>), GRID, dim3(256), 0, ST, __VA_ARGS__);                  \
-            else if (D <= 64) hipLaunchKernelGGL((KERNEL<float, 64>), GRID, dim3(256), 0, ST, __VA_ARGS__);             \
-            else hipLaunchKernelGGL((KERNEL<float, 128>), GRID, dim3(256), 0, ST, __VA_ARGS__);                         \
+            if (D <= 32) hipLaunchKernelGGL((KERNEL<float, 32, FLAG>), GRID, dim3(256), 0, ST, __VA_ARGS__);                  \
+            else if (D <= 64) hipLaunchKernelGGL((KERNEL<float, 64, FLAG>), GRID, dim3(256), 0, ST, __VA_ARGS__);             \
+            else hipLaunchKernelGGL((KERNEL<float, 128, FLAG>), GRID, dim3(256), 0, ST, __VA_ARGS__);                         \
         }                                                                                                       \
     } while (0)
 
 unsigned tiles(int64_t rows, int per) {
     const int64_t t = (rows + per - 1) / per;
     return (unsigned)(t < 1 ? 1 : t);
+}
+
+// The tiles for each pair and the places of a launch; listed: one tile for a workgroup.  A grid has fewer than 2^32 threads.
+struct Grid {
+    int tiles;
+    long long places;
+    int threads;            // of a workgroup
+    bool listed = false;
+    bool fits() const { return (places + REST) * threads < 1ll << 32; }
+    unsigned first_rest() const { return (unsigned)places; }
+    dim3 grid() const { return dim3((unsigned)(places + REST)); }
+};
+// Tiles of `per` rows for each pair of a sequence and a key head: as many as the longest has, or listed (`total` rows lie in all) where that is
+// over four times what there can be.  Measured on both sides (us, the longest's / listed; heads of 128, 32 / 8; forward, then backward):
+// sequences of 1 .. 2048, 1.8 times: 707 / 692, 2576 / 2863; 64 of 512 and one of 4096, 6.8 times: 682 / 572, 2264 / 2346; 255 of 256 and one of
+// 4096, 13 times: 1305 / 884, 4796 / 3514; 400 of 150 without hints, 216 times (16 heads of 64): 3958 / 309, 8633 / 849.
+Grid tiled(int64_t longest, int64_t total, int B, int Hk, int per) {
+    const int64_t all = Hk * (total / per + B);
+    const int each = (int)tiles(longest, per);
+    return places(B * Hk, each) > 4 * all + 4096 ? Grid{1 << 25, all, 256, true} : Grid{each, places(B * Hk, each), 256};
 }
 
 // The forward for few rows: rows of one token's heads or so (32 prompts' worth of short rows run 21 us in tiles of 128 and 11 in tiles of
@@ -1484,6 +1527,23 @@ Plan plan(int64_t Tq, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
     p.splits = (int)((max_k + p.chunk - 1) / p.chunk);
     if (p.splits < 1) p.splits = 1;
     return p;
+}
+// The backward's launches.  Tiles of 32, shared by the waves of a workgroup, where tiles of 128 would be too few for the chip.  Measured on both
+// sides (us, tiles of 128 / of 32; bf16): gq at 48 tiles 63 / 25, at 128 143 / 119, at 256 51 / 77; gk and gv at 64 241 / 72, at 128 438 / 155, at
+// 256 859 / 524.
+struct Backward {
+    bool q_split, k_split;
+    Grid q, k;
+};
+Backward backward_of(int64_t Tq, int64_t Tk, int B, int G, int Hk, int64_t longest_q, int64_t longest_k) {
+    const int64_t pairs = (int64_t)B * Hk, rows = longest_q * G;
+    Backward b;
+    b.q_split = pairs * tiles(rows, BM) <= 128 || rows <= 32;
+    b.k_split = pairs * tiles(longest_k, 128) <= 256 || longest_k <= 32;
+    const int qt = (int)tiles(rows, 32), kt = (int)tiles(longest_k, 32);
+    b.q = b.q_split ? Grid{qt, places(B * Hk, qt), 256} : tiled(rows, Tq * G, B, Hk, BM);
+    b.k = b.k_split ? Grid{kt, places(B * Hk, kt), 256} : tiled(longest_k, Tk, B, Hk, 128);
+    return b;
 }
 size_t part_bytes(int64_t Tq, int Hq, int D, int splits) {
     return splits > 1 ? (size_t)splits * Tq * Hq * (D * sizeof(float) + sizeof(float2)) : 0;
@@ -1523,10 +1583,12 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
         if (need && (!workspace || workspace_bytes < need || misaligned(workspace)))
             return sam3_seq_fail(ENOMEM_, "attention: workspace too small or misaligned: %zu < %zu", workspace_bytes, need);
         const long long items = (long long)B * Hk * p.splits;
-        if (items > 0x3fffffffll || places((int)items, p.tiles) > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
-        Few f{p.tiles, p.splits, p.chunk, (float*)workspace, nullptr, (unsigned)places((int)items, p.tiles)};
+        if (items > 0x3fffffffll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+        const Grid g{p.tiles, places((int)items, p.tiles), 64};
+        if (!g.fits()) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+        Few f{p.tiles, p.splits, p.chunk, (float*)workspace, nullptr, g.first_rest()};
         f.pstat = reinterpret_cast<float2*>(f.part + (p.splits > 1 ? (size_t)p.splits * Tq * Hq * D : 0));
-        const dim3 grid(f.first_rest + REST);
+        const dim3 grid = g.grid();
         hipStream_t st = (hipStream_t)stream;
 #define FEW(TY, W)                                                                                                    \
     do {                                                                                                              \
@@ -1545,13 +1607,28 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
         }
         return launched("sam3_seq_attn_fwd");
     }
-    const int64_t longest = max_q < Tq ? max_q : Tq;
-    const int nt = (int)tiles(longest * a.G, BM);
-    const long long first_rest = places(B * Hk, nt);
-    if (first_rest > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
-    const dim3 grid((unsigned)first_rest + REST);
-    BY_HEAD(k_attn_fwd, grid, (hipStream_t)stream, a, nt, (unsigned)first_rest);
+    const Grid g = tiled((max_q < Tq ? max_q : Tq) * a.G, Tq * a.G, B, Hk, BM);
+    if (!g.fits()) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+    if (g.listed) BY_HEAD(k_attn_fwd, true, g.grid(), (hipStream_t)stream, a, g.tiles, g.first_rest());
+    else BY_HEAD(k_attn_fwd, false, g.grid(), (hipStream_t)stream, a, g.tiles, g.first_rest());
     return launched("sam3_seq_attn_fwd");
+}
+
+int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
+    sam3_seq_clear_error();
+    if (int rc = check(Tq, Tk, B, Hq, Hk, 8, max_q, max_k, 1.f, 0)) return rc;
+    if (kernel < 0 || kernel > 2) return sam3_seq_fail(EINVAL_, "attention: no launch %d", kernel);
+    if (B == 0) max_q = max_k = 0;
+    const int64_t lq = max_q < Tq ? max_q : Tq, lk = max_k < Tk ? max_k : Tk;
+    Grid g;
+    if (kernel == 0) {
+        const Plan p = plan(Tq, B, Hq, Hk, max_q, max_k);
+        g = p.few ? Grid{p.tiles, places(B * Hk * p.splits, p.tiles), 64} : tiled(lq * (Hq / Hk), Tq * (Hq / Hk), B, Hk, BM);
+    } else {
+        const Backward w = backward_of(Tq, Tk, B, Hq / Hk, Hk, lq, lk);
+        g = kernel == 1 ? w.q : w.k;
+    }
+    return g.fits() ? g.places + REST : sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
 }
 
 size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq) { return Tq > 0 && Hq > 0 ? (size_t)Tq * Hq * 3 * sizeof(float) : 0; }
@@ -1582,24 +1659,19 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh; a.go_st = go_st; a.go_sh = go_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest_q = max_q < Tq ? max_q : Tq, longest_k = max_k < Tk ? max_k : Tk;
-    // Tiles of 32, shared by the waves of a workgroup, where tiles of 128 would be too few for the chip.  Measured on both sides (us, tiles of
-    // 128 / of 32; bf16): gq at 48 tiles 63 / 25, at 128 143 / 119, at 256 51 / 77; gk and gv at 64 241 / 72, at 128 438 / 155, at 256 859 / 524.
-    const int64_t pairs = (int64_t)B * Hk;
-    const bool q_split = pairs * tiles(longest_q * a.G, BM) <= 128 || longest_q * a.G <= 32,
-               k_split = pairs * tiles(longest_k, 128) <= 256 || longest_k <= 32;
-    const int qt = (int)tiles(longest_q * a.G, q_split ? 32 : BM), kt = (int)tiles(longest_k, k_split ? 32 : 128);
-    const long long q_rest = places(B * Hk, qt), k_rest = places(B * Hk, kt);
-    if (q_rest > 0x7ffffff0ll || k_rest > 0x7ffffff0ll) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+    const Backward w = backward_of(Tq, Tk, B, a.G, Hk, longest_q, longest_k);
+    if (!w.q.fits() || !w.k.fits()) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
     const bool q_one = longest_k <= 64, k_one = longest_q * a.G <= 64;      // not more than two blocks for the waves to share
     hipStream_t st = (hipStream_t)stream;
     if (Tq > 0) {
-        const dim3 grid((unsigned)q_rest + REST);
+        const dim3 grid = w.q.grid();
 #define GQ(TY, W)                                                                                                                       \
     do {                                                                                                                                \
         constexpr int NW = sizeof(TY) * W > 256 ? 2 : 4;                                                                                \
-        if (!q_split) hipLaunchKernelGGL((k_attn_gq<TY, W>), grid, dim3(256), 0, st, a, qt, (unsigned)q_rest);                          \
-        else if (q_one) hipLaunchKernelGGL((k_attn_gq_split<TY, W, 1>), grid, dim3(64), 0, st, a, qt, (unsigned)q_rest);                \
-        else hipLaunchKernelGGL((k_attn_gq_split<TY, W, NW>), grid, dim3(NW * 64), 0, st, a, qt, (unsigned)q_rest);                     \
+        if (w.q.listed) hipLaunchKernelGGL((k_attn_gq<TY, W, true>), grid, dim3(256), 0, st, a, w.q.tiles, w.q.first_rest());             \
+        else if (!w.q_split) hipLaunchKernelGGL((k_attn_gq<TY, W, false>), grid, dim3(256), 0, st, a, w.q.tiles, w.q.first_rest());                          \
+        else if (q_one) hipLaunchKernelGGL((k_attn_gq_split<TY, W, 1>), grid, dim3(64), 0, st, a, w.q.tiles, w.q.first_rest());                \
+        else hipLaunchKernelGGL((k_attn_gq_split<TY, W, NW>), grid, dim3(NW * 64), 0, st, a, w.q.tiles, w.q.first_rest());                     \
     } while (0)
         if (dtype == 0) { if (D <= 32) GQ(bf16_t, 32); else if (D <= 64) GQ(bf16_t, 64); else GQ(bf16_t, 128); }
         else { if (D <= 32) GQ(float, 32); else if (D <= 64) GQ(float, 64); else GQ(float, 128); }
@@ -1607,16 +1679,17 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
         if (int rc = launched("sam3_seq_attn_bwd")) return rc;
     }
     if (Tk > 0) {
-        const dim3 grid((unsigned)k_rest + REST);
+        const dim3 grid = w.k.grid();
 #define GKV(TY, W)                                                                                                                      \
     do {                                                                                                                                \
         constexpr int NW = sizeof(TY) * W > 256 ? 2 : 4;                                                                                \
-        if (!k_split) { if (GkvCfg<TY, W>::BR % a.G == 0) hipLaunchKernelGGL((k_attn_gkv<TY, W, true>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest); \
-                        else hipLaunchKernelGGL((k_attn_gkv<TY, W, false>), grid, dim3(256), 0, st, a, kt, (unsigned)k_rest); }          \
-        else if (k_one) { if (32 % a.G == 0) hipLaunchKernelGGL((k_attn_gkv_split<TY, W, 1, true>), grid, dim3(64), 0, st, a, kt, (unsigned)k_rest);      \
-                          else hipLaunchKernelGGL((k_attn_gkv_split<TY, W, 1, false>), grid, dim3(64), 0, st, a, kt, (unsigned)k_rest); } \
-        else { if (32 % a.G == 0) hipLaunchKernelGGL((k_attn_gkv_split<TY, W, NW, true>), grid, dim3(NW * 64), 0, st, a, kt, (unsigned)k_rest);           \
-               else hipLaunchKernelGGL((k_attn_gkv_split<TY, W, NW, false>), grid, dim3(NW * 64), 0, st, a, kt, (unsigned)k_rest); }      \
+        if (w.k.listed) hipLaunchKernelGGL((k_attn_gkv<TY, W, false, true>), grid, dim3(256), 0, st, a, w.k.tiles, w.k.first_rest());     \
+        else if (!w.k_split) { if (GkvCfg<TY, W>::BR % a.G == 0) hipLaunchKernelGGL((k_attn_gkv<TY, W, true, false>), grid, dim3(256), 0, st, a, w.k.tiles, w.k.first_rest()); \
+                        else hipLaunchKernelGGL((k_attn_gkv<TY, W, false, false>), grid, dim3(256), 0, st, a, w.k.tiles, w.k.first_rest()); }          \
+        else if (k_one) { if (32 % a.G == 0) hipLaunchKernelGGL((k_attn_gkv_split<TY, W, 1, true>), grid, dim3(64), 0, st, a, w.k.tiles, w.k.first_rest());      \
+                          else hipLaunchKernelGGL((k_attn_gkv_split<TY, W, 1, false>), grid, dim3(64), 0, st, a, w.k.tiles, w.k.first_rest()); } \
+        else { if (32 % a.G == 0) hipLaunchKernelGGL((k_attn_gkv_split<TY, W, NW, true>), grid, dim3(NW * 64), 0, st, a, w.k.tiles, w.k.first_rest());           \
+               else hipLaunchKernelGGL((k_attn_gkv_split<TY, W, NW, false>), grid, dim3(NW * 64), 0, st, a, w.k.tiles, w.k.first_rest()); }      \
     } while (0)
         if (dtype == 0) { if (D <= 32) GKV(bf16_t, 32); else if (D <= 64) GKV(bf16_t, 64); else GKV(bf16_t, 128); }
         else { if (D <= 32) GKV(float, 32); else if (D <= 64) GKV(float, 64); else GKV(float, 128); }
