@@ -519,6 +519,7 @@ __global__ __launch_bounds__(256) void k_rotary(Rope a, RopeTable tab, int pos_t
     }
 }
 
+constexpr long long MOST_BLOCKS = (1ll << 32) / 256 - 1;
 unsigned magic(unsigned d) { return (unsigned)((0x100000000ull + d - 1) / d); }
 
 }  // namespace
@@ -602,8 +603,11 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
     a.mul_row = magic(a.row_items);
     if ((uint64_t)a.TT * a.row_items * a.row_items >= 0x100000000ull) a.TT = 1;
     if ((uint64_t)a.row_items * a.row_items >= 0x100000000ull) return sam3_seq_fail(ENOTSUP_, "rotary: too many elements in a token's heads");
+    // (a grid has fewer than 2^32 threads: from 2^27 tokens on, more of them share a table)
+    if ((T + a.TT - 1) / a.TT > MOST_BLOCKS) a.TT = (int)(T / MOST_BLOCKS + 1 < 1024 ? T / MOST_BLOCKS + 1 : 1024);
     const long long blocks = (T + a.TT - 1) / a.TT;
-    if (blocks > 0x7fffffffll) return sam3_seq_fail(ENOTSUP_, "rotary: too many tokens");
+    if (blocks > MOST_BLOCKS || (uint64_t)a.TT * a.row_items * a.row_items >= 0x100000000ull || (int64_t)a.TT * pairs > 8192)
+        return sam3_seq_fail(ENOTSUP_, "rotary: too many tokens");
     const size_t lds = (size_t)a.TT * pairs * sizeof(float2);
     hipStream_t st = (hipStream_t)stream;
 #define ROT(TY, F) hipLaunchKernelGGL((k_rotary<TY, F>), dim3((unsigned)blocks), dim3(256), lds, st, a, tab, pos_type)

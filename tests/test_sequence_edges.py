@@ -69,3 +69,25 @@ def test_very_many_sequences_without_hints(lens, hq, hk, d, causal, dtype):
     assert (lse[:5] == -math.inf).all() and (lse[5 + sum(lens):] == -math.inf).all()
     with torch.no_grad():           # the same tiles, told how long they are
         assert torch.equal(sequence.packed_attention(*leaves, cu, causal=causal, max_q=max(lens), max_k=max(lens)), out)
+
+
+# ------------------------------------------------------------------------------------------------------ very many tokens
+def test_rotary_axes_refuses_more_tokens_than_a_launch_can_have():
+    import ctypes
+    lib, p = _ffi.load(), ctypes.c_void_p(64)
+    turns, axis = (ctypes.c_double * 4)(), (ctypes.c_ubyte * 4)()
+    for t in (1 << 46, (1 << 62) + 1):
+        assert lib.sam3_seq_rotary(p, 8, 8, None, 0, 0, p, None, p, 0, 1, 0, 1, turns, axis, 4, 0, 0, t, 1, 0, 8, 0, None) == -95
+        assert "tokens" in lib.sam3_seq_last_error().decode()
+
+
+@pytest.mark.gpu
+def test_rotary_axes_of_more_tokens_than_2_to_27():
+    """Eight tokens to a workgroup of 256 would be 2^32 threads and more, which no launch has."""
+    t = (1 << 27) + 4099
+    q = torch.randn(4099, 1, 8, generator=gen(1)).to("cuda", torch.bfloat16).repeat((t + 4098) // 4099, 1, 1)[:t]
+    pos = torch.arange(4099, device="cuda", dtype=torch.int32).repeat((t + 4098) // 4099)[None, :t]
+    out = sequence.rotary_axes(q, None, pos, (4,))
+    want = sequence.rotary_axes(q[:4099], None, pos[:, :4099], (4,))
+    whole = t // 4099 * 4099
+    assert torch.equal(out[:whole].view(-1, 4099, 1, 8), want.expand(whole // 4099, 4099, 1, 8).view(-1, 4099, 1, 8)) and torch.equal(out[whole:], want[:t - whole])
