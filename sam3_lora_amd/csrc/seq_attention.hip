@@ -595,43 +595,54 @@ __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_a
 #pragma unroll
         for (int s = 0; s < KS; ++s)
             st.qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + s * 16 + h * 8, live && s * 16 + h * 8 < a.D);
+        // With FINE an infinity among the values, multiplied by a weight's rest that is zero or negative, would come out as NaN: where a result is
+        // not finite the keys are gone over once more, each block checked as those at the border are.
+        for (bool checked = false;; checked = true) {
 #pragma unroll
-        for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
-        st.base = -3.0e38f;
-        st.l = 0.f;
-        for (long long c0 = (long long)split * f.chunk; c0 < jend; c0 += (long long)f.splits * f.chunk) {
-            const int begin = (int)c0, end = (int)(c0 + f.chunk < jend ? c0 + f.chunk : jend);
-            const int full = min(end, jall) >= begin ? (min(end, jall) - begin) / 32 : 0;       // blocks that need no mask
-            int blk = 0, buf = 0;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (blk < full) {
-                dk.load(k + (long long)(begin + blk * 32) * a.k_st, a.k_st, at_lds);
-                dv.load(v + (long long)(begin + blk * 32) * a.v_st, a.v_st, at_lds + TB);
-                wait_loads<0>();        // (for the rows' own loads too, which the loop would otherwise wait for)
-            }
-            for (; blk < full; ++blk, buf ^= 1) {
-                char* now = mine + buf * 2 * TB;
-                const unsigned next = at_lds + (buf ^ 1) * 2 * TB;
-                // what was read of the other buffer has arrived; then its new loads, and the wait for all but those
+            for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
+            st.base = -3.0e38f;
+            st.l = 0.f;
+            for (long long c0 = (long long)split * f.chunk; c0 < jend; c0 += (long long)f.splits * f.chunk) {
+                const int begin = (int)c0, end = (int)(c0 + f.chunk < jend ? c0 + f.chunk : jend);
+                const int full = !checked && min(end, jall) >= begin ? (min(end, jall) - begin) / 32 : 0;       // blocks that need no mask
+                int blk = 0, buf = 0;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (blk + 1 < full) {
-                    dk.load(k + (long long)(begin + (blk + 1) * 32) * a.k_st, a.k_st, next);
-                    dv.load(v + (long long)(begin + (blk + 1) * 32) * a.v_st, a.v_st, next + TB);
-                    wait_loads<2 * Dma<T, DP, 32, 64>::N>();
-                } else {
-                    wait_loads<0>();
+                if (blk < full) {
+                    dk.load(k + (long long)(begin + blk * 32) * a.k_st, a.k_st, at_lds);
+                    dv.load(v + (long long)(begin + blk * 32) * a.v_st, a.v_st, at_lds + TB);
+                    wait_loads<0>();        // (for the rows' own loads too, which the loop would otherwise wait for)
                 }
-                st.template step<false, FINE>(now, now + TB, lane, c2, 32);
+                for (; blk < full; ++blk, buf ^= 1) {
+                    char* now = mine + buf * 2 * TB;
+                    const unsigned next = at_lds + (buf ^ 1) * 2 * TB;
+                    // what was read of the other buffer has arrived; then its new loads, and the wait for all but those
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (blk + 1 < full) {
+                        dk.load(k + (long long)(begin + (blk + 1) * 32) * a.k_st, a.k_st, next);
+                        dv.load(v + (long long)(begin + (blk + 1) * 32) * a.v_st, a.v_st, next + TB);
+                        wait_loads<2 * Dma<T, DP, 32, 64>::N>();
+                    } else {
+                        wait_loads<0>();
+                    }
+                    st.template step<false, FINE>(now, now + TB, lane, c2, 32);
+                }
+                for (int i = full; begin + i * 32 < end; ++i) {
+                    const int k0 = begin + i * 32;
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    stage<T, DP, 32, false, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+                    const bool bad = __any(stage<T, DP, 32, true, 64>(mine + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; }));
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    st.template step<true, FINE>(mine, mine + TB, lane, c2, min(jmax, end) - k0);
+                    if (bad) add_nonfinite<T, DT>(st.acc, v + (long long)k0 * a.v_st, a.v_st, min(min(jmax, end) - k0, 32), a.D, h);
+                }
             }
-            for (int i = full; begin + i * 32 < end; ++i) {
-                const int k0 = begin + i * 32;
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                stage<T, DP, 32, false, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
-                const bool bad = __any(stage<T, DP, 32, true, 64>(mine + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; }));
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                st.template step<true, FINE>(mine, mine + TB, lane, c2, min(jmax, end) - k0);
-                if (bad) add_nonfinite<T, DT>(st.acc, v + (long long)k0 * a.v_st, a.v_st, min(min(jmax, end) - k0, 32), a.D, h);
-            }
+            if (!FINE || checked) break;
+            float odd = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) odd = fmaf(st.acc[d][i], 0.f, odd);
+            if (!__any(odd != 0.f)) break;
         }
         const float l = st.l + __shfl_xor(st.l, 32, 64);
         if (!live) continue;

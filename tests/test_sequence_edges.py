@@ -91,3 +91,38 @@ def test_rotary_axes_of_more_tokens_than_2_to_27():
     want = sequence.rotary_axes(q[:4099], None, pos[:, :4099], (4,))
     whole = t // 4099 * 4099
     assert torch.equal(out[:whole].view(-1, 4099, 1, 8), want.expand(whole // 4099, 4099, 1, 8).view(-1, 4099, 1, 8)) and torch.equal(out[whole:], want[:t - whole])
+
+
+# ----------------------------------------------------------------------------------------------- values that are not finite
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_one_token_sees_an_infinite_value(value, d, dtype):
+    """One token over its keys, in one chunk and in several: the value's infinity is the result's, whichever block of keys it lies in, and no other
+    element changes."""
+    g = gen(d)
+    lk, hq, hk = [70, 33, 200, 2100, 5000], 4, 2
+    q = rand(g, len(lk), hq, d, dtype=dtype).to("cuda", dtype)
+    k, v = (rand(g, sum(lk), hk, d, dtype=dtype).to("cuda", dtype) for _ in range(2))
+    cu_q, cu_k = ends([1] * len(lk)), ends(lk)
+
+    def call(v):
+        return sequence.packed_attention(q, k, v, cu_q, cu_k, max_q=1, max_k=max(lk))
+    good = call(v)
+    begin = 0
+    for i, n in enumerate(lk):
+        for at in {0, n // 2, n - 1, n - n % 32 - 1}:
+            bad = v.clone()
+            bad[begin + at, 1, 5] = value
+            bad[begin + at, 1, 8] = -value
+            out = call(bad)
+            got = out[i, hq // hk:]
+            want = good.clone()
+            want[i, hq // hk:, 5], want[i, hq // hk:, 8] = got[:, 5], got[:, 8]
+            assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(), want.nan_to_num()), (n, at)
+            if math.isnan(value):
+                assert got[:, 5].isnan().all() and got[:, 8].isnan().all(), (n, at)
+            else:
+                assert (got[:, 5] == value).all() and (got[:, 8] == -value).all(), (n, at)
+        begin += n
