@@ -189,6 +189,9 @@ __device__ __forceinline__ int seen_keys(int token, int nq, int nk, int causal) 
     return j < 0 ? 0 : j > nk ? nk : (int)j;
 }
 
+// 1 / sum of a row's weights.  There are none where the row sees no key (zeros come out), and where all its scores are -inf (0 / 0)
+__device__ __forceinline__ float one_over(float sum, int keys) { return sum != 0.f ? 1.f / sum : keys > 0 ? NAN : 0.f; }
+
 // rows of one (sequence, head group) as addresses: row r -> token r / G, head kv * G + r % G
 struct Rows {
     long long begin, st, sh;
@@ -521,7 +524,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 
             if (bad) add_nonfinite<T, DT>(st.acc, v + (long long)k0 * a.v_st, a.v_st, min(jmax - k0, BN), a.D, h);
         }
         const float l = st.l + __shfl_xor(st.l, 32, 64);
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const float inv = one_over(l, jmax);
         if (live) {
             const int t = row / a.G, head = kv * a.G + row - t * a.G;
             const long long at = (sq.begin + t) * a.Hq + head;
@@ -654,7 +657,7 @@ __global__ __launch_bounds__(64, (FewCfg<T, DP>::LDS >= 32768 ? 1 : 2)) void k_a
             for (int d = 0; d < DT; ++d) store_cols(f.part + to * a.D, st.acc[d], d, h, a.D, 1.f);
             if (h == 0) f.pstat[to] = make_float2(st.base, l);
         } else {
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            const float inv = one_over(l, jmax);
 #pragma unroll
             for (int d = 0; d < DT; ++d) store_cols(out + at * a.D, st.acc[d], d, h, a.D, inv);
             if (a.stats && h == 0) a.stats[at] = make_float2(st.base, inv);
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Attn a, Few f) {
                 o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
                 sum += part_sum[g];
             }
-            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+            const float inv = one_over(sum, seen_keys(t, sq.n, sk.n, a.causal));
             if (d < a.D) {
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + at * a.D + d) = make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
                 else *reinterpret_cast<float4*>(out + at * a.D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);

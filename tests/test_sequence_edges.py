@@ -126,3 +126,25 @@ def test_one_token_sees_an_infinite_value(value, d, dtype):
             else:
                 assert (got[:, 5] == value).all() and (got[:, 8] == -value).all(), (n, at)
         begin += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("times", [1, 300])
+@pytest.mark.parametrize("nk", [1, 70, 1500])
+def test_a_row_whose_scores_are_all_minus_infinity_is_not_one_that_sees_no_key(nk, times, dtype):
+    """softmax of nothing but -inf is 0 / 0, as it is in the formulas; a row without keys gives zeros.  With 300 sequences more the tiles of 128 run."""
+    g = gen(nk)
+    lq, lk = [3, 2] + [5] * (times - 1), [nk, 0] + [7] * (times - 1)
+    q, go = (rand(g, sum(lq), 2, 64, dtype=dtype).to("cuda", dtype) for _ in range(2))
+    k, v = (rand(g, sum(lk), 1, 64, dtype=dtype).to("cuda", dtype) for _ in range(2))
+    k[:nk, 0, 7] = k[:nk, 0, 7].abs() + 1
+    q[2, 1, 7] = -math.inf              # the last row of the first sequence sees all of its keys, in one of its heads
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out, lse = sequence.packed_attention(*leaves, ends(lq), ends(lk), max_q=max(lq), max_k=max(lk), return_lse=True)
+    assert out[2, 1].isnan().all() and lse[2, 1] == -math.inf
+    assert torch.isfinite(out[2, 0]).all() and not out[3:5].any() and torch.isfinite(out[5:]).all()
+    assert not out[0].any() if nk == 1 else torch.isfinite(out[:2]).all()
+    gq, gk, gv = torch.autograd.grad(out, leaves, go)
+    assert gq[2, 1].isnan().all() and gk[:nk].isnan().all() and gv[:nk].isnan().all()
+    assert torch.isfinite(gq[2, 0]).all() and not gq[3:5].any() and torch.isfinite(gq[5:]).all() and torch.isfinite(gk[nk:]).all() and torch.isfinite(gv[nk:]).all()
