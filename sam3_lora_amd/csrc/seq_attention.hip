@@ -205,7 +205,7 @@ struct Rows {
 // ROWS rows (n of them there, the others zeros) of DP elements (D of them there) into LDS by NT threads.
 // CHECK: infinities and NaN become zeros, and the answer says whether there were any.  A product over a tile that some of its rows
 // only see a part of multiplies what they do not see by zero, which a non-finite element would turn into NaN; such tiles are
-// staged with the check, and the rows that do see such an element get its effect afterwards (spoils(), add_nonfinite()).
+// staged with the check, and the rows that do see such an element get its effect afterwards (spoils(), add_nonfinite(), add_to_row()).
 __device__ __forceinline__ bool finite_bits(unsigned u, bf16_t) { return (u & 0x7f80u) != 0x7f80u && (u & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ bool finite_bits(unsigned u, float) { return (u & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ unsigned only_finite(unsigned u, bf16_t) {
@@ -237,6 +237,30 @@ __device__ bool spoils(const T* row, int D) {
     bool bad = false;
     for (int d = 0; d < D; ++d) bad |= !(fabsf(ld1(row + d)) <= 3.402823466e38f);
     return bad;
+}
+
+template <typename T>
+__device__ float dot(const T* a, const T* b, int D) {
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) s = fmaf(ld1(a + d), ld1(b + d), s);
+    return s;
+}
+// out += w x in memory, by a lane half's columns (store_cols()); rest: only where that is not finite, since the finite part is in it already
+template <typename T>
+__device__ void add_to_row(T* out, float w, const T* x, int D, int h, bool rest) {
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) {
+        const float y = w * ld1(x + d);
+        if ((d >> 2 & 1) == h && !(rest && fabsf(y) <= 3.402823466e38f)) st1(out + d, ld1(out + d) + y);
+    }
+}
+// Clears the rows of a staged tile that hold an infinity or a NaN: their products with the others of the tile come to nothing then.
+template <typename T, int DP, int NT>
+__device__ void clear_spoilt(char* lds, const T* base, long long st, int n, int D) {
+    for (int row = threadIdx.x % NT; row < n; row += NT)
+        if (spoils(base + row * st, D))
+            for (int c = 0; c < Tile<T, DP>::ROWB; c += 16) *reinterpret_cast<uint4*>(lds + row * Tile<T, DP>::ROWB + c) = make_uint4(0, 0, 0, 0);
 }
 
 // the result's registers of one 32-column block of a row, four neighbours at a time
@@ -740,6 +764,14 @@ struct GqState {
     f32x16 acc[DT];
     float base, delta, sum;
 
+    // the keys first .. end - 1 that are not finite, and that the steps took for zeros, into the row's gradient in memory
+    __device__ __forceinline__ void add_spoilt(T* out, float mul, const T* q, const T* go, const T* k, long long k_st, const T* v, long long v_st, int first, int end, int D, int h,
+                                               float c2) const {
+#pragma unroll 1
+        for (int j = first; j < end; ++j)
+            if (spoils(k + j * k_st, D))
+                add_to_row(out, __builtin_amdgcn_exp2f(fmaf(dot(q, k + j * k_st, D), c2, -base)) * (dot(go, v + j * v_st, D) - delta) * mul, k + j * k_st, D, h, false);
+    }
     template <bool MASK, bool SUM = false, bool FINE = false>
     __device__ __forceinline__ void step(const char* lk, const char* lv, int lane, float c2, int left) {
         const int h = lane >> 5;
@@ -779,11 +811,12 @@ struct GqState {
 };
 
 template <typename T, int DP, bool LISTED>
-__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq(Attn a, int tiles, unsigned first_rest) {
+__global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 64 ? 3 : 2)) void k_attn_gq(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
     constexpr int BN = GqCfg<T, DP>::BN, TB = BN * L::ROWB;
     constexpr int KS = DP / 16, DT = DP / 32;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
+    __shared__ int odd[4];          // a wave's: a key at the border was not finite (kept here, where it takes no register from the loop)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T* gq = (T*)a.gq;
     if (blockIdx.x >= first_rest) {
@@ -818,7 +851,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq
         const int jend = seen_keys(last / a.G, sq.n, sk.n, a.causal);
         const int jall = seen_keys(r0 / a.G, sq.n, sk.n, a.causal);
         const int jwave = r0 + wave * 32 < R ? seen_keys(min(r0 + wave * 32 + 31, last) / a.G, sq.n, sk.n, a.causal) : 0;
-        bool spoilt = false;        // the row sees a key that is not finite: so is its gradient
+        if (lane == 0) odd[wave] = 0;
         GqState<T, DP, BN> st;
         const float2 stat = live ? a.stats[at] : make_float2(0.f, 0.f);
         st.base = stat.x;
@@ -888,15 +921,19 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : 2)) void k_attn_gq
             bool bad = stage<T, DP, BN, true>(lds, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
             stage<T, DP, BN, false>(lds + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
             bad = __syncthreads_or(bad);
+            if (bad) {
+                if (lane == 0) odd[wave] = 1;
+                clear_spoilt<T, DP, 256>(lds, k + (long long)k0 * a.k_st, a.k_st, min(sk.n - k0, BN), a.D);
+                __syncthreads();
+            }
             if (k0 < jwave) st.template step<true, false, GqCfg<T, DP>::FINE>(lds, lds + TB, lane, c2, jmax - k0);
-            if (bad)
-                for (int j = 0; j < min(jmax - k0, BN); ++j) spoilt |= spoils(k + (k0 + j) * a.k_st, a.D);
         }
         if (live) {
             T* o = gq + at * a.D;
-            const float mul = spoilt ? NAN : a.scale * stat.y;
+            const float mul = a.scale * stat.y;
 #pragma unroll
             for (int d = 0; d < DT; ++d) store_cols(o, st.acc[d], d, h, a.D, mul);
+            if (odd[wave]) st.add_spoilt(o, mul, (const T*)a.q + qrows.at(row), (const T*)a.go + grows.at(row), k, a.k_st, v, a.v_st, jall / BN * BN, jmax, a.D, h, c2);
         }
     }
 }
@@ -910,6 +947,21 @@ struct GkvCfg {
     static constexpr bool V_LDS = sizeof(T) * DP >= 256;
     static constexpr int WAVES = sizeof(T) * DP > 256 ? 1 : 2;         // per SIMD
 };
+
+// What the steps left out of the rows first .. end - 1, which see a key: queries and gradients of the result that are not finite, into the key's
+// gradients in memory.  st: the statistics of row 0 (rare path)
+template <typename T>
+__device__ void add_spoilt(T* gk, T* gv, const Attn& a, const Rows& qrows, const Rows& grows, const T* k, const T* v, const float* st, long long pitch, int first, int end, int h) {
+#pragma unroll 1
+    for (int r = first; r < end; ++r) {
+        const T *q = (const T*)a.q + qrows.at(r), *go = (const T*)a.go + grows.at(r);
+        const bool of_q = spoils(q, a.D);
+        if (!of_q && !spoils(go, a.D)) continue;
+        const float p = __builtin_amdgcn_exp2f(fmaf(dot(q, k, a.D), a.scale * LOG2E, -st[r])) * (sizeof(T) == 4 ? st[2 * pitch + r] : 1.f);
+        add_to_row(gv, p, go, a.D, h, true);
+        add_to_row(gk, p * (dot(go, v, a.D) - st[pitch + r]) * a.scale, q, a.D, h, false);
+    }
+}
 
 // The rows of a step (BR of them, STEP to the next) of q and go into LDS by NT threads.  EVEN: the heads of a group divide a step, so a lane's rows stay where they are
 // from step to step and only the wave's address moves.  Otherwise each lane follows its rows: a step is adv_t tokens and adv_g heads, one
@@ -994,7 +1046,6 @@ struct GkvState {
     static constexpr bool F32 = sizeof(T) == 4;
     Frag<T> kf[KS], vf[V_LDS ? 1 : KS];
     f32x16 ak[DT], av[DT];
-    bool spoilt;        // a row that is not finite sees the key: so are its gradients
 
     __device__ __forceinline__ void begin(const T* k, const T* v, bool live, int D, int h) {
 #pragma unroll
@@ -1005,7 +1056,6 @@ struct GkvState {
         }
 #pragma unroll
         for (int i = 0; i < DT; ++i) ak[i] = zero16(), av[i] = zero16();
-        spoilt = false;
     }
     template <bool MASK, bool FINE = false>
     __device__ __forceinline__ void step(const char* lq, const char* lg, const char* lvw, const float* st, int pitch, int lane, float c2, int r0, int from, int end) {
@@ -1062,6 +1112,7 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
     constexpr bool F32 = sizeof(T) == 4;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB + (C::V_LDS ? BK * L::ROWB : 0)];
     __shared__ __attribute__((aligned(1024))) float stat[2][F32 ? 3 : 2][BR];
+    __shared__ int odd[4];          // a wave's: a row at the border was not finite (kept here, where it takes no register from the loop)
     char* lvt = lds + 4 * TB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T *gk = (T*)a.gk, *gv = (T*)a.gv;
@@ -1096,6 +1147,7 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
         const int k0 = (int)kk;
         const int key = k0 + wave * 32 + (lane & 31);
         const bool live = key < sk.n;
+        if (lane == 0) odd[wave] = 0;
         GkvState<T, DP, C::V_LDS> st;
         st.begin(k + (live ? key * a.k_st : 0), v + (live ? key * a.v_st : 0), live, a.D, h);
         __syncthreads();
@@ -1122,11 +1174,8 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             }
             bool bad = stage<T, DP, BR, true>(lds, (const T*)a.q, R - r0, a.D, [&](int r) { return qrows.at(r0 + r); });
             bad |= stage<T, DP, BR, true>(lds + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
-            bad = __syncthreads_or(bad);
+            if (__syncthreads_or(bad) && lane == 0) odd[wave] = 1;
             step(std::true_type{}, 0, r0);
-            if (bad)
-                for (int r = max(r0, r_key); r < min(r0 + BR, R); ++r)
-                    st.spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
         };
         int r0 = first;
         for (; r0 < R && r0 < r_all; r0 += BR) border(r0);
@@ -1163,8 +1212,16 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             T *ok = gk + ((sk.begin + key) * a.Hk + kv) * a.D, *ov = gv + ((sk.begin + key) * a.Hk + kv) * a.D;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                store_cols(ok, st.ak[d], d, h, a.D, st.spoilt ? NAN : a.scale);
-                store_cols(ov, st.av[d], d, h, a.D, st.spoilt ? NAN : 1.f);
+                store_cols(ok, st.ak[d], d, h, a.D, a.scale);
+                store_cols(ov, st.av[d], d, h, a.D, 1.f);
+            }
+            if (odd[wave]) {
+                int again = k0;
+                asm volatile("" : "+s"(again));         // (worked out again: kept, it would take registers from the loop)
+                const int head = first_row(again), full = head + (max(first_row(min(again + BK, sk.n) - 1) - head, 0) + BR - 1) / BR * BR;
+                const int tail = full < R ? R - (R - full) % BR : R;
+                add_spoilt(ok, ov, a, qrows, grows, k + key * a.k_st, v + key * a.v_st, rowstat, all, first_row(key), min(full, R), h);
+                add_spoilt(ok, ov, a, qrows, grows, k + key * a.k_st, v + key * a.v_st, rowstat, all, max(tail, first_row(key)), R, h);
             }
         }
     }
@@ -1176,7 +1233,7 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
 template <typename T, int DP, int NW>
 struct SplitCfg {
     static constexpr int TB = 32 * DP * (int)sizeof(T), LDS = NW * 4 * TB;
-    static constexpr int WAVES = LDS / NW >= 32768 || LDS > 65536 ? 1 : 2;      // per SIMD
+    static constexpr int WAVES = LDS / NW >= 32768 || LDS > 65536 ? 1 : LDS / NW <= 8192 ? 3 : 2;       // per SIMD
 };
 
 // NW results of 32 rows x DP (lane: row) summed over the waves: each thread gets four neighbouring columns of a row
@@ -1214,7 +1271,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
     constexpr int KS = DP / 16, DT = DP / 32, TB = SplitCfg<T, DP, NW>::TB;
     __shared__ __attribute__((aligned(1024))) char lds[SplitCfg<T, DP, NW>::LDS];
     __shared__ float part[NW][32], mul[32];
-    __shared__ int bad_row[32];
+    __shared__ int odd;             // a key at the border was not finite
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T* gq = (T*)a.gq;
     if (blockIdx.x >= first_rest) {
@@ -1245,7 +1302,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
         __syncthreads();
         if (a.D < DP)
             for (int i = lane; i < 4 * TB / 16; i += 64) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
-        if (threadIdx.x < 32) bad_row[threadIdx.x] = 0;
+        if (threadIdx.x == 0) odd = 0;
         __syncthreads();
         GqState<T, DP, 32> st;
         const float2 stat = live ? a.stats[at] : make_float2(0.f, 0.f);
@@ -1257,10 +1314,10 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             st.qf[s] = frag_global((const T*)a.q + (live ? qrows.at(row) : 0) + d, on);
             st.gf[s] = frag_global((const T*)a.go + (live ? grows.at(row) : 0) + d, on);
         }
-        // a block with a mask, through registers; false: nothing in it that is not finite
-        const auto bring = [&](int k0) {
+        // a block with a mask, through registers; checked: whether there is a key in it that is not finite
+        const auto bring = [&](auto checked, int k0) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            const bool bad = stage<T, DP, 32, true, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
+            const bool bad = stage<T, DP, 32, decltype(checked)::value, 64>(mine, k + (long long)k0 * a.k_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.k_st; });
             stage<T, DP, 32, false, 64>(mine + TB, v + (long long)k0 * a.v_st, sk.n - k0, a.D, [&](int r) { return (long long)r * a.v_st; });
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             return __any(bad);
@@ -1269,7 +1326,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
         if (jend <= EXACT_D) {
             st.delta = st.sum = 0.f;
             for (int k0 = wave * 32; k0 < jend; k0 += NW * 32) {
-                bring(k0);
+                bring(std::false_type{}, k0);
                 st.template step<true, true>(mine, mine + TB, lane, c2, jmax - k0);
             }
             delta = st.sum + __shfl_xor(st.sum, 32, 64);
@@ -1307,7 +1364,6 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
 #pragma unroll
         for (int i = 0; i < DT; ++i) st.acc[i] = zero16();
         const int full = jall / 32;
-        bool spoilt = false;
         int blk = wave, buf = 0;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (blk < full) {
@@ -1329,18 +1385,24 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             st.template step<false, false, true>(now, now + TB, lane, c2, 32);
         }
         for (; blk * 32 < jend; blk += NW) {
-            const bool bad = bring(blk * 32);
+            if (bring(std::true_type{}, blk * 32)) {
+                odd = 1;
+                clear_spoilt<T, DP, 64>(mine, k + (long long)blk * 32 * a.k_st, a.k_st, min(sk.n - blk * 32, 32), a.D);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
             st.template step<true, false, true>(mine, mine + TB, lane, c2, jmax - blk * 32);
-            if (bad)
-                for (int j = 0; j < min(jmax - blk * 32, 32); ++j) spoilt |= spoils(k + (blk * 32 + j) * a.k_st, a.D);
         }
-        if (spoilt) bad_row[lane & 31] = 1;
         if (wave == 0 && h == 0) mul[lane & 31] = a.scale * stat.y;
         over_waves<T, DP, NW>(reinterpret_cast<float*>(lds), st.acc, lane, wave, a.D, [&](int r, int d, const float4& o) {
             if (r0 + r >= R) return;
             const int t = (r0 + r) / a.G;
-            store4(gq + ((sq.begin + t) * a.Hq + kv * a.G + (r0 + r - t * a.G)) * a.D + d, o, bad_row[r] ? NAN : mul[r]);
+            store4(gq + ((sq.begin + t) * a.Hq + kv * a.G + (r0 + r - t * a.G)) * a.D + d, o, mul[r]);
         });
+        if (odd) {          // (read behind the barriers of over_waves)
+            __syncthreads();
+            if (wave == 0 && live)
+                st.add_spoilt(gq + at * a.D, a.scale * stat.y, (const T*)a.q + qrows.at(row), (const T*)a.go + grows.at(row), k, a.k_st, v, a.v_st, full * 32, jmax, a.D, h, c2);
+        }
     }
 }
 
@@ -1351,7 +1413,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
     constexpr int NS = F32 ? 3 : 2;
     __shared__ __attribute__((aligned(1024))) char lds[SplitCfg<T, DP, NW>::LDS];
     __shared__ __attribute__((aligned(1024))) float stat[NW][2][NS][32];
-    __shared__ int bad_key[32];
+    __shared__ int odd;             // a row at the border was not finite
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     T *gk = (T*)a.gk, *gv = (T*)a.gv;
     if (blockIdx.x >= first_rest) {
@@ -1384,7 +1446,7 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
         __syncthreads();
         if (a.D < DP)
             for (int i = lane; i < 4 * TB / 16; i += 64) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
-        if (threadIdx.x < 32) bad_key[threadIdx.x] = 0;
+        if (threadIdx.x == 0) odd = 0;
         __syncthreads();
         GkvState<T, DP, false> st;
         st.begin(k + (live ? key * a.k_st : 0), v + (live ? key * a.v_st : 0), live, a.D, h);
@@ -1393,8 +1455,9 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             return (t < 0 ? 0 : t > sq.n ? sq.n : (int)t) * a.G;
         };
         const int first = first_row(k0), r_all = first_row(min(k0 + 32, sk.n) - 1), r_key = live ? first_row(key) : R;
-        // steps of 32 rows from `first`: those below `lo` and the last one, if it is short, need a mask
-        const int steps = R > first ? (R - first + 31) / 32 : 0, lo = min((r_all - first + 31) / 32, steps), hi = max(lo, R > first ? (R - first) / 32 : 0);
+        // steps of 32 rows from `first`: those below `lo` and the last one, if it is short, need a mask.  One wave takes all of them that way: it
+        // has two at most, and with FINE an infinity in go that a weight's rest multiplies would come out as NaN
+        const int steps = R > first ? (R - first + 31) / 32 : 0, lo = NW == 1 ? steps : min((r_all - first + 31) / 32, steps), hi = max(lo, R > first ? (R - first) / 32 : 0);
         const auto border = [&](int s) {
             const int r0 = first + s * 32;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1407,13 +1470,11 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             bad |= stage<T, DP, 32, true, 64>(mine + TB, (const T*)a.go, R - r0, a.D, [&](int r) { return grows.at(r0 + r); });
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             st.template step<true, NW == 1>(mine, mine + TB, nullptr, &stat[wave][0][0][0], 32, lane, c2, r0, r_key, R);
-            if (__any(bad))
-                for (int r = max(r0, r_key); r < min(r0 + 32, R); ++r)
-                    st.spoilt |= spoils((const T*)a.q + qrows.at(r), a.D) || spoils((const T*)a.go + grows.at(r), a.D);
+            if (__any(bad)) odd = 1;
         };
         int s = wave;
         for (; s < lo; s += NW) border(s);
-        if (s < hi) {
+        if (NW > 1 && s < hi) {
             RowDma<T, DP, 32, EVEN, 64, NW * 32> dma(q0, g0, a, first + s * 32);
             const auto load = [&](unsigned to, unsigned st_to, int r0) {
                 dma.load(to, to + TB);
@@ -1439,14 +1500,21 @@ __global__ __launch_bounds__((NW * 64), (SplitCfg<T, DP, NW>::WAVES)) void k_att
             }
         }
         for (; s < steps; s += NW) border(s);
-        if (st.spoilt) bad_key[lane & 31] = 1;
         float* pool = reinterpret_cast<float*>(lds);
         over_waves<T, DP, NW>(pool, st.ak, lane, wave, a.D, [&](int r, int d, const float4& o) {
-            if (k0 + r < sk.n) store4(gk + ((sk.begin + k0 + r) * a.Hk + kv) * a.D + d, o, bad_key[r] ? NAN : a.scale);
+            if (k0 + r < sk.n) store4(gk + ((sk.begin + k0 + r) * a.Hk + kv) * a.D + d, o, a.scale);
         });
         over_waves<T, DP, NW>(pool, st.av, lane, wave, a.D, [&](int r, int d, const float4& o) {
-            if (k0 + r < sk.n) store4(gv + ((sk.begin + k0 + r) * a.Hk + kv) * a.D + d, o, bad_key[r] ? NAN : 1.f);
+            if (k0 + r < sk.n) store4(gv + ((sk.begin + k0 + r) * a.Hk + kv) * a.D + d, o, 1.f);
         });
+        if (odd) {          // (read behind the barriers of over_waves)
+            __syncthreads();
+            if (wave == 0 && live) {
+                T *ok = gk + ((sk.begin + key) * a.Hk + kv) * a.D, *ov = gv + ((sk.begin + key) * a.Hk + kv) * a.D;
+                add_spoilt(ok, ov, a, qrows, grows, k + key * a.k_st, v + key * a.v_st, rowstat, all, r_key, min(first + lo * 32, R), h);
+                add_spoilt(ok, ov, a, qrows, grows, k + key * a.k_st, v + key * a.v_st, rowstat, all, max(first + hi * 32, r_key), R, h);
+            }
+        }
     }
 }
 

@@ -148,3 +148,77 @@ def test_a_row_whose_scores_are_all_minus_infinity_is_not_one_that_sees_no_key(n
     gq, gk, gv = torch.autograd.grad(out, leaves, go)
     assert gq[2, 1].isnan().all() and gk[:nk].isnan().all() and gv[:nk].isnan().all()
     assert torch.isfinite(gq[2, 0]).all() and not gq[3:5].any() and torch.isfinite(gq[5:]).all() and torch.isfinite(gk[nk:]).all() and torch.isfinite(gv[nk:]).all()
+
+
+def ieee_ref(q, k, v, go, lq, lk, dtype):
+    """out and the gradients by the formulas in 64 bits, row by row over the keys that it sees, as infinities and NaN come out of them; and what
+    their finite elements may be off by.  A score is a sum of d products (fp32), so a weight is off by 2 E of itself with E = (d + 8) F times
+    the largest sum of |q k|, and once more by its rounding, u; dS = p (go v - D) by those, by D's (the rounded out, u, and the weights') and by a
+    rounding of its own; the results by theirs, and by F for each row or key that is summed: 5 u + 5 E and less of the sum of absolute terms."""
+    hq, hk, d = q.shape[1], k.shape[1], q.shape[2]
+    c = d ** -0.5
+    zero = lambda t: torch.zeros_like(t)      # noqa: E731
+    got, size = [zero(t) for t in (q, q, k, v)], [zero(t) for t in (q, q, k, v)]
+    fin = lambda t: torch.where(torch.isfinite(t), t, 0.0).abs()      # noqa: E731
+    a = b = 0
+    most = 0.0
+    for m, n in zip(lq, lk):
+        for i in range(m):
+            seen = min(max(i + 1 + n - m, 0), n)
+            if seen == 0:
+                continue
+            for h in range(hq):
+                kh = h // (hq // hk)
+                K, V, Q, G = k[b:b + seen, kh], v[b:b + seen, kh], q[a + i, h], go[a + i, h]
+                s = (K * Q).sum(1) * c
+                most = max(most, ((fin(K) * fin(Q)).sum(1) * c).max().item())
+                e = (s - s.max()).exp()
+                p = e / e.sum()
+                o = (p[:, None] * V).sum(0)
+                ds = p * ((V * G).sum(1) - (G * o).sum())
+                P = fin(p)
+                O = (P[:, None] * fin(V)).sum(0)
+                S = P * ((fin(V) * fin(G)).sum(1) + (fin(G) * O).sum())
+                for t, (ro, rq, rk, rv) in ((got, (o, (ds[:, None] * K).sum(0) * c, ds[:, None] * Q * c, p[:, None] * G)),
+                                            (size, (O, (S[:, None] * fin(K)).sum(0) * c, S[:, None] * fin(Q) * c, P[:, None] * fin(G)))):
+                    t[0][a + i, h], t[1][a + i, h] = ro, rq
+                    t[2][b:b + seen, kh] += rk
+                    t[3][b:b + seen, kh] += rv
+        a, b = a + m, b + n
+    E = (d + 8 + max(lq) * (hq // hk) + max(lk)) * 2.0 ** -24 * (1 + most)
+    return got, [(5 * unit(dtype) + 5 * E) * t for t in size]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("lq,lk,hq,hk,d,more", [([9], [9], 2, 1, 64, 0), ([40], [40], 2, 2, 32, 0), ([50], [90], 2, 1, 128, 0), ([3, 1], [140, 70], 4, 2, 64, 0),
+                                                ([150], [150], 2, 2, 64, 0), ([150], [200], 1, 1, 128, 300), ([140], [140], 3, 1, 32, 300)])
+@pytest.mark.parametrize("which", ["q", "k", "v", "go"])
+def test_what_is_not_finite_reaches_what_the_formulas_say(which, lq, lk, hq, hk, d, more, dtype):
+    """One infinity in a query, key, value or gradient: each element of the results is finite where the formulas' is, and right there; the others
+    are infinite or NaN as theirs are, wherever the borders of blocks lie (a value's infinity and gv's keep their sign; D, the sum of infinities
+    in another order, decides between the two in gq and gk)."""
+    g = gen(d)
+    tq, tk = sum(lq), sum(lk)
+    q, go = rand(g, tq + 20 * more, hq, d, dtype=dtype), rand(g, tq + 20 * more, hq, d, dtype=dtype)
+    k, v = rand(g, tk + 20 * more, hk, d, dtype=dtype), rand(g, tk + 20 * more, hk, d, dtype=dtype)
+    q[:tq, :, 5] = q[:tq, :, 5].abs() + 0.125           # an infinite k is +-inf in all scores
+    cu_q, cu_k = ends(lq + [20] * more), ends(lk + [20] * more)
+    for at in {0, 1, lk[0] // 2, lk[0] - 1}:
+        for value in (math.inf, -math.inf):
+            t = dict(q=q.clone(), k=k.clone(), v=v.clone(), go=go.clone())
+            row = min(at, lq[0] - 1) if which in ("q", "go") else at
+            t[which][row, 0, 5] = value
+            want, tol = ieee_ref(t["q"][:tq], t["k"][:tk], t["v"][:tk], t["go"][:tq], lq, lk, dtype)
+            leaves = [t[n].to("cuda", dtype).requires_grad_(True) for n in ("q", "k", "v")]
+            out = sequence.packed_attention(*leaves, cu_q, cu_k, max_q=max(lq + [20]), max_k=max(lk + [20]))
+            got = (out,) + torch.autograd.grad(out, leaves, t["go"].to("cuda", dtype))
+            for name, x, y, most in zip(("out", "gq", "gk", "gv"), got, want, tol):
+                x, what = x.detach().cpu().double(), (which, at, value, name)
+                assert torch.isfinite(x[len(y):]).all(), what
+                x, fin = x[:len(y)], torch.isfinite(y)
+                assert torch.equal(torch.isfinite(x), fin), what
+                if name in ("out", "gv"):
+                    assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x[~fin].nan_to_num(), y[~fin].nan_to_num()), what
+                off = (x - y)[fin].abs() - most[fin]
+                assert (off <= 0).all(), (what, off.max().item())
