@@ -1215,7 +1215,7 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
                 store_cols(ok, st.ak[d], d, h, a.D, a.scale);
                 store_cols(ov, st.av[d], d, h, a.D, 1.f);
             }
-            if (odd[wave]) {
+            if (__builtin_expect(odd[wave], 0)) {
                 int again = k0;
                 asm volatile("" : "+s"(again));         // (worked out again: kept, it would take registers from the loop)
                 const int head = first_row(again), full = head + (max(first_row(min(again + BK, sk.n) - 1) - head, 0) + BR - 1) / BR * BR;
