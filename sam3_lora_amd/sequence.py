@@ -20,6 +20,7 @@ from functools import lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _ffi
@@ -52,6 +53,13 @@ def _activation(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None)
     if not t.is_cuda:
         raise LoRAKernelError(f"sam3_lora_amd: the sequence operators run only on an AMD GPU (got a {t.device} tensor for {name}); "
                               "there is no CPU fallback.")
+
+
+def _recorded(a: torch.Tensor, b: Optional[torch.Tensor], c: Optional[torch.Tensor] = None) -> bool:
+    """Whether a call has to be made through its autograd function: a gradient is recorded; or derivatives run forward, which these functions
+    do not have and say so; or the call is traced, and would not be seen otherwise."""
+    return (torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad))) \
+        or forward_ad._current_level >= 0 or torch._C._is_tracing()
 
 
 _HERE = contextlib.nullcontext()
@@ -200,7 +208,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     The statistics and y come from the unrounded fp32 h.  Differentiable in x, residual and weight.
     """
     _norm_args(x, weight, residual, eps)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+    if _recorded(x, weight, residual):
         return _RMSNorm.apply(x, residual, weight, eps)
     y, h, _, _, _, _ = _norm_fwd(x, residual, weight, eps, True, False)
     return y if residual is None else (y, h)
@@ -220,8 +228,8 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
         raise ValueError(f"fmt must be FP8_E4M3 or FP8_E5M2, got {fmt}")
     if group != 0 and (group not in (32, 64, 128) or x.shape[-1] % group):
         raise ValueError(f"group must be 0, or 32, 64 or 128 and divide {x.shape[-1]}, got {group}")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        raise ValueError("rms_norm_q8 has no gradient: call it under torch.no_grad(), or rms_norm for training")
+    if _recorded(x, weight, residual):
+        raise ValueError("rms_norm_q8 has no gradient and no traced form: call it under torch.no_grad(), or rms_norm for training")
     _, h, _, _, image, scales = _norm_fwd(x, residual, weight, eps, False, False, (group, fmt))
     return (image, scales) if residual is None else (image, scales, h)
 
@@ -327,7 +335,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     if positions.requires_grad:
         raise ValueError("positions have no gradient")
     halves = pairing == "halves"
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _recorded(q, k):
         return _RotaryAxes.apply(q, k, positions, table, halves)
     qo, ko = _rotate(q, k, positions, table, halves, False)
     return qo if k is None else (qo, ko)
@@ -450,9 +458,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _recorded(q, k, v):
         if len_k is not None:
-            raise ValueError("len_k has no gradient: call packed_attention under torch.no_grad()")
+            raise ValueError("len_k has no gradient and no traced form: call packed_attention under torch.no_grad()")
         out, lse = _PackedAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, bool(causal), scale, return_lse)
     else:
         out, lse, _, _, _ = _attn_fwd(q, k, v, cu_q, cu_k, len_k, max_q, max_k, bool(causal), scale, return_lse)

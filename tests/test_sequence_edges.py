@@ -222,3 +222,50 @@ def test_what_is_not_finite_reaches_what_the_formulas_say(which, lq, lk, hq, hk,
                     assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x[~fin].nan_to_num(), y[~fin].nan_to_num()), what
                 off = (x - y)[fin].abs() - most[fin]
                 assert (off <= 0).all(), (what, off.max().item())
+
+
+# ------------------------------------------------------------------------------------------- derivatives that do not exist
+def operator_calls():
+    g = gen(4)
+    x, w = torch.randn(12, 64, generator=g).cuda(), torch.randn(64, generator=g).cuda()
+    q, k, v = (torch.randn(12, 2, 32, generator=g).cuda() for _ in range(3))
+    pos, cu = torch.arange(12, device="cuda", dtype=torch.float32)[None], ends([5, 7])
+    return {"norm": (lambda *t: sequence.rms_norm(t[0], t[1], residual=t[2]), (x, w, x * 2)), "norm alone": (sequence.rms_norm, (x, w)),
+            "rotary": (lambda *t: sequence.rotary_axes(t[0], t[1], t[2], (16,)), (q, k, pos)),
+            "attention": (lambda *t: sequence.packed_attention(*t, cu), (q, k, v)),
+            "lse": (lambda *t: sequence.packed_attention(*t, cu, return_lse=True), (q, k, v))}
+
+
+@pytest.mark.gpu
+def test_forward_derivatives_are_refused():
+    """A dual tensor does not require a gradient; without its tangent the result would count as constant."""
+    from torch.autograd import forward_ad
+    for name, (call, args) in operator_calls().items():
+        plain = call(*args)
+        with forward_ad.dual_level():
+            same = call(*args)              # nothing is dual
+            assert all(torch.equal(a, b) for a, b in zip(*((t,) if torch.is_tensor(t) else t for t in (plain, same)))), name
+            for i, t in enumerate(args):
+                dual = list(args)
+                dual[i] = forward_ad.make_dual(t, torch.ones_like(t))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises((NotImplementedError, RuntimeError)):
+                        call(*dual)
+    x, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    with forward_ad.dual_level(), torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+        sequence.rms_norm_q8(forward_ad.make_dual(x, x), w)
+
+
+@pytest.mark.gpu
+def test_traced_calls_are_calls():
+    """A trace holds the call, not the result of its example inputs."""
+    for name, (call, args) in operator_calls().items():
+        with torch.no_grad():
+            traced = torch.jit.trace(call, args, check_trace=False)
+        other = [t.flip(0) * 1.25 for t in args]
+        got, want = traced(*other), call(*other)
+        for a, b in zip(*((t,) if torch.is_tensor(t) else t for t in (got, want))):
+            assert torch.equal(a, b), name
+    x, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    with torch.no_grad(), pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(lambda x: sequence.rms_norm_q8(x, w)[1], (x,), check_trace=False)
