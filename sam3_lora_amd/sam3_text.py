@@ -171,6 +171,14 @@ class LayerScale(nn.Module):
         return x.mul_(self.gamma) if self.inplace else x * self.gamma
 
 
+def _as_written(m: nn.Module, cls: type) -> bool:
+    """Whether calling ``m`` is ``cls.forward`` and nothing else: no other forward, and no hook that code going round the call would miss."""
+    g = torch.nn.modules.module
+    return (type(m).forward is cls.forward and "forward" not in m.__dict__
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+            and not (g._global_forward_hooks or g._global_forward_pre_hooks or g._global_backward_hooks or g._global_backward_pre_hooks))
+
+
 class ResidualAttentionBlock(nn.Module):
     """Pre-norm block ``x += attn(ln_1(x)); x += mlp(ln_2(x))`` with ``nn.MultiheadAttention(batch_first=True)`` and
     the MLP ``c_fc -> GELU -> c_proj`` (text_encoder_ve.py:13-88)."""
@@ -208,9 +216,11 @@ class ResidualAttentionBlock(nn.Module):
         return x + self.ls_2(self.mlp(self.ln_2(x)))
 
     def packs(self) -> bool:
-        """Whether :meth:`forward_packed` computes what :meth:`forward` does."""
+        """Whether :meth:`forward_packed` computes what calling the block does."""
+        from .sam3_detr import MultiheadAttention
         a = self.attn
-        return (a._qkv_same_embed_dim and a.bias_k is None and not a.add_zero_attn and a.in_proj_bias is not None
+        return (_as_written(self, ResidualAttentionBlock) and _as_written(a, MultiheadAttention)
+                and a._qkv_same_embed_dim and a.bias_k is None and not a.add_zero_attn and a.in_proj_bias is not None
                 and not (a.dropout > 0 and self.training) and a.head_dim % 8 == 0 and a.head_dim <= 128
                 and a.in_proj_weight.dtype in (torch.bfloat16, torch.float32) and not torch.is_autocast_enabled("cuda"))
 
@@ -308,7 +318,8 @@ class TextTransformer(nn.Module):
         return x.new_zeros(B * L, x.shape[-1]).index_copy(0, at, x).view(B, L, -1)
 
     def packs(self) -> bool:
-        return self.attn_mask is not None and self.pool_type == "none" and all(b.packs() for b in self.transformer.resblocks)
+        return (self.attn_mask is not None and self.pool_type == "none" and _as_written(self, TextTransformer)
+                and _as_written(self.transformer, Transformer) and all(b.packs() for b in self.transformer.resblocks))
 
 
 class VETextEncoder(nn.Module):
@@ -317,7 +328,8 @@ class VETextEncoder(nn.Module):
 
     ``packed`` (off by default, :func:`set_packed_text`): on a GPU the tower runs on the prompts' own tokens, one prompt behind the other
     (``sequence.packed_attention``), instead of on ``context_length`` tokens each; memory and mask come out as before, except that the
-    memory's rows under the mask hold the resizer's bias."""
+    memory's rows under the mask hold the resizer's bias.  Where that form would miss something -- autocast, dropout of the attention's
+    weights, hooks on the encoder, its transformer, a block or its attention, or other modules in their place -- the padded form runs."""
 
     packed = False
 

@@ -269,3 +269,52 @@ def test_traced_calls_are_calls():
     x, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
     with torch.no_grad(), pytest.raises(ValueError, match="traced"):
         torch.jit.trace(lambda x: sequence.rms_norm_q8(x, w)[1], (x,), check_trace=False)
+
+
+# --------------------------------------------------------------------------------------------------- packed text tower
+def test_the_packed_tower_steps_back_where_it_would_miss_something():
+    """Hooks of the modules that the packed form goes round, another forward, or another module in an attention's place."""
+    import torch.nn as nn
+    from test_sequence import tower
+    enc = tower("cpu", torch.float32).encoder
+    assert enc.packs()
+    blk = enc.transformer.resblocks[1]
+    for m in (enc, enc.transformer, blk, blk.attn):
+        for register in (m.register_forward_hook, m.register_forward_pre_hook, m.register_full_backward_hook, m.register_full_backward_pre_hook):
+            handle = register(lambda *a: None)
+            assert not enc.packs()
+            handle.remove()
+            assert enc.packs()
+        m.forward = m.forward
+        assert not enc.packs()
+        del m.forward
+        assert enc.packs()
+    for register in (nn.modules.module.register_module_forward_hook, nn.modules.module.register_module_full_backward_hook):
+        handle = register(lambda *a: None)
+        assert not enc.packs()
+        handle.remove()
+        assert enc.packs()
+    blk.ln_1.register_forward_hook(lambda *a: None)         # these are called either way
+    blk.mlp.c_fc.register_forward_hook(lambda *a: None)
+    assert enc.packs()
+    stock = blk.attn
+    blk.attn = nn.MultiheadAttention(128, 4, batch_first=True)
+    assert not enc.packs()
+    blk.attn = nn.Identity()
+    assert not enc.packs()
+    blk.attn = stock
+    assert enc.packs()
+
+
+@pytest.mark.gpu
+def test_hooks_see_the_tower_with_the_packed_switch_on():
+    from sam3_lora_amd.sam3_text import set_packed_text
+    from test_sequence import PROMPTS, tower
+    enc = tower("cuda", torch.float32).eval()
+    seen = []
+    enc.encoder.transformer.resblocks[2].attn.register_forward_hook(lambda m, args, out: seen.append(out[0].shape))
+    with torch.no_grad():
+        want = enc(PROMPTS, device="cuda")
+        set_packed_text(enc)
+        got = enc(PROMPTS, device="cuda")
+    assert len(seen) == 2 and seen[0] == seen[1] and all(torch.equal(a, b) for a, b in zip(got, want))
