@@ -1604,6 +1604,9 @@ Plan plan(int64_t Tq, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
     int64_t chunk = keys / 1024 < 1024 ? keys / 1024 : 1024;
     if (chunk < 256) chunk = 256;
     if (chunk < keys / 8192) chunk = keys / 8192;
+    // The chunks' results take room for every row of q there is, sequence or not: no more of them than 2 GiB hold (8192 waves of 32 rows have 136 MB)
+    const int64_t fit = (1ll << 31) / (Tq * Hq * (128 * 4 + 8) + 1), most = fit > 1 ? fit : 1;
+    if (chunk * most < max_k) chunk = (max_k + most - 1) / most;
     chunk = (chunk + 127) / 128 * 128;
     p.chunk = (int)(chunk > 0x40000000 ? 0x40000000 : chunk);
     p.splits = (int)((max_k + p.chunk - 1) / p.chunk);

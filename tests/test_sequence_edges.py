@@ -41,6 +41,30 @@ def test_launches_that_do_not_exist_are_refused():
     assert lib.sam3_seq_attn_bwd(*([p, 8192, 8] * 4), p, p, p, p, p, p, p, 130000, 130000, 65000, 1024, 1024, 8, 130000, 130000, 1, 0.1, 0, p, 1 << 40, None) == -95
 
 
+def test_chunks_of_keys_take_a_bounded_workspace():
+    """The chunks' results have room for every row of q: with a hint that is too small, or room behind the sequences, no more than 2 GiB."""
+    need = _ffi.load().sam3_seq_attn_fwd_workspace_bytes
+    for tq, b, hq, hk, max_q, max_k in ((1 << 20, 1, 32, 8, 1, 1 << 20), (8192, 64, 32, 8, 1, 32768), (1 << 22, 1, 8, 8, 4, 1 << 30), (65536, 24, 32, 8, 1, 1 << 17)):
+        for d in (8, 64, 128):
+            assert need(tq, b, hq, hk, d, max_q, max_k, 0) <= 1 << 31, (tq, d)
+    assert need(24, 24, 32, 8, 128, 1, 32768, 0) == 24 * 32 * 520 * 32        # (chunks of 1024 keys, as without the bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+def test_one_token_each_in_a_buffer_with_very_much_room(dtype):
+    g = gen(6)
+    lk = [3000, 1, 700]
+    q = torch.zeros(200_000, 8, 64, device="cuda", dtype=dtype)
+    q[:3] = rand(g, 3, 8, 64, dtype=dtype)
+    k, v = (rand(g, sum(lk), 2, 64, dtype=dtype).to("cuda", dtype) for _ in range(2))
+    cu_q, cu_k = ends([1] * 3), ends(lk)
+    out = sequence.packed_attention(q, k, v, cu_q, cu_k, max_q=1, max_k=3000)
+    ref = attn_ref(q[:3].cpu().double(), k.cpu().double(), v.cpu().double(), [1] * 3, lk, True, 0.125, unit(dtype))
+    close(out[:3], ref["o"], ref["to"], "out")
+    assert not out[3:].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DT, ids=ids)
 @pytest.mark.parametrize("lens,hq,hk,d,causal", [([3, 0, 20, 7, 1, 0, 33, 12] * 150, 4, 2, 32, True), ([5] * 600 + [700] + [2] * 600, 14, 2, 64, True),
