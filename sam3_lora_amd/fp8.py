@@ -134,9 +134,11 @@ def fp8_linear(x2: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -> 
 
 
 def fp8_linear_q(xq: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -> torch.Tensor:
-    """:func:`fp8_linear` on an input its producer already wrote as e4m3 (``xq`` with scale ``sx``)."""
+    """:func:`fp8_linear` on an input its producer already wrote as e4m3 (``xq`` with scale ``sx``: one, or [rows, 1], one for each row, as
+    ``sequence.rms_norm_q8`` writes them)."""
     st = state_for(w)
-    return torch._scaled_mm(xq, st.wq.t(), scale_a=sx, scale_b=st.scale, bias=b, out_dtype=torch.bfloat16)
+    scale_b = st.scale if sx.numel() == 1 else st.scale.expand(1, w.shape[0]).contiguous()      # (the GEMM wants both in the same form)
+    return torch._scaled_mm(xq, st.wq.t(), scale_a=sx, scale_b=scale_b, bias=b, out_dtype=torch.bfloat16)
 
 
 def fp8_dx_q(gq: torch.Tensor, sg: torch.Tensor, w: torch.Tensor) -> torch.Tensor:

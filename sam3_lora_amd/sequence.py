@@ -3,7 +3,7 @@ Sequence operators around the adapted Linears: the norm, rotary positions and at
 images or video, as hand-written HIP kernels (C-ABI ``include/sam3_seq_amd.h``, ``csrc/seq_rows.hip``, ``csrc/seq_attention.hip``).
 
   rms_norm, rms_norm_q8   root-mean-square norm with the residual's addition, differentiable; the same with an 8-bit output and
-                          its scales in front of a frozen 8-bit GEMM (the counterparts of ``vit.layer_norm`` and its fp8 image)
+                          its scales (the counterparts of ``vit.layer_norm`` and its fp8 image), which ``fp8.fp8_linear_q`` multiplies
   rotary_axes             rotary positions with several axes (time, height, width, ...) on q and k, differentiable (the general
                           form of the trunk's 2-D tables, ``vit.axial_rope_table``)
   packed_attention        attention over packed sequences of different lengths, causal or not, with grouped heads, differentiable;
@@ -216,7 +216,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
 
 def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6, group: int = 0,
                 fmt: int = FP8_E4M3):
-    """:func:`rms_norm` with an 8-bit output for a frozen 8-bit GEMM: ``(image, scales)``, or ``(image, scales, h)`` with a residual.
+    """:func:`rms_norm` with an 8-bit output: ``(image, scales)``, or ``(image, scales, h)`` with a residual.  With one scale for a row,
+    ``fp8.fp8_linear_q(image, scales, w, b)`` (rows of a 2-D e4m3 image) is the frozen Linear behind it; scales of groups are for a product that
+    applies them group by group, which this package has not.
 
     image: [..., C] ``float8_e4m3fn`` (``fmt=FP8_E5M2``: ``float8_e5m2``) of ``y / scale``; scales: fp32 [..., 1], or [..., C / group] with one
     scale for every ``group`` (32, 64 or 128, a divisor of C) neighbouring columns.  A scale is the largest ``|y|`` of its part, at

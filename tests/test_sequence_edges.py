@@ -342,3 +342,25 @@ def test_hooks_see_the_tower_with_the_packed_switch_on():
         set_packed_text(enc)
         got = enc(PROMPTS, device="cuda")
     assert len(seen) == 2 and seen[0] == seen[1] and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ the 8-bit image multiplied
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,out,bias", [(1, 128, 64, True), (37, 1024, 256, True), (300, 512, 4096, False)])
+def test_the_frozen_linear_takes_the_norms_image(rows, width, out, bias):
+    """image x scales times the frozen weight's own image: products of 8-bit numbers are exact in fp32, their sum is off by (width + 1) F of the
+    absolute terms, the scales and the bias by a few F, the result by one rounding to bf16."""
+    from sam3_lora_amd import fp8
+    g = gen(width)
+    x, r = (rand(g, rows, width, dtype=torch.bfloat16, scale=s).to("cuda", torch.bfloat16) for s in (1, 3))
+    weight = (rand(g, width, dtype=torch.bfloat16, scale=0.2) + 1).to("cuda", torch.bfloat16)
+    w = rand(g, out, width, dtype=torch.bfloat16, scale=width ** -0.5).to("cuda", torch.bfloat16)
+    b = rand(g, out, dtype=torch.bfloat16).to("cuda", torch.bfloat16) if bias else None
+    with torch.no_grad():
+        image, scales, h = sequence.rms_norm_q8(x, weight, residual=r)
+        y = fp8.fp8_linear_q(image, scales, w, b)
+    st = fp8.state_for(w)
+    a, c = image.float().double() * scales.double(), st.wq.float().double() * st.scale.double()
+    want = a @ c.t() + (0 if b is None else b.double())
+    terms = a.abs() @ c.t().abs() + (0 if b is None else b.double().abs())
+    close(y, want.cpu(), (unit(torch.bfloat16) * want.abs() + (width + 8) * 2.0 ** -24 * terms).cpu(), "y")
