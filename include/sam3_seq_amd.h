@@ -47,7 +47,8 @@ int sam3_seq_rms_norm_bwd(const void* gy, const void* gh, const void* h, int64_t
  *   halves 0: pair i is elements (2i, 2i + 1);  1: elements (i, i + pairs).
  *   positions [axes, T] with strides (axis, token) in elements; pos_type 0 = int32, 1 = int64, 2 = fp32.
  *   axis, turns: HOST arrays of `pairs` entries, read before the call returns.
- * inverse != 0 turns the other way: the gradient of the rotation.  Angles are reduced in 64 bits.  D % 8 == 0.
+ * inverse != 0 turns the other way: the gradient of the rotation.  Angles are reduced in 64 bits (turns is: the result is good to
+ * fp32 at positions up to 2^30).  D % 8 == 0.
  */
 int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* q_out, void* k_out,
                     const void* positions, int64_t pos_sa, int64_t pos_st, int pos_type, int axes, const double* turns,

@@ -392,8 +392,9 @@ bool bad_pitch(int64_t ld, int dtype) { return (ld % (dtype == 0 ? 8 : 4)) != 0;
 
 // ------------------------------------------------------------------------------------------------- rotary positions
 // A workgroup takes TT tokens: their angles (one per token and pair, shared by all heads of q and k) are reduced in 64 bits to a
-// fraction of a turn -- exact to 2^-24 of a turn at any position -- and put into LDS as (cos, sin); then the threads walk the
-// tokens' chunks of 16 bytes (bf16), q's heads and k's in one row.
+// fraction of a turn and put into LDS as (cos, sin); then the threads walk the tokens' chunks of 16 bytes (bf16), q's heads and k's in one
+// row.  A rate is off by 2^-52 of itself or so, and with it the turns by 2^-54 of the position: 2^-24 of a turn, what fp32 holds of the
+// fraction, up to positions of 2^30, and in proportion more behind them (2^-14 at 2^40).
 struct RopeTable {
     double turns[128];
     unsigned char axis[128];

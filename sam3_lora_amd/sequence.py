@@ -313,7 +313,8 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     spectrum: ``"shared"``: pair i of n in all turns by ``theta ** (-i / n)`` per step, whatever its axis; ``"per_axis"``: each axis
     starts its own spectrum (``vit.axial_rope_table`` is ``sections=(D/4, D/4)``, per axis).
     pairing: ``"adjacent"``: elements (2i, 2i + 1), the trunk's convention; ``"halves"``: elements (i, i + n).
-    Angles are reduced in 64 bits, so far positions keep their precision.  Differentiable in q and k.
+    Angles are reduced in 64 bits: they are good to fp32 at positions up to 2^30, and off by 2^-54 of a turn times the position behind that.
+    Differentiable in q and k.
     """
     _activation("q", q)
     if q.dim() < 2 or not 0 < q.shape[-1] <= 256 or q.shape[-1] % 8:

@@ -364,3 +364,24 @@ def test_the_frozen_linear_takes_the_norms_image(rows, width, out, bias):
     want = a @ c.t() + (0 if b is None else b.double())
     terms = a.abs() @ c.t().abs() + (0 if b is None else b.double().abs())
     close(y, want.cpu(), (unit(torch.bfloat16) * want.abs() + (width + 8) * 2.0 ** -24 * terms).cpu(), "y")
+
+
+# ------------------------------------------------------------------------------------------------------- far positions
+@pytest.mark.gpu
+def test_angles_of_far_positions_against_fifty_digits():
+    """Up to 2^30 an angle is off by 2^-24 of a turn, and by the fp32 functions (a rounding of half a turn's fraction, 2 ulp) behind that; at 2^40
+    by 2^-14 of a turn."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = 60
+    pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+    positions = [0, 1, -5, 12345, (1 << 20) + 7, (1 << 30) - 1, -(1 << 30) + 3, (1 << 29) + 12345, (1 << 40) - 9, 10 ** 12]
+    pairs = 16
+    q = torch.zeros(len(positions), 1, 2 * pairs, device="cuda")
+    q[..., 0::2] = 1.0
+    got = sequence.rotary_axes(q, None, torch.tensor([positions], device="cuda"), (pairs,))[:, 0].cpu().double()
+    for t, pos in enumerate(positions):
+        for i in range(pairs):
+            turns = Decimal(pos) * (Decimal(10000).ln() * Decimal(-i) / Decimal(pairs)).exp() / (2 * pi)
+            angle = 2 * math.pi * float(turns - turns.to_integral_value())
+            tol = 2 * math.pi * 2.0 ** -24 * max(1.0, abs(pos) / 2.0 ** 30) + (math.pi / 2 + 4) * 2.0 ** -24
+            assert abs(got[t, 2 * i].item() - math.cos(angle)) <= tol and abs(got[t, 2 * i + 1].item() - math.sin(angle)) <= tol, (pos, i)
