@@ -71,7 +71,7 @@ int sam3_seq_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, in
  * (2^32 threads: B * Hk in the tens of millions), as the calls do.
  * Key and value rows that a query does not see never enter its result, whatever they hold.
  */
-int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int64_t max_q, int64_t max_k);
+int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype);
 size_t sam3_seq_attn_fwd_workspace_bytes(int64_t Tq, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype);
 int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                       int64_t v_st, int64_t v_sh, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k, void* out,

@@ -208,7 +208,7 @@ def _declare(lib):
     lib.sam3_seq_rotary.argtypes = strided * 2 + [c_void_p] * 3 + [c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                                                    c_int64, c_int, c_int, c_int, c_int, c_void_p]
     lib.sam3_seq_attn_workgroups.restype = c_int64
-    lib.sam3_seq_attn_workgroups.argtypes = [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int64]
+    lib.sam3_seq_attn_workgroups.argtypes = [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]
     lib.sam3_seq_attn_fwd_workspace_bytes.restype = c_size_t
     lib.sam3_seq_attn_fwd_workspace_bytes.argtypes = [c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int]
     shape = [c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int, c_float, c_int]      # Tq, Tk, B, Hq, Hk, D, max_q, max_k, ...

@@ -1614,17 +1614,22 @@ Plan plan(int64_t Tq, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
     return p;
 }
 // The backward's launches.  Tiles of 32, shared by the waves of a workgroup, where tiles of 128 would be too few for the chip.  Measured on both
-// sides (us, tiles of 128 / of 32; bf16): gq at 48 tiles 63 / 25, at 128 143 / 119, at 256 51 / 77; gk and gv at 64 241 / 72, at 128 438 / 155, at
-// 256 859 / 524.
+// sides (us, tiles of 128 / of 32; causal sequences of 2048, one query head to a key head, tiles of 128 counted):
+//   gq      bf16, heads of 128   128: 76 / 52, 256: 82 / 103;    of 64   128: 39 / 25, 256: 41 / 39, 512: 56 / 75
+//           fp32, heads of 64    128: 221 / 90, 256: 227 / 174, 384: 402 / 256, 1024: 660 / 674;    of 128   64: 421 / 415, 128: 424 / 498
+//   gk, gv  bf16, heads of 128   128: 107 / 53, 256: 118 / 104, 384: 140 / 153;    of 64   256: 55 / 38, 384: 68 / 59, 512: 70 / 73
+//           fp32, heads of 64    256: 289 / 205, 512: 508 / 407, 1024: 842 / 808;    of 128   64: 521 / 433, 128: 526 / 491, 256: 530 / 969
+// Sequences of 512 change sides earlier (gk, gv of heads of 128: bf16 at 192, 50 / 56; fp32 at 64, 148 / 141).
 struct Backward {
     bool q_split, k_split;
     Grid q, k;
 };
-Backward backward_of(int64_t Tq, int64_t Tk, int B, int G, int Hk, int64_t longest_q, int64_t longest_k) {
+Backward backward_of(int64_t Tq, int64_t Tk, int B, int G, int Hk, int D, int64_t longest_q, int64_t longest_k, int dtype) {
     const int64_t pairs = (int64_t)B * Hk, rows = longest_q * G;
     Backward b;
-    b.q_split = pairs * tiles(rows, BM) <= 128 || rows <= 32;
-    b.k_split = pairs * tiles(longest_k, 128) <= 256 || longest_k <= 32;
+    const bool wide = dtype == 1 && D > 64;         // (two waves of 512 registers each share a tile then)
+    b.q_split = pairs * tiles(rows, BM) <= (wide ? 64 : 128) || rows <= 32;
+    b.k_split = pairs * tiles(longest_k, 128) <= (wide ? 96 : 256) || longest_k <= 32;
     const int qt = (int)tiles(rows, 32), kt = (int)tiles(longest_k, 32);
     b.q = b.q_split ? Grid{qt, places(B * Hk, qt), 256} : tiled(rows, Tq * G, B, Hk, BM);
     b.k = b.k_split ? Grid{kt, places(B * Hk, kt), 256} : tiled(longest_k, Tk, B, Hk, 128);
@@ -1699,9 +1704,9 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     return launched("sam3_seq_attn_fwd");
 }
 
-int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
+int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int Hq, int Hk, int D, int64_t max_q, int64_t max_k, int dtype) {
     sam3_seq_clear_error();
-    if (int rc = check(Tq, Tk, B, Hq, Hk, 8, max_q, max_k, 1.f, 0)) return rc;
+    if (int rc = check(Tq, Tk, B, Hq, Hk, D, max_q, max_k, 1.f, dtype)) return rc;
     if (kernel < 0 || kernel > 2) return sam3_seq_fail(EINVAL_, "attention: no launch %d", kernel);
     if (B == 0) max_q = max_k = 0;
     const int64_t lq = max_q < Tq ? max_q : Tq, lk = max_k < Tk ? max_k : Tk;
@@ -1710,7 +1715,7 @@ int64_t sam3_seq_attn_workgroups(int kernel, int64_t Tq, int64_t Tk, int B, int 
         const Plan p = plan(Tq, B, Hq, Hk, max_q, max_k);
         g = p.few ? Grid{p.tiles, places(B * Hk * p.splits, p.tiles), 64} : tiled(lq * (Hq / Hk), Tq * (Hq / Hk), B, Hk, BM);
     } else {
-        const Backward w = backward_of(Tq, Tk, B, Hq / Hk, Hk, lq, lk);
+        const Backward w = backward_of(Tq, Tk, B, Hq / Hk, Hk, D, lq, lk, dtype);
         g = kernel == 1 ? w.q : w.k;
     }
     return g.fits() ? g.places + REST : sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
@@ -1744,7 +1749,7 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     a.q_st = q_st; a.q_sh = q_sh; a.k_st = k_st; a.k_sh = k_sh; a.v_st = v_st; a.v_sh = v_sh; a.go_st = go_st; a.go_sh = go_sh;
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest_q = max_q < Tq ? max_q : Tq, longest_k = max_k < Tk ? max_k : Tk;
-    const Backward w = backward_of(Tq, Tk, B, a.G, Hk, longest_q, longest_k);
+    const Backward w = backward_of(Tq, Tk, B, a.G, Hk, D, longest_q, longest_k, dtype);
     if (!w.q.fits() || !w.k.fits()) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
     const bool q_one = longest_k <= 64, k_one = longest_q * a.G <= 64;      // not more than two blocks for the waves to share
     hipStream_t st = (hipStream_t)stream;

@@ -22,20 +22,28 @@ def test_launches_are_as_large_as_the_rows_ask_for(tq, tk, b, hq, hk, max_q, max
     many sequences can have, whatever is said of the longest one."""
     lib = _ffi.load()
     for kernel, rows, heads in ((0, tq * (hq // hk), hk), (1, tq * (hq // hk), hk), (2, tk, hk)):
-        n = lib.sam3_seq_attn_workgroups(kernel, tq, tk, b, hq, hk, max_q, max_k)
+        n = lib.sam3_seq_attn_workgroups(kernel, tq, tk, b, hq, hk, 64, max_q, max_k, 0)
         most = heads * (rows // 128 + b)
         assert 0 < n < (1 << 32) // 256
         assert n <= 4 * most + 16384, (kernel, n, most)         # (chunks of keys: up to 8192 more)
 
 
+def test_the_backwards_tiles_follow_the_type_and_the_head():
+    """Eight pairs of 2048 (128 tiles of 128 rows or keys): tiles of 32, but for heads over 64 in fp32, where 128 are many enough."""
+    f = _ffi.load().sam3_seq_attn_workgroups
+    for d, dtype, wide in ((64, 0, False), (128, 0, False), (64, 1, False), (72, 1, True), (128, 1, True)):
+        for kernel in (1, 2):
+            assert f(kernel, 2048, 2048, 1, 8, 8, d, 2048, 2048, dtype) - f(kernel, 2048, 2048, 1, 8, 8, d, 0, 0, dtype) == 8 * ((16 if wide else 64) - 1)
+
+
 def test_launches_that_do_not_exist_are_refused():
     import ctypes
     lib, p = _ffi.load(), ctypes.c_void_p(64)
-    assert lib.sam3_seq_attn_workgroups(3, 8, 8, 1, 2, 2, 8, 8) == -22
-    assert lib.sam3_seq_attn_workgroups(0, 8, 8, 1, 3, 2, 8, 8) == -22
+    assert lib.sam3_seq_attn_workgroups(3, 8, 8, 1, 2, 2, 64, 8, 8, 0) == -22
+    assert lib.sam3_seq_attn_workgroups(0, 8, 8, 1, 3, 2, 64, 8, 8, 0) == -22
     # 65000 sequences of 1024 key heads: 66.6 million workgroups
     for kernel in range(3):
-        assert lib.sam3_seq_attn_workgroups(kernel, 130000, 130000, 65000, 1024, 1024, 130000, 130000) == -95
+        assert lib.sam3_seq_attn_workgroups(kernel, 130000, 130000, 65000, 1024, 1024, 8, 130000, 130000, 0) == -95
     assert lib.sam3_seq_attn_fwd(p, 8192, 8, p, 8192, 8, p, 8192, 8, p, p, None, p, None, None, 130000, 130000, 65000, 1024, 1024, 8, 130000, 130000, 1, 0.1, 0,
                                  None, 0, None) == -95
     assert lib.sam3_seq_attn_bwd(*([p, 8192, 8] * 4), p, p, p, p, p, p, p, 130000, 130000, 65000, 1024, 1024, 8, 130000, 130000, 1, 0.1, 0, p, 1 << 40, None) == -95
@@ -78,7 +86,7 @@ def test_very_many_sequences_without_hints(lens, hq, hk, d, causal, dtype):
     lib = _ffi.load()
     pairs, tiles = len(lens) * hk, tq * (hq // hk) // 128
     for kernel in range(3):
-        assert lib.sam3_seq_attn_workgroups(kernel, tq, tq, len(lens), hq, hk, tq, tq) < pairs * tiles / 4
+        assert lib.sam3_seq_attn_workgroups(kernel, tq, tq, len(lens), hq, hk, d, tq, tq, 0) < pairs * tiles / 4
     cu = ends(lens) + 5
     leaves = [t.to("cuda", dtype).requires_grad_(True) for t in (q, k, v)]
     out, lse = sequence.packed_attention(*leaves, cu, causal=causal, return_lse=True)
