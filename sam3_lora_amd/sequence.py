@@ -16,7 +16,9 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import operator
 from functools import lru_cache
+from numbers import Integral
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -326,7 +328,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     if q.shape[-2] == 0 or (k is not None and k.shape[-2] == 0):
         raise ValueError("q and k must have heads")
     if type(sections) is not tuple:
-        sections = tuple(int(n) for n in sections)
+        sections = tuple(operator.index(n) for n in sections)
     table = _rotation_table(sections, float(theta), spectrum, q.shape[-1])
     if pairing not in ("adjacent", "halves"):
         raise ValueError(f"pairing must be 'adjacent' or 'halves', got {pairing!r}")
@@ -455,9 +457,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     if len_k is not None:
         _index("len_k", len_k, n - 1, q.device)
     for name, m in (("max_q", max_q), ("max_k", max_k)):
-        if m is not None and not (isinstance(m, int) and 0 <= m < 2 ** 31):
+        if m is not None and not ((type(m) is int or isinstance(m, Integral)) and 0 <= m < 2 ** 31):
             raise ValueError(f"{name} must be a length, got {m}")
-    max_q, max_k = tq if max_q is None else min(max_q, tq), tk if max_k is None else min(max_k, tk)
+    max_q, max_k = tq if max_q is None else min(int(max_q), tq), tk if max_k is None else min(int(max_k), tk)
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")

@@ -393,3 +393,77 @@ def test_angles_of_far_positions_against_fifty_digits():
             angle = 2 * math.pi * float(turns - turns.to_integral_value())
             tol = 2 * math.pi * 2.0 ** -24 * max(1.0, abs(pos) / 2.0 ** 30) + (math.pi / 2 + 4) * 2.0 ** -24
             assert abs(got[t, 2 * i].item() - math.cos(angle)) <= tol and abs(got[t, 2 * i + 1].item() - math.sin(angle)) <= tol, (pos, i)
+
+
+# ------------------------------------------------------------------------------------------------ sizes as programs have them
+@pytest.mark.gpu
+def test_lengths_and_sections_of_other_integer_types():
+    """Lengths as numpy's reductions give them are lengths; sections that are not whole numbers are refused, not cut off."""
+    import numpy as np
+    g = gen(8)
+    lens = np.array([5, 40, 9])
+    q, k, v = (torch.randn(54, 2, 32, generator=g).cuda() for _ in range(3))
+    cu = ends(lens.tolist())
+    want = sequence.packed_attention(q, k, v, cu, max_q=40, max_k=40)
+    for m in (lens.max(), np.int32(40), np.uint16(40)):
+        assert torch.equal(sequence.packed_attention(q, k, v, cu, max_q=m, max_k=m), want)
+    for m in (40.0, np.float32(40), -np.int64(1), torch.tensor(40), "40"):
+        with pytest.raises(ValueError, match="length"):
+            sequence.packed_attention(q, k, v, cu, max_q=m)
+    pos = torch.arange(54, device="cuda")[None].expand(2, 54)
+    turned = sequence.rotary_axes(q, None, pos, (8, 4))
+    assert torch.equal(sequence.rotary_axes(q, None, pos, np.array([8, 4])), turned) and torch.equal(sequence.rotary_axes(q, None, pos, [8, 4]), turned)
+    for sections in ([8.7, 4], (8.7, 4), [torch.tensor(8.0), 4]):
+        with pytest.raises(TypeError):
+            sequence.rotary_axes(q, None, pos, sections)
+
+
+# ------------------------------------------------------------------------------------------------------ captured calls
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["many", "few"])
+def test_a_captured_call_follows_the_bounds_of_each_replay(kind):
+    """Without hints (tiles listed by the bounds), and one token each over chunks of keys: the lengths lie on the GPU, and a replay takes those that
+    lie there then; two graphs of the same call in turn with eager work between."""
+    g = gen(9)
+    rng = torch.Generator().manual_seed(5)
+    b, tq, tk, hq, hk = (700, 3000, 3000, 2, 1) if kind == "many" else (3, 3, 9000, 4, 2)
+    q, go = (torch.randn(tq, hq, 64, generator=g).cuda().bfloat16() for _ in range(2))
+    k, v = (torch.randn(tk, hk, 64, generator=g).cuda().bfloat16() for _ in range(2))
+    how = {} if kind == "many" else dict(max_q=1, max_k=4000)
+
+    def bounds(total):
+        cut = torch.randint(0, total + 1, (b - 1,), generator=rng).sort().values
+        return torch.cat([torch.zeros(1, dtype=torch.long), cut, torch.tensor([total])]).int().cuda()
+
+    def call(q, k, v, cu_q, cu_k):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out, lse = sequence.packed_attention(*leaves, cu_q, cu_k, return_lse=True, **how)
+        return (out, lse) + torch.autograd.grad(out, leaves, go)
+    inputs = []
+    for _ in range(2):
+        cu = bounds(tq) if kind == "many" else ends([1] * 3)
+        inputs.append([q.clone(), k.clone(), v.clone(), cu, cu.clone() if kind == "many" else bounds(tk)])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for args in inputs:
+            call(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for args in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(*args))
+        graphs.append(graph)
+    for _ in range(4):
+        for args in inputs:
+            args[0].copy_(args[0].flip(0))
+            cu = bounds(tk)
+            args[4].copy_(cu)
+            if kind == "many":
+                args[3].copy_(cu)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, args in zip(outs, inputs):
+            assert all(torch.equal(a, c) for a, c in zip(out, call(*args)))
