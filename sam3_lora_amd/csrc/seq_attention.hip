@@ -11,11 +11,13 @@
 // next product without leaving the lane -- the sum over k runs in the order the registers hold it, and the other operand, read
 // from LDS by transposing reads, follows that order.
 //
-// Prompts are bound by the matrix cores and by what the chip may draw (it runs them at 1.75 to 2.0 GHz of 2.4): with 32 / 8 heads of 128
-// and 8192 tokens that all see each other the forward runs at 925 TF, gq at 1090 (three products) and gk, gv at 970 (four), where a
-// library product of 8192^3 runs at 1295; heads of 64 (16 of them, 4 x 5184 tokens) at 810, 910 and 910, the exponentials next to fewer
-// products.  The backward recomputes the scores in both of its kernels, seven products for the five of the formulas: one pass with sums
-// in memory would need atomics, whose order changes the result, or a second pass over 32-bit partial sums.
+// Prompts are bound by the order inside a wave: scores, maximum, exponentials and the second product follow each other, and the two or three
+// waves of a SIMD do not cover the waits.  By counters (with 32 / 8 heads of 128 and 8192 tokens that all see each other; heads of 64: 16, 4 x 5184
+// tokens) the matrix cores are busy 47, 61 and 52 % of the cycles in the forward, gq and gk, gv (64: 38, 47 and 47 %), vector units 7 to 17 %,
+// LDS 20 to 39 % without bank conflicts, at 1.6 to 1.9 GHz of 2.4: no unit is full.  The forward runs at 1000 TF, gq at 1160 (three products) and
+// gk, gv at 1155 (four), where a library product of 8192^3 runs at 1295; heads of 64 at 825, 965 and 1000.  The backward recomputes the
+// scores in both of its kernels, seven products for the five of the formulas: one pass with sums in memory would need atomics, whose order
+// changes the result, or a second pass over 32-bit partial sums.
 #include "seq_common.inc"
 
 #include <type_traits>
@@ -473,7 +475,7 @@ struct FwdState {
     }
 };
 
-// (three waves share a SIMD's registers up to heads of 128 bytes: 4 x 5184, heads of 64: 707 -> 674 us)
+// (three waves share a SIMD's registers up to heads of 128 bytes: 4 x 5184, heads of 64: 599 -> 545 us)
 template <typename T, int DP, bool LISTED>
 __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 128 ? 3 : 2)) void k_attn_fwd(Attn a, int tiles, unsigned first_rest) {
     typedef Tile<T, DP> L;
@@ -566,8 +568,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP > 256 ? 1 : sizeof(T) * DP <= 
 // With few rows (one new token of each request: the heads of one group) the keys are what has to be read, once, and nothing else
 // counts.  A wave is a workgroup here: it takes 32 rows and a chunk of keys in blocks of 32, with two tiles of its own that the next
 // block's loads fill while it computes (no barrier: a wave waits for its own loads), and the chunks' results meet in k_attn_join.
-// Bound by HBM: 24 requests of 1 .. 32768 keys, 8 key heads of 128 (2.03 GB) in 420 us = 4.8 TB/s, where a copy runs at 5.1.  Workgroups of 2
-// or 4 waves that join in LDS were 15 to 50 % slower on short caches (32768 keys of one request: 46 and 60 us against 40).
+// Bound by HBM: 24 requests of 1 .. 32768 keys, 8 key heads of 128 (2.03 GB) in 403 to 440 us = 4.6 to 5.0 TB/s, where a copy runs at 5.1.  Workgroups of 2
+// or 4 waves that join in LDS were 15 to 50 % slower on short caches (32768 keys of one request: 46 and 60 us against 40 of this kernel then).
 template <typename T, int DP>
 struct FewCfg {
     static constexpr int TB = 32 * DP * (int)sizeof(T), LDS = 4 * TB;
@@ -1202,7 +1204,7 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
                 step(std::false_type{}, NOW, r0);
                 r0 += BR;
             };
-            // Two steps at a time: the buffers' places are part of the instructions (heads of 128: 2335 -> 2270 us; the forward and gq gain nothing)
+            // Two steps at a time: the buffers' places are part of the instructions (heads of 128, 5 prompts of 601 .. 5184: 1339 -> 1280 us; the forward and gq gain nothing)
             int t = 0;
             for (; t + 1 < nfull; t += 2) {
                 full(std::integral_constant<int, 0>{}, t);
@@ -1588,9 +1590,9 @@ Grid tiled(int64_t longest, int64_t total, int B, int Hk, int per) {
     return places(B * Hk, each) > 4 * all + 4096 ? Grid{1 << 25, all, 256, true} : Grid{each, places(B * Hk, each), 256};
 }
 
-// The forward for few rows: rows of one token's heads or so (32 prompts' worth of short rows run 21 us in tiles of 128 and 11 in tiles of
-// 32), or where the tiles of 128 rows would leave most of the chip idle and there are keys to split: at 32 tiles over 8192 keys 195 us in
-// tiles of 128, 85 split and joined; at 128 tiles over 4096 keys 110 and 161, so not there.
+// The forward for few rows: rows of one token's heads or so (96 prompts of 2 .. 32 tokens: 19 us in tiles of 128, 11 in tiles of 32), or
+// where the tiles of 128 rows would leave most of the chip idle and there are keys to split.  In tiles of 128 / split and joined (us, heads of
+// 128): 16 tiles over 1024 keys 33 / 31, 64 over 8192 200 / 160, 128 over 8192 206 / 292, 128 over 4096 109 / 161.
 struct Plan {
     bool few;
     int tiles, splits, chunk;
@@ -1602,7 +1604,8 @@ Plan plan(int64_t Tq, int B, int Hq, int Hk, int64_t max_q, int64_t max_k) {
     if (!p.few) return p;
     p.tiles = (int)tiles(rows, 32);
     // Chunks of 256 to 1024 keys as long as that gives 1024 waves, four for each CU; longer ones for a lot of keys, where 8192 of them
-    // even out different lengths (1 .. 32768 keys of 24 requests: 378 us, with 4096 chunks 410).
+    // even out different lengths (24 requests of 1 .. 32768 keys, three draws: 437, 376 and 366 us; 4096 chunks 403, 386 and 383; 2048 486, 464
+    // and 442).
     const int64_t keys = max_k * pairs * p.tiles;
     int64_t chunk = keys / 1024 < 1024 ? keys / 1024 : 1024;
     if (chunk < 256) chunk = 256;

@@ -207,7 +207,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
 
     x, residual: [..., C] (rows may be strided), weight: [C], one type (bf16 or fp32); C a multiple of 8, at most 16384.  Returns y, or
     ``(y, h)`` with a residual: h, rounded, is the stream that the next block adds to, and its gradient joins the norm's in one pass.
-    The statistics and y come from the unrounded fp32 h.  Differentiable in x, residual and weight.
+    The statistics and y come from the unrounded fp32 h; squares that leave fp32 (elements over 1.8e19) give zeros.  Differentiable in x,
+    residual and weight.
     """
     _norm_args(x, weight, residual, eps)
     if _recorded(x, weight, residual):
@@ -425,12 +426,14 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     (cu_k None: the same rows).  They do not decrease; sequences may be empty.  Rows in front of the first and behind the last sequence
     give zeros.
     causal: the last query of a sequence sees all its keys, the one before it all but the last, and so on; False: all see all.  A query
-    that sees no key gives zeros.  One new token per request over its cache is ``cu_q = arange(B + 1)``.
+    that sees no key gives zeros.  One new token per request over its cache is ``cu_q = arange(B + 1)``, with ``max_q=1`` and ``max_k``.
     len_k: int32 [B], for caches with room behind each request: only the first ``len_k[b]`` of the rows from ``cu_k[b]`` count (without
-    gradients).  max_q, max_k: the longest lengths where the caller knows them: they size the launch (longer ones still come out right).
+    gradients).  max_q, max_k: the longest lengths where the caller knows them: they choose the kernels and size the launch (longer ones still come out
+    right; without them one token over long caches takes 1.8 times as long).
     scale: of the scores, 1 / sqrt(D) if None.  return_lse: also the logarithm of each row's sum, fp32 [Tq, Hq], without a gradient.
 
-    Keys and values that a query does not see do not enter its result, whatever they hold.  Sums and statistics are fp32; for bf16 the
+    Keys and values that a query does not see do not enter its result, whatever they hold; an infinity or NaN that it does see gives what the
+    formulas give.  Sums and statistics are fp32; for bf16 the
     probabilities are rounded to bf16 for the product with v, but for calls of few rows, where they keep 16 bits.  Gradients come out the
     same in every run.
     """
