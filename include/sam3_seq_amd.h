@@ -80,7 +80,7 @@ int sam3_seq_attn_fwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
 
 /*
  * Its gradients, each sum in a fixed order: gq [Tq, Hq, D], gk, gv [Tk, Hk, D] contiguous, from go [Tq, Hq, D] (strides as q's), out and
- * stats of the forward (contiguous) and the forward's inputs.  Rows of no sequence get zeros.  The workspace holds three fp32 for each row.
+ * stats of the forward (contiguous) and the forward's inputs.  gk and gv may both be NULL: not wanted, and not computed.  Rows of no sequence get zeros.  The workspace holds three fp32 for each row.
  */
 size_t sam3_seq_attn_bwd_workspace_bytes(int64_t Tq, int Hq);
 int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,

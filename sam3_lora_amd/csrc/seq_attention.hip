@@ -1746,7 +1746,7 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     if (Tk > 0) {
         if (int rc = check_tensor("k", k, k_st, k_sh, false, dtype)) return rc;
         if (int rc = check_tensor("v", v, v_st, v_sh, false, dtype)) return rc;
-        if (!gk || !gv || misaligned(gk) || misaligned(gv)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
+        if (!gk != !gv || misaligned(gk) || misaligned(gv)) return sam3_seq_fail(EINVAL_, "attention: null or misaligned pointer");
     }
     if (!cu_q || !cu_k) return sam3_seq_fail(EINVAL_, "attention: null pointer");
     Attn a{};
@@ -1756,7 +1756,7 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
     a.Tq = Tq; a.Tk = Tk; a.B = B; a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.causal = causal; a.scale = scale;
     const int64_t longest_q = max_q < Tq ? max_q : Tq, longest_k = max_k < Tk ? max_k : Tk;
     const Backward w = backward_of(Tq, Tk, B, a.G, Hk, D, longest_q, longest_k, dtype);
-    if (!w.q.fits() || !w.k.fits()) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
+    if (!w.q.fits() || (gk && !w.k.fits())) return sam3_seq_fail(ENOTSUP_, "attention: too many tiles of rows");
     const bool q_one = longest_k <= 64, k_one = longest_q * a.G <= 64;      // not more than two blocks for the waves to share
     hipStream_t st = (hipStream_t)stream;
     if (Tq > 0) {
@@ -1774,7 +1774,7 @@ int sam3_seq_attn_bwd(const void* q, int64_t q_st, int64_t q_sh, const void* k, 
 #undef GQ
         if (int rc = launched("sam3_seq_attn_bwd")) return rc;
     }
-    if (Tk > 0) {
+    if (Tk > 0 && gk) {
         const dim3 grid = w.k.grid();
 #define GKV(TY, W)                                                                                                                      \
     do {                                                                                                                                \

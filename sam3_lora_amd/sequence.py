@@ -394,16 +394,16 @@ class _PackedAttention(torch.autograd.Function):
             return (None,) * 10
         q, k, v, out, stats, cu_q, cu_k = ctx.saved_tensors
         go = _near(go, q.shape[1] > k.shape[1])
-        gq, gk, gv = _new(q), _new(k), _new(v)
+        need = ctx.needs_input_grad
+        gq, gk, gv = (_new(q), _new(k), _new(v)) if need[1] or need[2] else (_new(q), None, None)
         qt, qh, kt, kh, vt, vh = ctx.strides
         gs = _strides(go)
         ws = q.new_empty(ctx.nbytes, dtype=torch.uint8)
         with _on(q.device):
             _check(_ffi.load().sam3_seq_attn_bwd(
                 q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, go.data_ptr(), gs[0], gs[1], out.data_ptr(),
-                stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *ctx.shape, ws.data_ptr(),
+                stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), gq.data_ptr(), _ptr(gk), _ptr(gv), *ctx.shape, ws.data_ptr(),
                 ctx.nbytes, _stream(q.device)), "sam3_seq_attn_bwd")
-        need = ctx.needs_input_grad
         return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None) + (None,) * 7
 
 

@@ -467,3 +467,38 @@ def test_a_captured_call_follows_the_bounds_of_each_replay(kind):
         torch.cuda.synchronize()
         for out, args in zip(outs, inputs):
             assert all(torch.equal(a, c) for a, c in zip(out, call(*args)))
+
+
+# ------------------------------------------------------------------------------------------------------- partial gradients
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("times", [1, 150])
+def test_attention_gradients_one_by_one(times, dtype):
+    """Each gradient alone has the bits that it has among the others; frozen keys and values cost neither their kernel nor its tensors."""
+    g = gen(15)
+    lens = [90, 33, 0, 7] * times
+    q, go = (rand(g, sum(lens), 4, 64, dtype=dtype).to("cuda", dtype) for _ in range(2))
+    k, v = (rand(g, sum(lens), 2, 64, dtype=dtype).to("cuda", dtype) for _ in range(2))
+    cu = ends(lens)
+
+    def grads(*need):
+        leaves = [t.detach().requires_grad_(n) for t, n in zip((q, k, v), need)]
+        out = sequence.packed_attention(*leaves, cu, max_q=90, max_k=90)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(out, [t for t, n in zip(leaves, need) if n], go)
+        return got, torch.cuda.max_memory_allocated() - before
+    (gq, gk, gv), most = grads(True, True, True)
+    for need, want in (((True, False, False), (gq,)), ((False, True, False), (gk,)), ((False, False, True), (gv,)), ((True, False, True), (gq, gv)), ((False, True, True), (gk, gv))):
+        got, peak = grads(*need)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        if need == (True, False, False):
+            assert peak <= most - 2 * k.numel() * k.element_size() + 4096
+
+
+def test_gradients_of_keys_without_those_of_values_are_refused():
+    import ctypes
+    lib, p = _ffi.load(), ctypes.c_void_p(64)
+    for gk, gv in ((None, p), (p, None)):
+        assert lib.sam3_seq_attn_bwd(*([p, 64, 64] * 4), p, p, p, p, p, gk, gv, 8, 8, 1, 4, 4, 64, 8, 8, 1, 0.1, 0, p, 1 << 20, None) == -22
