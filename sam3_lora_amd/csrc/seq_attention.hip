@@ -233,29 +233,51 @@ __device__ __forceinline__ bool stage(char* lds, const T* base, int n, int D, AD
     }
     return bad;
 }
-// does a row hold an infinity or a NaN (rare path)
+// does a row hold an infinity or a NaN (rare path, as what follows: the rows are read 8 elements at a time, and no further than it takes)
 template <typename T>
 __device__ bool spoils(const T* row, int D) {
-    bool bad = false;
-    for (int d = 0; d < D; ++d) bad |= !(fabsf(ld1(row + d)) <= 3.402823466e38f);
-    return bad;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 8) {
+        Raw8<T> x;
+        float f[8], s = 0.f;
+        x.load(row + d);
+        x.get(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(f[j], 0.f, s);
+        if (s != 0.f) return true;
+    }
+    return false;
 }
-
 template <typename T>
 __device__ float dot(const T* a, const T* b, int D) {
     float s = 0.f;
 #pragma unroll 1
-    for (int d = 0; d < D; ++d) s = fmaf(ld1(a + d), ld1(b + d), s);
+    for (int d = 0; d < D; d += 8) {
+        Raw8<T> x, y;
+        float f[8], g[8];
+        x.load(a + d);
+        y.load(b + d);
+        x.get(f);
+        y.get(g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(f[j], g[j], s);
+    }
     return s;
 }
-// out += w x in memory, by a lane half's columns (store_cols()); rest: only where that is not finite, since the finite part is in it already
+// out += w x in memory, by a lane half's columns (store_cols()); rest: only where that is not finite, since the finite part is in it already.
+// Whether all of the columns are NaN now: nothing that is added later changes them.
 template <typename T>
-__device__ void add_to_row(T* out, float w, const T* x, int D, int h, bool rest) {
+__device__ bool add_to_row(T* out, float w, const T* x, int D, int h, bool rest) {
+    bool nan = true;
 #pragma unroll 1
-    for (int d = 0; d < D; ++d) {
-        const float y = w * ld1(x + d);
-        if ((d >> 2 & 1) == h && !(rest && fabsf(y) <= 3.402823466e38f)) st1(out + d, ld1(out + d) + y);
-    }
+    for (int d = 4 * h; d < D; d += 8)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float y = w * ld1(x + d + j), z = ld1(out + d + j), sum = rest && fabsf(y) <= 3.402823466e38f ? z : z + y;
+            nan &= sum != sum;
+            st1(out + d + j, sum);
+        }
+    return nan;
 }
 // Clears the rows of a staged tile that hold an infinity or a NaN: their products with the others of the tile come to nothing then.
 template <typename T, int DP, int NT>
@@ -772,8 +794,9 @@ struct GqState {
                                                float c2) const {
 #pragma unroll 1
         for (int j = first; j < end; ++j)
-            if (spoils(k + j * k_st, D))
-                add_to_row(out, __builtin_amdgcn_exp2f(fmaf(dot(q, k + j * k_st, D), c2, -base)) * (dot(go, v + j * v_st, D) - delta) * mul, k + j * k_st, D, h, false);
+            if (spoils(k + j * k_st, D) &&
+                add_to_row(out, __builtin_amdgcn_exp2f(fmaf(dot(q, k + j * k_st, D), c2, -base)) * (dot(go, v + j * v_st, D) - delta) * mul, k + j * k_st, D, h, false))
+                return;
     }
     template <bool MASK, bool SUM = false, bool FINE = false>
     __device__ __forceinline__ void step(const char* lk, const char* lv, int lane, float c2, int left) {
@@ -958,11 +981,10 @@ __device__ void add_spoilt(T* gk, T* gv, const Attn& a, const Rows& qrows, const
 #pragma unroll 1
     for (int r = first; r < end; ++r) {
         const T *q = (const T*)a.q + qrows.at(r), *go = (const T*)a.go + grows.at(r);
-        const bool of_q = spoils(q, a.D);
-        if (!of_q && !spoils(go, a.D)) continue;
+        if (!spoils(q, a.D) && !spoils(go, a.D)) continue;
         const float p = __builtin_amdgcn_exp2f(fmaf(dot(q, k, a.D), a.scale * LOG2E, -st[r])) * (sizeof(T) == 4 ? st[2 * pitch + r] : 1.f);
-        add_to_row(gv, p, go, a.D, h, true);
-        add_to_row(gk, p * (dot(go, v, a.D) - st[pitch + r]) * a.scale, q, a.D, h, false);
+        const bool all_v = add_to_row(gv, p, go, a.D, h, true), all_k = add_to_row(gk, p * (dot(go, v, a.D) - st[pitch + r]) * a.scale, q, a.D, h, false);
+        if (all_v && all_k) return;
     }
 }
 
@@ -1099,8 +1121,8 @@ struct GkvState {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                // (left alone, the compiler keeps four reloads in the loop: heads of 128, 5 prompts of 601 .. 5184: 1330 -> 1250 us)
-                if (V_LDS && !F32 && d == 0) __builtin_amdgcn_sched_barrier(0);
+                // (left alone, the compiler keeps five reloads in the loop: heads of 128, 5 prompts of 601 .. 5184: 1330 -> 1250 us)
+                if (V_LDS && !F32 && d == 1) __builtin_amdgcn_sched_barrier(0);
                 const Frag<T> gf = L::col_frag(lg, 16 * t, d, lane), qf = L::col_frag(lq, 16 * t, d, lane);
                 av[d] = mma(gf, pf[t], av[d]);
                 ak[d] = mma(qf, df[t], ak[d]);
@@ -1222,11 +1244,14 @@ __global__ __launch_bounds__(256, (GkvCfg<T, DP>::WAVES)) void k_attn_gkv(Attn a
             }
             if (__builtin_expect(odd[wave], 0)) {
                 int again = k0;
-                asm volatile("" : "+s"(again));         // (worked out again: kept, it would take registers from the loop)
+                asm volatile("" : "+s"(again));         // (all worked out again: kept, it would take registers from the loop)
                 const int head = first_row(again), full = head + (max(first_row(min(again + BK, sk.n) - 1) - head, 0) + BR - 1) / BR * BR;
                 const int tail = full < R ? R - (R - full) % BR : R;
-                add_spoilt(ok, ov, a, qrows, grows, k + key * a.k_st, v + key * a.v_st, rowstat, all, first_row(key), min(full, R), h);
-                add_spoilt(ok, ov, a, qrows, grows, k + key * a.k_st, v + key * a.v_st, rowstat, all, max(tail, first_row(key)), R, h);
+                const long long at = sk.begin + again + wave * 32 + (lane & 31);
+                const T *kr = (const T*)a.k + at * a.k_st + kv * a.k_sh, *vr = (const T*)a.v + at * a.v_st + kv * a.v_sh;
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part)
+                    add_spoilt(ok, ov, a, qrows, grows, kr, vr, rowstat, all, part ? max(tail, first_row(key)) : first_row(key), part ? R : min(full, R), h);
             }
         }
     }

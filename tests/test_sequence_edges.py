@@ -502,3 +502,23 @@ def test_gradients_of_keys_without_those_of_values_are_refused():
     lib, p = _ffi.load(), ctypes.c_void_p(64)
     for gk, gv in ((None, p), (p, None)):
         assert lib.sam3_seq_attn_bwd(*([p, 64, 64] * 4), p, p, p, p, p, gk, gv, 8, 8, 1, 4, 4, 64, 8, 8, 1, 0.1, 0, p, 1 << 20, None) == -22
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DT, ids=ids)
+@pytest.mark.parametrize("bad", ["q", "k", "v", "go", "all"])
+def test_nothing_but_nan_comes_out_as_nan(bad, dtype):
+    """A step that has diverged: whole tensors of NaN, at sizes where every block of the border holds some."""
+    g = gen(17)
+    lens = [700, 33, 260] * 20
+    t = {n: rand(g, sum(lens), h, 64, dtype=dtype).to("cuda", dtype) for n, h in (("q", 4), ("k", 2), ("v", 2), ("go", 4))}
+    for n in t:
+        if bad in (n, "all"):
+            t[n].fill_(math.nan)
+    cu = ends(lens)
+    leaves = [t[n].requires_grad_(True) for n in ("q", "k", "v")]
+    out = sequence.packed_attention(*leaves, cu, max_q=700, max_k=700)
+    gq, gk, gv = torch.autograd.grad(out, leaves, t["go"])
+    assert out.isnan().all() if bad != "go" else torch.isfinite(out).all()
+    assert gq.isnan().all() and gk.isnan().all()
+    assert gv.isnan().all() if bad != "v" else torch.isfinite(gv).all()
